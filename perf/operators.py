@@ -199,7 +199,7 @@ def _handles(st):
         h["args"] = P.RopeAppendArgs(rotary_dim=case["rotary"], adjacent_pairs=case["pairs"] == "adjacent", n_positions=st["cos"].shape[0], **common)
     else:
         h["args"] = P.PagedChunkArgs(max_q_len=st["longest"], max_seq_len=st["furthest"], scale=case["head_dim"] ** -0.5, **common)
-        h["workspace"] = be.alloc_zeroed((max(1, P.paged_chunk_workspace(be, h["args"])),), np.uint8)
+        h["workspace"] = be.import_tensor(torch.zeros(max(16, P.paged_chunk_workspace(be, h["args"])), dtype=torch.uint8, device="cuda"))
     return h
 
 
