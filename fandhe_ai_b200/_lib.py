@@ -63,6 +63,26 @@ class PagedAttentionPlanC(C.Structure):
                 ("workspace_elems", C.c_uint64)]
 
 
+class RopeAppendArgsC(C.Structure):
+    """b200_rope_append_args"""
+    _fields_ = [("layout", PagedKvLayoutC), ("batch", C.c_uint64), ("rows", C.c_uint64), ("num_heads", C.c_uint64),
+                ("num_kv_heads", C.c_uint64), ("max_blocks_per_seq", C.c_uint64), ("qkv_stride", C.c_uint64),
+                ("rotary_dim", C.c_uint64), ("n_positions", C.c_uint64), ("adjacent_pairs", C.c_int32),
+                ("io_dtype", C.c_int32)]
+
+
+class PagedChunkArgsC(C.Structure):
+    """b200_paged_chunk_args"""
+    _fields_ = [("layout", PagedKvLayoutC), ("batch", C.c_uint64), ("rows", C.c_uint64), ("max_q_len", C.c_uint64),
+                ("max_seq_len", C.c_uint64), ("num_heads", C.c_uint64), ("num_kv_heads", C.c_uint64),
+                ("max_blocks_per_seq", C.c_uint64), ("q_stride", C.c_uint64), ("scale", C.c_float), ("io_dtype", C.c_int32)]
+
+
+class SampleArgsC(C.Structure):
+    """b200_sample_args"""
+    _fields_ = [("rows", C.c_uint64), ("vocab", C.c_uint64), ("row_stride", C.c_uint64), ("dtype", C.c_int32)]
+
+
 class DecoderConfigC(C.Structure):
     """b200_decoder_config"""
     _fields_ = [("n_layers", C.c_int32), ("d_model", C.c_int32), ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32),
@@ -102,6 +122,17 @@ SIGNATURES = {
     "b200_release": (_I32, [_P, _P]),
     "b200_buf_bytes": (_SZ, [_P]),
     "b200_buf_device_ptr": (_P, [_P]),
+    "b200_buf_import": (_I32, [_P, _P, _SZ, C.POINTER(_P)]),
+    "b200_ctx_wait_stream": (_I32, [_P, _P]),
+    "b200_stream_wait_ctx": (_I32, [_P, _P]),
+    "b200_rope_table": (_I32, [C.c_double, _U64, _U64, _P, _P]),
+    "b200_validate_ragged_batch": (_I32, [_P, _P, _P, C.POINTER(PagedChunkArgsC)]),
+    "b200_validate_rope_append": (_I32, [C.POINTER(RopeAppendArgsC)]),
+    "b200_validate_sample": (_I32, [C.POINTER(SampleArgsC)]),
+    "b200_rope_paged_kv_append": (_I32, [_P, _P, _SZ, _P, _P, _P, _P, _P, _P, _P, _P, C.POINTER(RopeAppendArgsC), _P, _SZ]),
+    "b200_paged_chunk_workspace": (_I32, [_P, C.POINTER(PagedChunkArgsC), C.POINTER(_SZ)]),
+    "b200_paged_chunk_attention": (_I32, [_P, _P, _SZ, _P, _P, _P, _P, _P, C.POINTER(PagedChunkArgsC), _P, _P, _SZ]),
+    "b200_sample_tokens": (_I32, [_P, _P, _SZ, C.POINTER(SampleArgsC), _P, _P, _P, _P, _P, _P, _P, _P]),
     "b200_quantize_i8_per_row": (_I32, [_P, _P, _SZ, _I64, _I64, _P, _SZ, _P, _SZ]),
     "b200_dequantize_i8_per_row": (_I32, [_P, _P, _SZ, _P, _SZ, _I64, _I64, _P, _SZ]),
     "b200_quantize_fp8_e4m3_per_tensor": (_I32, [_P, _P, _SZ, _I64, _P, _SZ, _P, _SZ]),

@@ -44,6 +44,25 @@ class DeviceBuffer:
         return lib().b200_buf_device_ptr(self.handle) or 0
 
 
+class ImportedBuffer(DeviceBuffer):
+    """Handle for device memory that belongs to somebody else (`Backend.import_device`); `owner` is kept alive with it.
+    Releasing it (explicitly or with the object) waits for the backend's stream and frees the handle, not the memory."""
+
+    def __init__(self, backend: "Backend", handle: int, nbytes: int, shape=None, dtype=None, owner=None):
+        super().__init__(backend, handle, nbytes, shape, dtype)
+        self.owner = owner
+
+    def release(self) -> None:
+        super().release()
+        self.owner = None
+
+    def __del__(self):
+        try:
+            self.release()
+        except Exception:
+            pass
+
+
 class Backend:
     """One context per CUDA ordinal: single stream, enqueue-only ops, `download` is the sync point."""
 
@@ -78,6 +97,29 @@ class Backend:
         h = C.c_void_p()
         check(lib().b200_upload(self._ctx, a.ctypes.data_as(C.c_void_p), a.nbytes, C.byref(h)))
         return DeviceBuffer(self, h.value or 0, a.nbytes, a.shape, a.dtype)
+
+    def import_device(self, ptr: int, nbytes: int, shape=None, dtype=None, owner=None) -> ImportedBuffer:
+        """Handle for `nbytes` of device memory of another library on the same GPU (nothing is copied).  This backend
+        works on its own stream: order it against the memory's writers and readers with `wait_stream` / `stream_wait`."""
+        h = C.c_void_p()
+        check(lib().b200_buf_import(self._ctx, ptr, nbytes, C.byref(h)))
+        return ImportedBuffer(self, h.value or 0, nbytes, shape, dtype, owner)
+
+    def import_tensor(self, tensor) -> ImportedBuffer:
+        """`import_device` of a contiguous CUDA tensor (anything with torch's data_ptr / nbytes / is_contiguous)."""
+        if not tensor.is_contiguous():
+            raise ValueError("import_tensor: the tensor must be contiguous")
+        item = tensor.element_size()
+        dtype = {1: np.uint8, 2: np.uint16, 4: np.float32 if tensor.is_floating_point() else np.int32, 8: np.uint64}[item]
+        return self.import_device(tensor.data_ptr(), tensor.nbytes, tuple(tensor.shape), dtype, owner=tensor)
+
+    def wait_stream(self, cuda_stream: int) -> None:
+        """Later calls of this backend run after everything enqueued on `cuda_stream` so far."""
+        check(lib().b200_ctx_wait_stream(self._ctx, cuda_stream))
+
+    def stream_wait(self, cuda_stream: int) -> None:
+        """Later work of `cuda_stream` runs after everything this backend has enqueued so far."""
+        check(lib().b200_stream_wait_ctx(self._ctx, cuda_stream))
 
     def upload_into(self, array: np.ndarray, dst: DeviceBuffer, offset_bytes: int = 0) -> None:
         a = np.ascontiguousarray(array)

@@ -455,11 +455,67 @@ int32_t b200_release(b200_ctx* ctx, b200_buf* buf) {
     if (buf->ptr) {
         cudaSetDevice(ctx->ordinal);
         cudaStreamSynchronize(ctx->stream);
-        cudaFree(buf->ptr);
+        if (!buf->imported) cudaFree(buf->ptr);
         cudaGetLastError();
     }
     delete buf;
     return B200_OK;
+}
+
+int32_t b200_buf_import(b200_ctx* ctx, void* device_ptr, size_t bytes, b200_buf** out) {
+    if (!out) return fail(B200_INVALID_ARGUMENT, "buf_import: out is null");
+    *out = nullptr;
+    if (int32_t st = check_ctx(ctx)) return st;
+    if (bytes > 0) {
+        if (!device_ptr) return fail(B200_INVALID_ARGUMENT, "buf_import: device pointer is null");
+        if (reinterpret_cast<uintptr_t>(device_ptr) > UINTPTR_MAX - (bytes - 1)) return fail(B200_INVALID_ARGUMENT, "buf_import: range wraps around");
+        if (int32_t st = set_device(ctx)) return st;
+        // both ends of the range: device memory of this ordinal
+        for (uint8_t* p : {static_cast<uint8_t*>(device_ptr), static_cast<uint8_t*>(device_ptr) + (bytes - 1)}) {
+            cudaPointerAttributes attr;
+            const cudaError_t e = cudaPointerGetAttributes(&attr, p);
+            if (e != cudaSuccess || attr.type != cudaMemoryTypeDevice) {
+                cudaGetLastError();
+                return fail(B200_INVALID_ARGUMENT, "buf_import: not device memory");
+            }
+            if (attr.device != ctx->ordinal)
+                return fail(B200_DEVICE_MISMATCH, "buf_import: memory of device " + std::to_string(attr.device) + ", context of device " +
+                                                      std::to_string(ctx->ordinal));
+        }
+    }
+    b200_buf* b = new (std::nothrow) b200_buf();
+    if (!b) return fail(B200_DEVICE_ALLOCATION_FAILED, "host allocation of the buffer handle failed");
+    b->owner = ctx;
+    b->generation = ctx->generation;
+    b->ptr = bytes > 0 ? device_ptr : nullptr;
+    b->bytes = bytes;
+    b->imported = true;
+    *out = b;
+    return B200_OK;
+}
+
+// `after` waits on the device for everything enqueued on `before` so far
+static int32_t order_streams(b200_ctx* ctx, cudaStream_t before, cudaStream_t after, const char* what) {
+    if (int32_t st = check_ctx(ctx)) return st;
+    if (int32_t st = set_device(ctx)) return st;
+    cudaEvent_t ev = nullptr;
+    cudaError_t e = cudaEventCreateWithFlags(&ev, cudaEventDisableTiming);
+    if (e == cudaSuccess) e = cudaEventRecord(ev, before);
+    if (e == cudaSuccess) e = cudaStreamWaitEvent(after, ev, 0);
+    if (ev) cudaEventDestroy(ev);       // released by the driver once it has completed
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(B200_INVALID_ARGUMENT, std::string(what) + ": " + cudaGetErrorString(e));
+    }
+    return B200_OK;
+}
+int32_t b200_ctx_wait_stream(b200_ctx* ctx, void* stream) {
+    if (!ctx) return fail(B200_INVALID_ARGUMENT, "ctx_wait_stream: context is null");
+    return order_streams(ctx, static_cast<cudaStream_t>(stream), ctx->stream, "ctx_wait_stream");
+}
+int32_t b200_stream_wait_ctx(b200_ctx* ctx, void* stream) {
+    if (!ctx) return fail(B200_INVALID_ARGUMENT, "stream_wait_ctx: context is null");
+    return order_streams(ctx, ctx->stream, static_cast<cudaStream_t>(stream), "stream_wait_ctx");
 }
 
 size_t b200_buf_bytes(const b200_buf* buf) { return buf ? buf->bytes : 0; }

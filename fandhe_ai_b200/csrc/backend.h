@@ -43,6 +43,7 @@ struct b200_buf {
     uint64_t generation = 0;
     void* ptr = nullptr;
     size_t bytes = 0;
+    bool imported = false;              // memory of the caller (b200_buf_import): never freed here
 };
 
 namespace b200 {

@@ -59,6 +59,41 @@ bool paged_attention_can_quantize(const PagedAttnPlan& plan);
 cudaError_t paged_attention_static_scratch(int device, void** out);
 size_t paged_attention_static_scratch_capacity();
 
+// ---- paged_chunk.cu: a batch of ragged chunks.  Sequence b brings the token rows [q_starts[b], q_starts[b + 1]) and holds
+// seq_lens[b] cached tokens, the new ones last among them; rows from q_starts[batch] on belong to nobody and are left alone.
+struct RaggedShape {
+    int64_t rows;            // token rows of the activations
+    int64_t row_stride;      // elements from one activation row to the next
+    int batch, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq;
+    int max_q_len, max_seq_len;      // attention: bounds of the new and the cached tokens of a sequence
+    float scale;
+};
+struct RopeShape {
+    int rotary_dim;          // leading elements of a head that are rotated
+    int adjacent;            // pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2)
+    int64_t n_positions;     // rows of the cos / sin tables
+};
+// qkv rows [q heads | k heads | v heads] -> q_out (dense rows, the type of qkv) and the pools, q and k rotated.
+cudaError_t rope_paged_kv_append(const RaggedShape& sh, const RopeShape& rope, const void* qkv, int io_bf16, const float* cos_t,
+                                 const float* sin_t, const uint32_t* positions, const uint32_t* tables, const uint32_t* q_starts,
+                                 const uint32_t* seq_lens, void* q_out, void* k_pool, void* v_pool, int kv_bf16, int sm_count,
+                                 uint32_t* err, cudaStream_t s);
+size_t paged_chunk_workspace_bytes(const RaggedShape& sh, int io_bf16, int kv_bf16, int sm_count);
+cudaError_t paged_chunk_attention(const RaggedShape& sh, const void* q, int io_bf16, const void* k_pool, const void* v_pool, int kv_bf16,
+                                  const uint32_t* tables, const uint32_t* q_starts, const uint32_t* seq_lens, void* workspace, void* out,
+                                  int sm_count, uint32_t* err, cudaStream_t s);
+
+// ---- sample_tokens.cu
+struct SampleShape {
+    int64_t rows, row_stride;
+    int vocab;
+    int cluster, per_cta, run, shift;      // set by the launcher
+};
+cudaError_t sample_tokens(const SampleShape& shape, const void* logits, int bf16, const float* temperature, const int* top_k,
+                          const float* top_p, const float* min_p, const float* uniform, int* ids, float* prob, int* kept, int sm_count,
+                          cudaStream_t s);
+int64_t sample_tokens_max_vocab();
+
 // ---- decode_kernels.cu (one CTA per token row; `raw` = split-K planes [splits][M][N] of int32)
 cudaError_t embed_norm_quant(const int* ids, const float* table, int vocab, int M, int d, const float* norm_w, float eps,
                              float* h, int8_t* xq, float* sx, uint32_t* err, cudaStream_t s);

@@ -1,0 +1,301 @@
+// A batch of ragged chunks over the paged KV cache: the append of its keys and values with the rotary rotation on the way, and
+// the general form of its attention (paged_chunk_tc5.cuh holds the tensor-core form).
+//
+// Sequence b brings the token rows [q_starts[b], q_starts[b + 1]); it holds seq_lens[b] cached tokens of which those rows are the
+// last, so row r of it stands at position seq_lens[b] - (q_starts[b + 1] - r).  All three arrays live on the device; nothing in
+// them is trusted: an index out of range sets the error word and touches nothing.
+#include "kernels.cuh"
+#include "launch.cuh"
+#include "ptx.cuh"
+
+namespace b200 {
+namespace {
+
+// Index of the sequence that row `row` belongs to, by one pass of the whole block over q_starts (one load latency instead of the
+// log2(batch) dependent ones of a binary search): the number of starts[1..batch] that are <= row.  `batch` when it belongs to none.
+__device__ __forceinline__ int sequence_of_row(const uint32_t* __restrict__ q_starts, int batch, int64_t row) {
+    int seq = 0;
+    for (int b0 = 0; b0 < batch; b0 += blockDim.x) {
+        const int b = b0 + threadIdx.x;
+        seq += __syncthreads_count(b < batch && int64_t(q_starts[b + 1]) <= row);
+    }
+    return seq;
+}
+
+// ------------------------------------------------------------------------------------ append
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+__device__ __forceinline__ float as_f32(float v) { return v; }
+__device__ __forceinline__ float as_f32(uint16_t v) { return bf16_bits_to_f32(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ uint16_t from_f32<uint16_t>(float v) { return static_cast<uint16_t>(f32_to_bf16_bits(v)); }
+
+template <typename T, int N>
+__device__ __forceinline__ void load_f32(const T* p, float (&x)[N]) {
+    constexpr int W = sizeof(T) * N > 16 ? 16 / sizeof(T) : N;      // at most 16 bytes an access
+#pragma unroll
+    for (int g = 0; g < N; g += W) {
+        const Pack<T, W> raw = *reinterpret_cast<const Pack<T, W>*>(p + g);
+#pragma unroll
+        for (int k = 0; k < W; ++k) x[g + k] = as_f32(raw.v[k]);
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_f32(T* p, const float (&x)[N]) {
+    constexpr int W = sizeof(T) * N > 16 ? 16 / sizeof(T) : N;
+#pragma unroll
+    for (int g = 0; g < N; g += W) {
+        Pack<T, W> raw;
+#pragma unroll
+        for (int k = 0; k < W; ++k) raw.v[k] = from_f32<T>(x[g + k]);
+        *reinterpret_cast<Pack<T, W>*>(p + g) = raw;
+    }
+}
+
+// One block per token row (grid.y blocks share the heads of a row when there are few rows).  A thread's unit of work is a pair of
+// N-element groups that rotate into each other (ADJ: one group holding N / 2 pairs) or a group that is copied; N elements are 16
+// bytes of the activation type, or N = 1 (ADJ: 2) where an alignment or a size does not allow that.
+template <typename T, typename KvT, int N, bool ADJ>
+__global__ void __launch_bounds__(256)
+rope_append_kernel(RaggedShape sh, RopeShape rope, const T* __restrict__ qkv, const float* __restrict__ cos_t,
+                   const float* __restrict__ sin_t, const uint32_t* __restrict__ positions, const uint32_t* __restrict__ tables,
+                   const uint32_t* __restrict__ q_starts, const uint32_t* __restrict__ seq_lens, T* __restrict__ q_out,
+                   KvT* __restrict__ k_pool, KvT* __restrict__ v_pool, uint32_t* err) {
+    const int64_t row = blockIdx.x;
+    const int seq = sequence_of_row(q_starts, sh.batch, row);
+    if (seq >= sh.batch) return;                                        // behind the last sequence
+    const int64_t end = q_starts[seq + 1], len = seq_lens[seq];
+    const int64_t slot_pos = len - (end - row);                         // position in the cache
+    const int64_t angle_pos = positions ? int64_t(positions[row]) : slot_pos;
+    if (slot_pos < 0 || slot_pos >= int64_t(sh.max_blocks_per_seq) * sh.block_size || angle_pos < 0 || angle_pos >= rope.n_positions) {
+        if (threadIdx.x == 0) atomicCAS(err, 0u, static_cast<uint32_t>(kErrRaggedBatch));
+        return;
+    }
+    const uint32_t blk = tables[int64_t(seq) * sh.max_blocks_per_seq + slot_pos / sh.block_size];
+    if (blk >= uint32_t(sh.num_blocks)) {
+        if (threadIdx.x == 0) atomicCAS(err, 0u, static_cast<uint32_t>(kErrAppendSlot));
+        return;
+    }
+    const int d = sh.head_dim, half = rope.rotary_dim / 2;
+    const int64_t ekv = int64_t(sh.num_kv_heads) * d;
+    const int64_t slot = (int64_t(blk) * sh.block_size + slot_pos % sh.block_size) * ekv;
+    const T* src = qkv + row * sh.row_stride;
+    T* q_row = q_out + row * (int64_t(sh.num_q_heads) * d);
+    const float* c_row = cos_t + angle_pos * half;
+    const float* s_row = sin_t + angle_pos * half;
+    const int turned = ADJ ? rope.rotary_dim / N : half / N;            // units of a head that rotate
+    const int units = turned + (d - rope.rotary_dim) / N;
+    const int turning_heads = sh.num_q_heads + sh.num_kv_heads;
+    const int total = turning_heads * units + sh.num_kv_heads * (d / N);
+    for (int w = blockIdx.y * blockDim.x + threadIdx.x; w < total; w += gridDim.y * blockDim.x) {
+        if (w >= turning_heads * units) {                               // v: a copy
+            const int e = (w - turning_heads * units) * N;
+            float x[N];
+            load_f32<T, N>(src + int64_t(turning_heads) * d + e, x);
+            store_f32<KvT, N>(v_pool + slot + e, x);
+            continue;
+        }
+        const int head = w / units, unit = w % units;
+        const T* h = src + int64_t(head) * d;
+        const bool is_q = head < sh.num_q_heads;
+        auto put = [&](int e, const float (&x)[N]) {
+            if (is_q) store_f32<T, N>(q_row + int64_t(head) * d + e, x);
+            else store_f32<KvT, N>(k_pool + slot + int64_t(head - sh.num_q_heads) * d + e, x);
+        };
+        if (unit >= turned) {
+            const int e = rope.rotary_dim + (unit - turned) * N;
+            float x[N];
+            load_f32<T, N>(h + e, x);
+            put(e, x);
+        } else if constexpr (ADJ) {
+            const int e = unit * N;
+            float x[N], c[N / 2], s[N / 2], y[N];
+            load_f32<T, N>(h + e, x);
+            load_f32<float, N / 2>(c_row + e / 2, c);
+            load_f32<float, N / 2>(s_row + e / 2, s);
+#pragma unroll
+            for (int k = 0; k < N / 2; ++k) {
+                y[2 * k] = fmaf(x[2 * k], c[k], -(x[2 * k + 1] * s[k]));
+                y[2 * k + 1] = fmaf(x[2 * k + 1], c[k], x[2 * k] * s[k]);
+            }
+            put(e, y);
+        } else {
+            const int e = unit * N;
+            float a[N], b[N], c[N], s[N], ya[N], yb[N];
+            load_f32<T, N>(h + e, a);
+            load_f32<T, N>(h + e + half, b);
+            load_f32<float, N>(c_row + e, c);
+            load_f32<float, N>(s_row + e, s);
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                ya[k] = fmaf(a[k], c[k], -(b[k] * s[k]));
+                yb[k] = fmaf(b[k], c[k], a[k] * s[k]);
+            }
+            put(e, ya);
+            put(e + half, yb);
+        }
+    }
+}
+
+template <typename T, typename KvT>
+cudaError_t launch_append(const RaggedShape& sh, const RopeShape& rope, const void* qkv, const float* cos_t, const float* sin_t,
+                          const uint32_t* positions, const uint32_t* tables, const uint32_t* q_starts, const uint32_t* seq_lens, void* q_out,
+                          void* k_pool, void* v_pool, int sm_count, uint32_t* err, cudaStream_t s) {
+    constexpr int N = 16 / sizeof(T);
+    auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+    // 16-byte accesses: every group of N elements starts on such a boundary in all six arrays
+    const bool wide = aligned(qkv) && aligned(q_out) && aligned(k_pool) && aligned(v_pool) && aligned(cos_t) && aligned(sin_t) &&
+                      sh.row_stride % N == 0 && sh.head_dim % 8 == 0 && rope.rotary_dim % (2 * N) == 0;
+    const int per_row = (sh.num_q_heads + 2 * sh.num_kv_heads) * sh.head_dim / (wide ? 2 * N : 2);
+    // blocks per row: as many as keep every SM busy, each with 64 units of work at least
+    int split = 1;
+    while (split < 16 && sh.rows * split < 2 * sm_count && per_row / (2 * split) >= 64) split *= 2;
+    int threads = 256;
+    while (threads > 64 && per_row / split <= threads / 2) threads /= 2;
+    const dim3 grid(static_cast<unsigned>(sh.rows), split);
+#define B200_APPEND(NN, ADJ)                                                                                                             \
+    rope_append_kernel<T, KvT, NN, ADJ><<<grid, threads, 0, s>>>(sh, rope, static_cast<const T*>(qkv), cos_t, sin_t, positions, tables,     \
+                                                                 q_starts, seq_lens, static_cast<T*>(q_out), static_cast<KvT*>(k_pool), \
+                                                                 static_cast<KvT*>(v_pool), err)
+    if (wide) {
+        if (rope.adjacent) B200_APPEND(N, true);
+        else B200_APPEND(N, false);
+    } else if (rope.adjacent && sh.head_dim % 2 == 0 && sh.row_stride % 2 == 0) {
+        B200_APPEND(2, true);
+    } else {
+        B200_APPEND(1, false);
+    }
+#undef B200_APPEND
+    return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------------------------ attention, general form
+constexpr int kGenThreads = 128;
+constexpr int kGenMaxDimsPerLane = 8;   // head_dim <= 256
+
+// One block per (token row, query head): four warps walk the visible keys, each with its own running maximum and sum, lanes stride
+// the head; the warps are merged at the end.  Any head_dim up to 256, any block size, f32 or bf16 pools.  A key beyond a row's
+// mask is not read, so what stands there does not matter.
+template <typename T, typename KvT>
+__global__ void __launch_bounds__(kGenThreads)
+paged_chunk_generic_kernel(RaggedShape sh, const T* __restrict__ q, const KvT* __restrict__ k_pool, const KvT* __restrict__ v_pool,
+                           const uint32_t* __restrict__ tables, const uint32_t* __restrict__ q_starts,
+                           const uint32_t* __restrict__ seq_lens, T* __restrict__ out, uint32_t* err) {
+    __shared__ float red_m[4], red_l[4];
+    __shared__ float red_o[4][256];
+    const int64_t row = blockIdx.x;
+    const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int seq = sequence_of_row(q_starts, sh.batch, row);
+    if (seq >= sh.batch) return;
+    const int dh = sh.head_dim;
+    const int64_t len = seq_lens[seq], new_rows = int64_t(q_starts[seq + 1]) - int64_t(q_starts[seq]);
+    const int64_t cap = int64_t(sh.max_blocks_per_seq) * sh.block_size;
+    int64_t limit = len - (int64_t(q_starts[seq + 1]) - row) + 1;       // visible keys
+    if (len > cap || len > sh.max_seq_len || new_rows > len || new_rows > sh.max_q_len) {
+        if (threadIdx.x == 0) atomicCAS(err, 0u, static_cast<uint32_t>(kErrRaggedBatch));
+        limit = 0;
+    }
+    const int kvh = h / (sh.num_q_heads / sh.num_kv_heads);
+    const int64_t ekv = int64_t(sh.num_kv_heads) * dh;
+    const T* q_row = q + row * sh.row_stride + int64_t(h) * dh;
+    T* o_row = out + (row * sh.num_q_heads + h) * dh;
+    float qs[kGenMaxDimsPerLane], acc[kGenMaxDimsPerLane];
+#pragma unroll
+    for (int t = 0; t < kGenMaxDimsPerLane; ++t) {
+        const int d = lane + 32 * t;
+        qs[t] = d < dh ? as_f32(q_row[d]) : 0.0f;
+        acc[t] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;
+    bool bad = false;
+    for (int64_t j = warp; j < limit; j += 4) {
+        const uint32_t blk = tables[int64_t(seq) * sh.max_blocks_per_seq + j / sh.block_size];
+        if (blk >= uint32_t(sh.num_blocks)) { bad = true; break; }
+        const int64_t off = (int64_t(blk) * sh.block_size + j % sh.block_size) * ekv + int64_t(kvh) * dh;
+        float s = 0.0f;
+#pragma unroll
+        for (int t = 0; t < kGenMaxDimsPerLane; ++t) {
+            const int d = lane + 32 * t;
+            if (d < dh) s = fmaf(qs[t], as_f32(k_pool[off + d]), s);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        s *= sh.scale;
+        const float m_new = fmaxf(m, s);
+        const float base = m_new == -INFINITY ? 0.0f : m_new;
+        const float corr = expf(m - base), p = expf(s - base);
+        l = fmaf(l, corr, p);
+#pragma unroll
+        for (int t = 0; t < kGenMaxDimsPerLane; ++t) {
+            const int d = lane + 32 * t;
+            if (d < dh) acc[t] = fmaf(p, as_f32(v_pool[off + d]), acc[t] * corr);
+        }
+        m = m_new;
+    }
+    if (lane == 0) { red_m[warp] = m; red_l[warp] = l; }
+#pragma unroll
+    for (int t = 0; t < kGenMaxDimsPerLane; ++t) {
+        const int d = lane + 32 * t;
+        if (d < dh) red_o[warp][d] = acc[t];
+    }
+    const int any_bad = __syncthreads_or(bad ? 1 : 0);
+    if (any_bad) {
+        if (threadIdx.x == 0) atomicCAS(err, 0u, static_cast<uint32_t>(kErrAttnBlockId));
+        for (int d = threadIdx.x; d < dh; d += kGenThreads) o_row[d] = from_f32<T>(__int_as_float(0x7FC00000));
+        return;
+    }
+    const float mm = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+    float w[4], ll = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        w[t] = red_m[t] == -INFINITY ? 0.0f : expf(red_m[t] - mm);
+        ll = fmaf(red_l[t], w[t], ll);
+    }
+    for (int d = threadIdx.x; d < dh; d += kGenThreads) {
+        float o = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) o = fmaf(red_o[t][d], w[t], o);
+        o_row[d] = from_f32<T>(limit > 0 ? o / ll : 0.0f);
+    }
+}
+
+}  // namespace
+
+cudaError_t rope_paged_kv_append(const RaggedShape& sh, const RopeShape& rope, const void* qkv, int io_bf16, const float* cos_t,
+                                 const float* sin_t, const uint32_t* positions, const uint32_t* tables, const uint32_t* q_starts,
+                                 const uint32_t* seq_lens, void* q_out, void* k_pool, void* v_pool, int kv_bf16, int sm_count,
+                                 uint32_t* err, cudaStream_t s) {
+    if (sh.rows == 0 || sh.batch == 0) return cudaSuccess;
+    if (io_bf16)
+        return kv_bf16 ? launch_append<uint16_t, uint16_t>(sh, rope, qkv, cos_t, sin_t, positions, tables, q_starts, seq_lens, q_out, k_pool, v_pool, sm_count, err, s)
+                       : launch_append<uint16_t, float>(sh, rope, qkv, cos_t, sin_t, positions, tables, q_starts, seq_lens, q_out, k_pool, v_pool, sm_count, err, s);
+    return kv_bf16 ? launch_append<float, uint16_t>(sh, rope, qkv, cos_t, sin_t, positions, tables, q_starts, seq_lens, q_out, k_pool, v_pool, sm_count, err, s)
+                   : launch_append<float, float>(sh, rope, qkv, cos_t, sin_t, positions, tables, q_starts, seq_lens, q_out, k_pool, v_pool, sm_count, err, s);
+}
+
+size_t paged_chunk_workspace_bytes(const RaggedShape&, int, int, int) { return 0; }
+
+cudaError_t paged_chunk_attention(const RaggedShape& sh, const void* q, int io_bf16, const void* k_pool, const void* v_pool, int kv_bf16,
+                                  const uint32_t* tables, const uint32_t* q_starts, const uint32_t* seq_lens, void*, void* out, int,
+                                  uint32_t* err, cudaStream_t s) {
+    if (sh.rows == 0 || sh.batch == 0) return cudaSuccess;
+    const dim3 grid(static_cast<unsigned>(sh.rows), sh.num_q_heads);
+    auto go = [&](auto t, auto kv) {
+        using T = decltype(t);
+        using KvT = decltype(kv);
+        paged_chunk_generic_kernel<T, KvT><<<grid, kGenThreads, 0, s>>>(sh, static_cast<const T*>(q), static_cast<const KvT*>(k_pool),
+                                                                       static_cast<const KvT*>(v_pool), tables, q_starts, seq_lens,
+                                                                       static_cast<T*>(out), err);
+    };
+    if (io_bf16) { if (kv_bf16) go(uint16_t(), uint16_t()); else go(uint16_t(), 0.0f); }
+    else { if (kv_bf16) go(0.0f, uint16_t()); else go(0.0f, 0.0f); }
+    return cudaGetLastError();
+}
+
+}  // namespace b200

@@ -25,6 +25,7 @@ enum DeviceErr : uint32_t {
     kErrAttnBlockId = 0x202,    // attention met a block id >= num_blocks in a used slot
     kErrAppendSlot = 0x203,     // append met a slot >= pool rows
     kErrAttnSeqLen = 0x204,     // attention met a sequence length beyond the table width or the planned maximum
+    kErrRaggedBatch = 0x205,    // a sequence of a ragged batch brings more rows than it holds tokens or than planned, or a position is beyond the tables
     kErrPeerWait = 0x301,       // cross-GPU flag wait ran out
     kErrPeerFailed = 0x302,     // a peer GPU reported that its own wait ran out (poisoned flag)
     kErrTokenId = 0x401,        // embedding gather met an id outside the vocabulary

@@ -1,0 +1,522 @@
+// Drawing the next token of every row of logits on the device.
+//
+// For a row x[0..V) with temperature T the weight of token i is w_i = e^((x_i - max x) / T); a logit of -inf has weight
+// zero and is never kept.  Tokens are taken in the order "larger logit first, equal logits: lower index first":
+//   S1 = the first top_k of them (all for top_k <= 0),
+//   S2 = the shortest prefix of S1 whose weight reaches top_p * W(S1) (all of S1 for top_p >= 1),
+//   S3 = the tokens of S2 with w_i >= min_p (the first token always),
+// and the drawn token is the smallest index i of S3 at which the running sum over S3 in index order exceeds u * W(S3).
+//
+// Arithmetic.  A token stands next to a border of these sums in every row (neighbours in a flat row of 128k tokens are 1e-5 of
+// the sum apart), so weights are computed in f64 and held as integers, w * 2^shift rounded (vocab * 2^shift <= 2^62, so
+// no sum of a row overflows): integer sums do not depend on their order, whatever the cluster size or the scheduling.
+//
+// One cluster of C thread blocks owns a row and keeps it in its shared memory, so that the logits are read from HBM once
+// however many passes the filters take.  Selection needs no sort: tokens fall into 2048 bins of (max - x) / T (a monotone
+// function, 1/32 of a doubling of the weight per bin), the bin a border falls into is found from the counts, and only the
+// few tokens of that bin are ranked exactly.  A bin that holds more than kCandidates tokens (flat or heavily tied rows) is
+// resolved by bisection over the ordered pair (logit, index) instead.
+#include <cfloat>
+
+#include "kernels.cuh"
+#include "launch.cuh"
+#include "ptx.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kCandidates = 512;
+constexpr int kMaxCluster = 8;
+constexpr int kMaxPerCta = 49152;      // 192 KB of f32 logits per thread block
+
+struct Shared {
+    uint64_t exchange[2][kMaxCluster][4];     // [phase][source rank][value], written by the peers
+    uint64_t warp_sum[kWarps][4];
+    uint32_t hist[kBins];
+    uint32_t total[kBins];                    // the bins of the whole row
+    float cand_x[kCandidates];
+    uint32_t cand_i[kCandidates];
+    float all_x[kCandidates];
+    uint32_t all_i[kCandidates];
+    uint64_t all_w[kCandidates];
+    uint32_t scan_count[kWarps];
+    float scan_mass[kWarps];
+    uint32_t n_cand;
+    uint32_t found[4];
+    unsigned long long best;
+};
+
+__device__ __forceinline__ void st_cluster_u64(uint32_t addr, uint64_t v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int m) {
+    return static_cast<uint64_t>(__shfl_xor_sync(0xffffffffu, static_cast<unsigned long long>(v), m));
+}
+
+// f32 -> u32 with the same order (-inf smallest); -0 is made +0 first so that equal logits have equal keys
+__device__ __forceinline__ uint32_t order_key(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+// larger = earlier in the order (larger logit, then lower index)
+__device__ __forceinline__ uint64_t order_pair(float x, uint32_t i) {
+    return (static_cast<uint64_t>(order_key(x)) << 32) | (0xFFFFFFFFu - i);
+}
+
+template <typename T>
+__device__ __forceinline__ float logit_f32(T v);
+template <>
+__device__ __forceinline__ float logit_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float logit_f32<uint16_t>(uint16_t v) { return bf16_bits_to_f32(v); }
+
+struct Row {
+    float max_x, bin_scale;
+    double inv_t, scale;      // 1 / T, 2^shift
+
+    __device__ __forceinline__ int bin(float x) const {       // kBins for -inf
+        const float d = max_x - x;
+        if (d == 0.0f) return 0;
+        if (x == -INFINITY) return kBins;
+        return static_cast<int>(fminf(d * bin_scale, static_cast<float>(kBins - 1)));
+    }
+    __device__ __forceinline__ double weight_f64(float x) const {
+        return exp((static_cast<double>(x) - static_cast<double>(max_x)) * inv_t);
+    }
+    __device__ __forceinline__ uint64_t weight(float x) const { return static_cast<uint64_t>(__double2ull_rn(weight_f64(x) * scale)); }
+};
+
+// Sums (or with kMax: maxima) of N values over the cluster; `mine` receives nothing, `out` the totals, and
+// sh.exchange[phase][rank] keeps the per-block values until the phase after next.
+template <int N, bool kMax>
+__device__ __forceinline__ void cluster_reduce(Shared& sh, int& phase, uint32_t rank, uint32_t nranks, const uint64_t (&v)[N],
+                                               uint64_t (&out)[N]) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t x[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        x[k] = v[k];
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) {
+            const uint64_t o = shfl_xor_u64(x[k], m);
+            x[k] = kMax ? (o > x[k] ? o : x[k]) : x[k] + o;
+        }
+        if (lane == 0) sh.warp_sum[warp][k] = x[k];
+    }
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            x[k] = lane < kWarps ? sh.warp_sum[lane][k] : 0;
+#pragma unroll
+            for (int m = 16; m > 0; m >>= 1) {
+                const uint64_t o = shfl_xor_u64(x[k], m);
+                x[k] = kMax ? (o > x[k] ? o : x[k]) : x[k] + o;
+            }
+            if (static_cast<uint32_t>(lane) < nranks) st_cluster_u64(mapa_shared(smem_u32(&sh.exchange[phase][rank][k]), lane), x[k]);
+        }
+    }
+    cluster_sync_all();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        out[k] = 0;
+        for (uint32_t r = 0; r < nranks; ++r) {
+            const uint64_t o = sh.exchange[phase][r][k];
+            out[k] = kMax ? (o > out[k] ? o : out[k]) : out[k] + o;
+        }
+    }
+    phase ^= 1;
+}
+
+struct Cut {                 // kept: bin < bin, or bin == bin and not after (x, i)
+    int bin;
+    uint64_t pair;
+    __device__ __forceinline__ bool keeps(int b, float x, uint32_t i) const { return b < bin || (b == bin && order_pair(x, i) >= pair); }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, const T* __restrict__ logits,
+                                                                 const float* __restrict__ temperature, const int* __restrict__ top_k,
+                                                                 const float* __restrict__ top_p, const float* __restrict__ min_p,
+                                                                 const float* __restrict__ uniform, int* __restrict__ ids,
+                                                                 float* __restrict__ prob, int* __restrict__ kept) {
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
+    float* xs = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
+    const uint32_t nranks = p.cluster, rank = nranks > 1 ? cluster_ctarank() : 0;
+    const int64_t row = blockIdx.x / nranks;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int64_t first = int64_t(rank) * p.per_cta;
+    const int64_t left = int64_t(p.vocab) - first;
+    const int n = left <= 0 ? 0 : (left < p.per_cta ? int(left) : p.per_cta);
+    const T* src = logits + row * p.row_stride + first;
+    int phase = 0;
+
+    // ---- the row into shared memory; its first maximum; is there a NaN or +inf?
+    uint64_t best = 0, bad = 0;
+    auto take = [&](int i, float x) {
+        xs[i] = x;
+        if (!(x < INFINITY)) bad = 1;
+        const uint64_t pr = order_pair(x, uint32_t(first) + i);
+        if (x != -INFINITY && pr > best) best = pr;
+    };
+    constexpr int kVec = 16 / sizeof(T);
+    int done = 0;
+    if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+        done = n / kVec * kVec;
+        for (int g = tid; g < n / kVec; g += kThreads) {
+            const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(src) + g);
+            const T* v = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) take(g * kVec + k, logit_f32<T>(v[k]));
+        }
+    }
+    for (int i = done + tid; i < n; i += kThreads) take(i, logit_f32<T>(src[i]));
+    for (int b = tid; b < kBins; b += kThreads) sh.hist[b] = 0;
+    if (tid == 0) sh.n_cand = 0;
+    if (nranks > 1) cluster_sync_all();      // the peers are running: their shared memory may be written
+    const uint64_t best_bad[2] = {best, bad};
+    uint64_t top[2];
+    cluster_reduce<2, true>(sh, phase, rank, nranks, best_bad, top);
+
+    const float t = temperature ? temperature[row] : 1.0f;
+    const int k = top_k ? top_k[row] : 0;
+    const float tp = top_p ? top_p[row] : 1.0f;
+    const float mp = min_p ? min_p[row] : 0.0f;
+    const float u = uniform[row];
+    const bool valid = top[0] != 0 && top[1] == 0 && t >= 0.0f && t < INFINITY && tp == tp && mp == mp && u >= 0.0f && u < 1.0f;
+    const uint32_t best_i = 0xFFFFFFFFu - static_cast<uint32_t>(top[0]);
+    if (!valid || t == 0.0f || k == 1 || tp <= 0.0f) {      // nothing to draw from, or the first maximum is all that is kept
+        if (rank == 0 && tid == 0) {
+            ids[row] = valid ? int(best_i) : -1;
+            if (prob) prob[row] = valid ? 1.0f : 0.0f;
+            if (kept) kept[row] = valid ? 1 : 0;
+        }
+        return;
+    }
+    Row r;
+    {
+        const uint32_t key = static_cast<uint32_t>(top[0] >> 32);
+        r.max_x = __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
+        r.bin_scale = fminf(46.166241308f / t, FLT_MAX);      // 32 log2(e) / T
+        r.inv_t = 1.0 / static_cast<double>(t);
+        r.scale = static_cast<double>(1ull << p.shift);
+    }
+    const int run = p.run, lo = tid * run, hi = min(n, lo + run);
+    auto index = [&](int i) { return uint32_t(first) + i; };
+
+    // gathers the candidates of all blocks; returns their number (known not to exceed kCandidates)
+    auto gather = [&](bool weights) -> int {
+        __syncthreads();                     // every thread has added its candidates
+        const uint64_t mine[1] = {tid == 0 ? uint64_t(sh.n_cand) : 0};
+        uint64_t sum[1];
+        const int ph = phase;
+        cluster_reduce<1, false>(sh, phase, rank, nranks, mine, sum);
+        int at = 0;
+        for (uint32_t q = 0; q < nranks; ++q) {
+            const int m = int(sh.exchange[ph][q][0]);
+            for (int i = tid; i < m; i += kThreads) {
+                sh.all_x[at + i] = __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&sh.cand_x[i]), q)));
+                sh.all_i[at + i] = ld_cluster_u32(mapa_shared(smem_u32(&sh.cand_i[i]), q));
+            }
+            at += m;
+        }
+        __syncthreads();
+        if (weights)
+            for (int i = tid; i < at; i += kThreads) sh.all_w[i] = r.weight(sh.all_x[i]);
+        cluster_sync_all();                  // the peers have read this block's list: it may be refilled
+        if (tid == 0) { sh.n_cand = 0; sh.best = ~0ull; }
+        __syncthreads();
+        return at;
+    };
+    auto add_candidate = [&](float x, uint32_t i) {
+        const uint32_t at = atomicAdd(&sh.n_cand, 1u);
+        if (at < kCandidates) { sh.cand_x[at] = x; sh.cand_i[at] = i; }
+    };
+    // The last pair of bin `b` (under `under`) that belongs to the prefix in which `enough` is not reached before it, by
+    // bisection over the 64-bit order: `measure` gives a token's contribution, `base` what lies above the bin.
+    auto bisect = [&](int b, const Cut& under, bool by_weight, uint64_t base, double enough) -> uint64_t {
+        uint64_t a = 0, z = ~0ull;           // the largest pair P with measure(pairs >= P) >= enough
+        while (a < z) {
+            const uint64_t mid = a + ((z - a) >> 1) + 1;
+            uint64_t s[1] = {0}, sum[1];
+            for (int i = lo; i < hi; ++i) {
+                const float x = xs[i];
+                if (r.bin(x) == b && order_pair(x, index(i)) >= mid && under.keeps(b, x, index(i))) s[0] += by_weight ? r.weight(x) : 1ull;
+            }
+            cluster_reduce<1, false>(sh, phase, rank, nranks, s, sum);
+            if (static_cast<double>(base + sum[0]) >= enough) a = mid;
+            else z = mid - 1;
+        }
+        return a;
+    };
+
+    // ---- the bins of the row
+    for (int i = lo; i < hi; ++i) {
+        const int b = r.bin(xs[i]);
+        if (b < kBins) atomicAdd(&sh.hist[b], 1u);
+    }
+    if (nranks > 1) {
+        cluster_sync_all();
+        const int slice = kBins / int(nranks);
+        for (int b = int(rank) * slice + tid; b < int(rank + 1) * slice; b += kThreads) {
+            uint32_t s = 0;
+            for (uint32_t q = 0; q < nranks; ++q) s += ld_cluster_u32(mapa_shared(smem_u32(&sh.hist[b]), q));
+            for (uint32_t q = 0; q < nranks; ++q) st_cluster_u32(mapa_shared(smem_u32(&sh.total[b]), q), s);
+        }
+        cluster_sync_all();
+    } else {
+        __syncthreads();
+        for (int b = tid; b < kBins; b += kThreads) sh.total[b] = sh.hist[b];
+        __syncthreads();
+    }
+    // prefix over the bins: each thread owns four of them
+    constexpr int kPer = kBins / kThreads;
+    uint32_t c4[kPer], count_before;
+    float m4[kPer], mass_before;
+    uint32_t all_count = 0;
+    float all_mass = 0.0f;
+    {
+        uint32_t c = 0;
+        float m = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+            const int b = tid * kPer + q;
+            c4[q] = sh.total[b];
+            m4[q] = float(c4[q]) * exp2f(-(float(b) + 0.5f) * (1.0f / 32.0f));     // an estimate: only decides where to look
+            c += c4[q];
+            m += m4[q];
+        }
+        uint32_t cs = c;
+        float ms = m;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t cu = __shfl_up_sync(0xffffffffu, cs, o);
+            const float mu = __shfl_up_sync(0xffffffffu, ms, o);
+            if (lane >= o) { cs += cu; ms += mu; }
+        }
+        if (lane == 31) { sh.scan_count[warp] = cs; sh.scan_mass[warp] = ms; }
+        __syncthreads();
+        uint32_t cb = 0;
+        float mb = 0.0f;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) { cb += sh.scan_count[w]; mb += sh.scan_mass[w]; }
+            all_count += sh.scan_count[w];
+            all_mass += sh.scan_mass[w];
+        }
+        count_before = cb + cs - c;
+        mass_before = mb + ms - m;
+    }
+    Cut cut{kBins, 0};
+
+    // ---- top-k: the bin in which the k-th token lies, then its rank inside the bin
+    float k_mass = all_mass;
+    if (k > 0 && uint32_t(k) < all_count) {
+        uint32_t cb = count_before;
+        float mb = mass_before;
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+            if (cb < uint32_t(k) && uint32_t(k) <= cb + c4[q]) {
+                sh.found[0] = tid * kPer + q;
+                sh.found[1] = uint32_t(k) - cb;
+                sh.found[2] = __float_as_uint(mb + m4[q] * (float(uint32_t(k) - cb) / float(c4[q])));
+            }
+            cb += c4[q];
+            mb += m4[q];
+        }
+        __syncthreads();
+        const int bk = int(sh.found[0]);
+        const uint32_t want = sh.found[1];
+        k_mass = __uint_as_float(sh.found[2]);
+        cut.bin = bk;
+        if (sh.total[bk] <= kCandidates) {
+            for (int i = lo; i < hi; ++i)
+                if (r.bin(xs[i]) == bk) add_candidate(xs[i], index(i));
+            const int m = gather(false);
+            for (int i = tid; i < m; i += kThreads) {
+                const uint64_t mine = order_pair(sh.all_x[i], sh.all_i[i]);
+                uint32_t ahead = 0;
+                for (int j = 0; j < m; ++j) ahead += order_pair(sh.all_x[j], sh.all_i[j]) > mine;
+                if (ahead == want - 1) sh.best = mine;
+            }
+            __syncthreads();
+            cut.pair = sh.best;
+        } else {
+            cut.pair = bisect(bk, Cut{kBins, 0}, false, 0, double(want));
+        }
+    }
+
+    // ---- top-p: exact sums around the estimated bin until the border lies inside it, then the border inside the bin
+    if (tp < 1.0f) {
+        int blo = 0, bhi = cut.bin < kBins ? cut.bin : kBins - 1;
+        const float est = tp * k_mass;
+        if (tid == 0) sh.found[3] = uint32_t(bhi);
+        __syncthreads();
+        {
+            float mb = mass_before;
+#pragma unroll
+            for (int q = 0; q < kPer; ++q) {
+                if (mb < est && est <= mb + m4[q]) atomicMin(&sh.found[3], uint32_t(tid * kPer + q));
+                mb += m4[q];
+            }
+        }
+        __syncthreads();
+        int bp = min(int(sh.found[3]), bhi);
+        double target = 0.0;
+        uint64_t above = 0;
+        const Cut k_cut = cut;
+        for (;;) {
+            uint64_t s[3] = {0, 0, 0}, sum[3];
+            for (int i = lo; i < hi; ++i) {
+                const float x = xs[i];
+                const int b = r.bin(x);
+                if (b == kBins || !k_cut.keeps(b, x, index(i))) continue;
+                const uint64_t w = r.weight(x);
+                s[0] += w;
+                if (b < bp) s[1] += w;
+                else if (b == bp) s[2] += w;
+            }
+            cluster_reduce<3, false>(sh, phase, rank, nranks, s, sum);
+            target = double(tp) * double(sum[0]);
+            above = sum[1];
+            if (double(above) >= target && bp > blo) {               // the border lies above this bin
+                bhi = bp - 1;
+                // walk towards it by the estimated masses
+                float gap = float((double(above) - target) / r.scale);
+                int b = bhi;
+                while (b > blo) {
+                    const float est_b = float(sh.total[b]) * exp2f(-(float(b) + 0.5f) * (1.0f / 32.0f));
+                    if (gap < est_b) break;
+                    gap -= est_b;
+                    --b;
+                }
+                bp = b;
+            } else if (double(above + sum[2]) < target && bp < bhi) {  // ... below it
+                blo = bp + 1;
+                float gap = float((target - double(above + sum[2])) / r.scale);
+                int b = blo;
+                while (b < bhi) {
+                    const float est_b = float(sh.total[b]) * exp2f(-(float(b) + 0.5f) * (1.0f / 32.0f));
+                    if (gap <= est_b) break;
+                    gap -= est_b;
+                    ++b;
+                }
+                bp = b;
+            } else {
+                break;
+            }
+        }
+        cut.bin = bp;
+        if (sh.total[bp] <= kCandidates) {
+            for (int i = lo; i < hi; ++i)
+                if (r.bin(xs[i]) == bp && k_cut.keeps(bp, xs[i], index(i))) add_candidate(xs[i], index(i));
+            const int m = gather(true);
+            for (int i = tid; i < m; i += kThreads) {
+                const uint64_t mine = order_pair(sh.all_x[i], sh.all_i[i]);
+                uint64_t ahead = above;
+                for (int j = 0; j < m; ++j)
+                    if (order_pair(sh.all_x[j], sh.all_i[j]) > mine) ahead += sh.all_w[j];
+                if (double(ahead) < target) atomicMin(&sh.best, static_cast<unsigned long long>(mine));   // the last kept one
+            }
+            __syncthreads();
+            cut.pair = sh.best;
+        } else {
+            cut.pair = bisect(bp, k_cut, true, above, target);
+        }
+    }
+
+    // ---- the draw: sums of the kept weights in index order
+    uint64_t s[2] = {0, 0}, sum[2];
+    const double floor_w = double(mp) * r.scale;
+    auto kept_weight = [&](int i, uint64_t* w) -> bool {
+        const float x = xs[i];
+        const int b = r.bin(x);
+        if (b == kBins || !cut.keeps(b, x, index(i))) return false;
+        *w = r.weight(x);
+        return double(*w) >= floor_w || index(i) == best_i;
+    };
+    for (int i = lo; i < hi; ++i) {
+        uint64_t w;
+        if (kept_weight(i, &w)) { s[0] += w; s[1] += 1; }
+    }
+    const int ph = phase;
+    cluster_reduce<2, false>(sh, phase, rank, nranks, s, sum);
+    // u = 0 draws the first kept token however small its weight is, so the running sum there is that of the counts
+    const int by = u == 0.0f ? 1 : 0;
+    const double goal = double(u) * double(sum[0]);
+    uint64_t before = 0;
+    for (uint32_t q = 0; q < rank; ++q) before += sh.exchange[ph][q][by];
+    const uint64_t own_sum = sh.exchange[ph][rank][by];
+    if (double(before) <= goal && double(before + own_sum) > goal) {      // one block, and in it one thread, holds the token
+        uint64_t c = s[by];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t up = static_cast<uint64_t>(__shfl_up_sync(0xffffffffu, static_cast<unsigned long long>(c), o));
+            if (lane >= o) c += up;
+        }
+        if (lane == 31) sh.warp_sum[warp][3] = c;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) before += sh.warp_sum[w][3];
+        before += c - s[by];
+        if (double(before) <= goal && double(before + s[by]) > goal) {
+            uint64_t w = 0;
+            for (int i = lo; i < hi; ++i) {
+                if (!kept_weight(i, &w)) continue;
+                before += by ? 1 : w;
+                if (double(before) > goal) {
+                    ids[row] = int(index(i));
+                    if (prob) prob[row] = float(r.weight_f64(xs[i]) * r.scale / double(sum[0]));
+                    if (kept) kept[row] = int(sum[1]);
+                    break;
+                }
+            }
+        }
+    }
+}
+
+}  // namespace
+
+cudaError_t sample_tokens(const SampleShape& want, const void* logits, int bf16, const float* temperature, const int* top_k,
+                          const float* top_p, const float* min_p, const float* uniform, int* ids, float* prob, int* kept, int sm_count,
+                          cudaStream_t s) {
+    SampleShape p = want;
+    if (p.rows == 0) return cudaSuccess;
+    // Blocks per row: enough that 16384 logits fit one block's share (so that two blocks share an SM), and for few rows as
+    // many as there are idle SMs as long as each keeps 4096 logits.
+    int c = 1;
+    while (c < kMaxCluster && (p.vocab > int64_t(c) * 16384 || (p.rows * c * 2 <= sm_count && p.vocab >= c * 2 * 4096))) c *= 2;
+    p.cluster = c;
+    p.per_cta = (((p.vocab + c - 1) / c) + 7) / 8 * 8;
+    if (p.per_cta > kMaxPerCta) return cudaErrorInvalidValue;
+    p.run = ((p.per_cta + kThreads - 1) / kThreads) | 1;      // odd: the threads' runs start in different banks
+    int bits = 1;
+    while ((int64_t(1) << bits) < p.vocab) ++bits;
+    p.shift = 62 - bits;
+    const int smem = int(sizeof(Shared)) + p.per_cta * 4;
+    static int configured[2][64] = {};
+    const dim3 grid(static_cast<unsigned>(p.rows * c));
+    if (bf16) {
+        if (cudaError_t e = ensure_dynamic_smem(sample_tokens_kernel<uint16_t>, smem, configured[0])) return e;
+        return launch_ex(sample_tokens_kernel<uint16_t>, grid, dim3(kThreads), smem, s, c, false, p, static_cast<const uint16_t*>(logits),
+                         temperature, top_k, top_p, min_p, uniform, ids, prob, kept);
+    }
+    if (cudaError_t e = ensure_dynamic_smem(sample_tokens_kernel<float>, smem, configured[1])) return e;
+    return launch_ex(sample_tokens_kernel<float>, grid, dim3(kThreads), smem, s, c, false, p, static_cast<const float*>(logits),
+                     temperature, top_k, top_p, min_p, uniform, ids, prob, kept);
+}
+
+int64_t sample_tokens_max_vocab() { return int64_t(kMaxPerCta) * kMaxCluster; }
+
+}  // namespace b200

@@ -9,8 +9,8 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from ._lib import DecoderConfigC, check, lib
-from .backend import Backend
+from ._lib import DecoderConfigC, SampleArgsC, check, lib
+from .backend import F32, Backend, DeviceBuffer
 
 W_EMBED, W_ATTN_NORM, W_QKV, W_O, W_MLP_NORM, W_GATE_UP, W_DOWN, W_FINAL_NORM, W_LM_HEAD = range(9)
 
@@ -77,6 +77,37 @@ def sampling_weights(logits, strategy: int, k: int = 0, temperature: float = 1.0
     check(lib().b200_sampling_weights(x.ctypes.data_as(C.c_void_p), rows, vocab, strategy, k, C.c_float(temperature),
                                       out.ctypes.data_as(C.c_void_p)))
     return out
+
+
+@dataclass(frozen=True)
+class SampleArgs:
+    """b200_sample_args; the C form is built once per object."""
+    rows: int
+    vocab: int
+    row_stride: int = 0          # elements from one row to the next; 0: dense
+    dtype: int = F32
+
+    def __post_init__(self):
+        object.__setattr__(self, "_c", C.byref(SampleArgsC(self.rows, self.vocab, self.row_stride, self.dtype)))
+
+
+def validate_sample(args: SampleArgs) -> None:
+    check(lib().b200_validate_sample(args._c))
+
+
+def _handle(buf: DeviceBuffer | None):
+    return buf.handle if buf is not None else None
+
+
+def sample_tokens(be: Backend, logits: DeviceBuffer, args: SampleArgs, uniform: DeviceBuffer, ids: DeviceBuffer,
+                  temperature: DeviceBuffer | None = None, top_k: DeviceBuffer | None = None, top_p: DeviceBuffer | None = None,
+                  min_p: DeviceBuffer | None = None, prob: DeviceBuffer | None = None, kept: DeviceBuffer | None = None,
+                  logits_off: int = 0) -> DeviceBuffer:
+    """Draws one token per row of device logits under temperature, top-k, top-p and min-p (per-row device arrays, None: off)
+    from the given uniform numbers; see b200_sample_tokens.  Returns `ids`."""
+    check(lib().b200_sample_tokens(be._ctx, logits.handle, logits_off, args._c, _handle(temperature), _handle(top_k),
+                                   _handle(top_p), _handle(min_p), uniform.handle, ids.handle, _handle(prob), _handle(kept)))
+    return ids
 
 
 @dataclass

@@ -13,7 +13,8 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from ._lib import PagedAttentionArgsC, PagedAttentionPlanC, PagedKvLayoutC, check, lib
+from ._lib import (PagedAttentionArgsC, PagedAttentionPlanC, PagedChunkArgsC, PagedKvLayoutC, RopeAppendArgsC, check,
+                   lib)
 from .backend import BF16, F32, Backend, DeviceBuffer
 
 SENTINEL = 0xFFFFFFFF  # unused block-table slot
@@ -150,3 +151,99 @@ def paged_attention_forward_noalloc(be: Backend, q: DeviceBuffer, k_pool: Device
 
 def paged_attention_tuning(be: Backend, chunk_blocks: int = 0) -> None:
     check(lib().b200_paged_attention_tuning(be._ctx, chunk_blocks))
+
+
+# ------------------------------------------------------------------------------------------ serving step of a ragged batch
+# Sequence b brings the token rows [q_starts[b], q_starts[b + 1]) and holds seq_lens[b] cached tokens, the new ones last among
+# them; q_starts, seq_lens and the block tables are u32 buffers on the device.  See include/b200_backend.h.
+
+@dataclass(frozen=True)
+class RopeAppendArgs:
+    """b200_rope_append_args; the C form is built once per object."""
+    layout: PagedKvLayout
+    batch: int
+    rows: int
+    num_heads: int
+    num_kv_heads: int
+    max_blocks_per_seq: int
+    rotary_dim: int
+    n_positions: int
+    adjacent_pairs: bool = False
+    io_dtype: int = F32
+    qkv_stride: int = 0
+
+    def __post_init__(self):
+        object.__setattr__(self, "_c", C.byref(RopeAppendArgsC(
+            self.layout.to_c(), self.batch, self.rows, self.num_heads, self.num_kv_heads, self.max_blocks_per_seq,
+            self.qkv_stride, self.rotary_dim, self.n_positions, int(self.adjacent_pairs), self.io_dtype)))
+
+
+@dataclass(frozen=True)
+class PagedChunkArgs:
+    """b200_paged_chunk_args; the C form is built once per object."""
+    layout: PagedKvLayout
+    batch: int
+    rows: int
+    max_q_len: int
+    max_seq_len: int
+    num_heads: int
+    num_kv_heads: int
+    max_blocks_per_seq: int
+    scale: float
+    io_dtype: int = F32
+    q_stride: int = 0
+
+    def __post_init__(self):
+        object.__setattr__(self, "_c", C.byref(PagedChunkArgsC(
+            self.layout.to_c(), self.batch, self.rows, self.max_q_len, self.max_seq_len, self.num_heads, self.num_kv_heads,
+            self.max_blocks_per_seq, self.q_stride, self.scale, self.io_dtype)))
+
+
+def rope_table(theta: float, rotary_dim: int, n_positions: int):
+    """(cos, sin) of p * theta^(-2 i / rotary_dim) as f32 [n_positions, rotary_dim / 2], computed in f64 on the host."""
+    cos, sin = (np.empty((n_positions, rotary_dim // 2), np.float32) for _ in range(2))
+    check(lib().b200_rope_table(theta, rotary_dim, n_positions, cos.ctypes.data_as(C.c_void_p), sin.ctypes.data_as(C.c_void_p)))
+    return cos, sin
+
+
+def validate_ragged_batch(block_tables, q_starts, seq_lens, args: PagedChunkArgs) -> None:
+    """Checks host copies of the arrays against the arguments (what the kernels check on the device), or raises."""
+    t, q, s = _u32(block_tables).ravel(), _u32(q_starts).ravel(), _u32(seq_lens).ravel()
+    if t.size != args.batch * args.max_blocks_per_seq or q.size != args.batch + 1 or s.size != args.batch:
+        raise ValueError("validate_ragged_batch: array sizes differ from the arguments")
+    check(lib().b200_validate_ragged_batch(t.ctypes.data_as(C.c_void_p), q.ctypes.data_as(C.c_void_p),
+                                           s.ctypes.data_as(C.c_void_p), args._c))
+
+
+def validate_rope_append(args: RopeAppendArgs) -> None:
+    check(lib().b200_validate_rope_append(args._c))
+
+
+def rope_paged_kv_append(be: Backend, qkv: DeviceBuffer, cos_table: DeviceBuffer, sin_table: DeviceBuffer,
+                         block_tables: DeviceBuffer, q_starts: DeviceBuffer, seq_lens: DeviceBuffer, k_pool: DeviceBuffer,
+                         v_pool: DeviceBuffer, args: RopeAppendArgs, q_out: DeviceBuffer,
+                         positions: DeviceBuffer | None = None, qkv_off: int = 0, q_out_off: int = 0) -> DeviceBuffer:
+    """Appends the keys and values of a ragged batch (rows of [q | k | v]) to the paged cache, q and k rotated to their
+    positions; returns q_out, the rotated queries."""
+    check(lib().b200_rope_paged_kv_append(be._ctx, qkv.handle, qkv_off, cos_table.handle, sin_table.handle,
+                                          positions.handle if positions is not None else None, block_tables.handle,
+                                          q_starts.handle, seq_lens.handle, k_pool.handle, v_pool.handle, args._c,
+                                          q_out.handle, q_out_off))
+    return q_out
+
+
+def paged_chunk_workspace(be: Backend, args: PagedChunkArgs) -> int:
+    """Bytes of workspace that `paged_chunk_attention` needs for these arguments."""
+    n = C.c_size_t()
+    check(lib().b200_paged_chunk_workspace(be._ctx, args._c, C.byref(n)))
+    return int(n.value)
+
+
+def paged_chunk_attention(be: Backend, q: DeviceBuffer, k_pool: DeviceBuffer, v_pool: DeviceBuffer, block_tables: DeviceBuffer,
+                          q_starts: DeviceBuffer, seq_lens: DeviceBuffer, args: PagedChunkArgs, workspace: DeviceBuffer | None,
+                          out: DeviceBuffer, q_off: int = 0, out_off: int = 0) -> DeviceBuffer:
+    """Attention of every new token of a ragged batch over its sequence's cached tokens up to itself."""
+    check(lib().b200_paged_chunk_attention(be._ctx, q.handle, q_off, k_pool.handle, v_pool.handle, block_tables.handle,
+                                           q_starts.handle, seq_lens.handle, args._c,
+                                           workspace.handle if workspace is not None else None, out.handle, out_off))
+    return out

@@ -18,8 +18,8 @@
  *  - Everything is enqueue-only on the context's single stream, except
  *    b200_download and b200_synchronize, which are the synchronisation points
  *    (crates/tensor-core/src/buffer.rs:61-69).
- *  - Buffers are created only by the backend and carry the generation of the
- *    context that made them; handing in a buffer of another context or generation
+ *  - Buffers are created only by the backend (b200_buf_import makes a handle for the
+ *    caller's device memory) and carry the generation of the context that made them; handing in a buffer of another context or generation
  *    is an error (B200_DEVICE_MISMATCH / B200_STALE_DEVICE_GENERATION), never UB.
  *  - There is no CPU fallback.  An unsupported request is B200_UNSUPPORTED.
  */
@@ -128,6 +128,17 @@ int32_t b200_download(b200_ctx* ctx, const b200_buf* src, size_t src_offset, voi
 int32_t b200_release(b200_ctx* ctx, b200_buf* buf);   /* Drop of DeviceBuffer (buffer.rs:40-48) */
 size_t b200_buf_bytes(const b200_buf* buf);
 void* b200_buf_device_ptr(const b200_buf* buf);
+/* A handle for device memory that belongs to the caller (another library's allocation on the same ordinal); the one
+ * exception to "buffers are created only by the backend", with no counterpart in the reference.  Both ends of the range
+ * are checked to be device memory of the context's ordinal (InvalidArgument / DeviceMismatch); the memory must stay
+ * allocated until b200_release, which waits for the context's stream and frees the handle only.  The context works on its
+ * own stream: memory that another stream has written or will read is ordered by the two calls below. */
+int32_t b200_buf_import(b200_ctx* ctx, void* device_ptr, size_t bytes, b200_buf** out);
+/* Later work of the context starts after everything enqueued on `cuda_stream` (a cudaStream_t of the same device, NULL:
+ * its legacy default stream) so far ... */
+int32_t b200_ctx_wait_stream(b200_ctx* ctx, void* cuda_stream);
+/* ... and later work of `cuda_stream` after everything the context has enqueued so far.  Neither call blocks the host. */
+int32_t b200_stream_wait_ctx(b200_ctx* ctx, void* cuda_stream);
 
 /* ------------------------------------------------------------------ quantisation API
  * Shaped after the reference's proposed QuantOps {quantize, dequantize, gemm_i8_s32_scaled}
@@ -322,6 +333,110 @@ int32_t b200_paged_attention_forward_noalloc(b200_ctx* ctx, const b200_buf* q, s
 
 /* Blocks per split of the decode-attention kernel (1..256; 0 restores the default of 32), for tuning. */
 int32_t b200_paged_attention_tuning(b200_ctx* ctx, int32_t chunk_blocks);
+
+/* ------------------------------------------------------------------ serving step of a ragged batch
+ * Continuous batching brings a different number of new tokens for every sequence: a chunk of a prompt here, one token or a few
+ * drafted ones there.  The batch is described by three u32 arrays that live on the device:
+ *   q_starts[batch + 1]  sequence b brings the token rows [q_starts[b], q_starts[b + 1]); non-decreasing, q_starts[0] = 0; a
+ *                        sequence may bring none, and the rows from q_starts[batch] up to `rows` belong to nobody: they
+ *                        are neither read nor written (a batch padded to a fixed size, as a captured graph wants it);
+ *   seq_lens[batch]      cached tokens INCLUDING the new ones, which are the last of them;
+ *   block_tables[batch, max_blocks_per_seq]   as for b200_paged_attention_forward_resident; entries behind the last used
+ *                        block are not read.
+ * The host cannot check their contents: an entry out of range (a block id >= num_blocks, a sequence longer than its table, than
+ * max_seq_len, with more rows than tokens or than max_q_len) makes the kernel set the device error word (reported by the
+ * next download / synchronize) and touch nothing out of range; that sequence's results mean nothing then.
+ * No counterpart in the reference, whose append takes host slots and whose attention one l_new for the whole batch
+ * (crates/tensor-core/src/backend_ops.rs:4709-4786).  All of these calls only enqueue on the context's stream and allocate
+ * nothing, so they can be captured into a graph. */
+
+/* cos / sin of the angles p * theta^(-2 i / rotary_dim), p < n_positions, i < rotary_dim / 2, computed in f64; host arrays
+ * [n_positions, rotary_dim / 2].  Pure host function, needs no device. */
+int32_t b200_rope_table(double theta, uint64_t rotary_dim, uint64_t n_positions, float* cos_out, float* sin_out);
+
+typedef struct b200_rope_append_args {
+    b200_paged_kv_layout layout;
+    uint64_t batch;
+    uint64_t rows;                 /* token rows of qkv and q_out, at least q_starts[batch] */
+    uint64_t num_heads;            /* query heads; a multiple of num_kv_heads */
+    uint64_t num_kv_heads;         /* divides embed_dim; head_dim = embed_dim / num_kv_heads, at most 256 */
+    uint64_t max_blocks_per_seq;
+    uint64_t qkv_stride;           /* elements from one row of qkv to the next; 0: rows are dense */
+    uint64_t rotary_dim;           /* leading elements of a q or k head that are rotated; even, 0 .. head_dim */
+    uint64_t n_positions;          /* rows of the cos / sin tables */
+    int32_t adjacent_pairs;        /* 0: element i turns with i + rotary_dim / 2 (what the decoder does); 1: 2 i with 2 i + 1 */
+    int32_t io_dtype;              /* B200_F32 or B200_BF16: type of qkv and q_out */
+} b200_rope_append_args;
+
+/* Appends the keys and values of a ragged batch to the paged cache and rotates queries and keys on the way.  A row of qkv
+ * holds the q heads, then the k heads, then the v heads (the order of B200_W_QKV).  With the pair (a, b) at the angle of the
+ * row's position: (a, b) -> (a cos - b sin, b cos + a sin), computed in f32 and rounded once to the target's type.  Keys and
+ * values go to the pool row of the token's place in the cache; q_out gets the rotated queries as dense rows
+ * [rows, num_heads * head_dim].  positions: u32 [rows] row of the cos / sin tables for each token, NULL: its place in the
+ * cache.  q_out must not overlap qkv.  Two tokens with the same cache place (a block shared by two sequences) leave either. */
+int32_t b200_rope_paged_kv_append(b200_ctx* ctx, const b200_buf* qkv, size_t qkv_off, const b200_buf* cos_table,
+                                  const b200_buf* sin_table, const b200_buf* positions, const b200_buf* block_tables,
+                                  const b200_buf* q_starts, const b200_buf* seq_lens, b200_buf* k_pool, b200_buf* v_pool,
+                                  const b200_rope_append_args* args, b200_buf* q_out, size_t q_out_off);
+
+typedef struct b200_paged_chunk_args {
+    b200_paged_kv_layout layout;
+    uint64_t batch;
+    uint64_t rows;                 /* token rows of q and out, at least q_starts[batch] */
+    uint64_t max_q_len;            /* upper bound of the new tokens of a sequence */
+    uint64_t max_seq_len;          /* upper bound of seq_lens */
+    uint64_t num_heads;
+    uint64_t num_kv_heads;
+    uint64_t max_blocks_per_seq;
+    uint64_t q_stride;             /* elements from one row of q to the next; 0: rows are dense */
+    float scale;                   /* multiplied into the scores; finite */
+    int32_t io_dtype;              /* B200_F32 or B200_BF16: type of q and out */
+} b200_paged_chunk_args;
+
+/* What the kernels check on the device, for callers that hold the arrays on the host too; also every rule on the arguments
+ * themselves.  b200_validate_rope_append and b200_validate_sample check the arguments of the other two.  Pure host functions,
+ * need no device. */
+int32_t b200_validate_ragged_batch(const uint32_t* block_tables, const uint32_t* q_starts, const uint32_t* seq_lens,
+                                   const b200_paged_chunk_args* args);
+int32_t b200_validate_rope_append(const b200_rope_append_args* args);
+
+/* Bytes of workspace that b200_paged_chunk_attention needs for these arguments (0 is possible). */
+int32_t b200_paged_chunk_workspace(b200_ctx* ctx, const b200_paged_chunk_args* args, size_t* bytes);
+
+/* Attention of every new token over its sequence's cached tokens up to and including itself (their keys and values are in the
+ * cache already): out[r, h, :] = softmax_j(scale * q_r . k_j) . v_j over j <= seq_len - new + i for the i-th new token.
+ * out is dense [rows, num_heads * head_dim].  What the cache holds beyond a token's reach does not matter, NaN and
+ * infinities included.  With io_dtype F32 the products are exact to f32 (q and the softmax weights enter the bf16 tensor
+ * cores as sums of bf16 terms); with BF16 the softmax weights are rounded to bf16 for the second product.  Accumulators,
+ * maxima and sums are f32.  The contents of the workspace need not be kept between calls; calls that may overlap (other
+ * contexts, other streams replaying a captured graph) need workspaces of their own. */
+int32_t b200_paged_chunk_attention(b200_ctx* ctx, const b200_buf* q, size_t q_off, const b200_buf* k_pool, const b200_buf* v_pool,
+                                   const b200_buf* block_tables, const b200_buf* q_starts, const b200_buf* seq_lens,
+                                   const b200_paged_chunk_args* args, b200_buf* workspace, b200_buf* out, size_t out_off);
+
+typedef struct b200_sample_args {
+    uint64_t rows;
+    uint64_t vocab;                /* 1 .. 393216 */
+    uint64_t row_stride;           /* elements from one row of logits to the next; 0: rows are dense */
+    int32_t dtype;                 /* B200_F32 or B200_BF16 */
+} b200_sample_args;
+
+int32_t b200_validate_sample(const b200_sample_args* args);
+
+/* Draws one token per row of logits on the device from given random numbers.  Per-row parameters (device arrays [rows], each
+ * may be NULL): temperature f32 (NULL: 1; 0: the first maximum), top_k i32 (NULL or <= 0: off), top_p f32 (NULL or >= 1: off),
+ * min_p f32 (NULL or <= 0: off); uniform f32 in [0, 1).  With w_i = e^((x_i - max x) / temperature), tokens ordered by falling
+ * logit and equal logits by rising index (the order of top_k_indices, crates/autodiff/src/generate/mod.rs:359-369): the
+ * first top_k of them are kept; of those the shortest prefix whose weight reaches top_p of theirs; of those the ones
+ * with w_i >= min_p; the first token always.  Drawn is the smallest kept index at which the running sum of the kept weights,
+ * in index order, exceeds uniform * their sum.  Weights are computed in f64 and summed exactly.  A logit of -inf is a masked token and
+ * never kept.  ids i32 [rows]; prob f32 [rows] (may be NULL): the drawn token's share of the kept weight; kept i32 [rows]
+ * (may be NULL): how many tokens were kept.  A row that offers nothing to draw from answers id -1, prob 0, kept 0: all
+ * logits -inf, a NaN or +inf among them, a temperature that is negative or not finite, a NaN parameter, or uniform outside
+ * [0, 1).  Pinned weights for a host generator: b200_sampling_weights. */
+int32_t b200_sample_tokens(b200_ctx* ctx, const b200_buf* logits, size_t logits_off, const b200_sample_args* args,
+                           const b200_buf* temperature, const b200_buf* top_k, const b200_buf* top_p, const b200_buf* min_p,
+                           const b200_buf* uniform, b200_buf* ids, b200_buf* prob, b200_buf* kept);
 
 /* ------------------------------------------------------------------ host page table
  * BlockTable of the reference (crates/autodiff/src/nn/paged_kv.rs:158-364), host only: blocks are
