@@ -59,6 +59,9 @@ bool paged_attention_can_quantize(const PagedAttnPlan& plan);
 cudaError_t paged_attention_static_scratch(int device, void** out);
 size_t paged_attention_static_scratch_capacity();
 
+// Tensor map of a row-major [rows, cols] bf16 array, 128-byte swizzled boxes of box_rows x box_cols (64) elements.
+bool make_bf16_rows_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box_cols, int box_rows);
+
 // ---- paged_chunk.cu: a batch of ragged chunks.  Sequence b brings the token rows [q_starts[b], q_starts[b + 1]) and holds
 // seq_lens[b] cached tokens, the new ones last among them; rows from q_starts[batch] on belong to nobody and are left alone.
 struct RaggedShape {

@@ -265,6 +265,77 @@ paged_chunk_generic_kernel(RaggedShape sh, const T* __restrict__ q, const KvT* _
     }
 }
 
+#include "paged_chunk_tc5.cuh"
+
+// What a call launches: decided from the arguments alone, so that the workspace query and the call agree.
+struct ChunkPlan {
+    bool tc5;
+    int64_t items;             // upper bound
+    int chunk_tiles, max_chunks;
+};
+
+ChunkPlan plan_chunk(const RaggedShape& sh, int io_bf16, int kv_bf16, int sm_count) {
+    ChunkPlan plan = {false, 0, 0, 1};
+    const int item = io_bf16 ? 2 : 4;
+    if (!kv_bf16 || (sh.head_dim != 64 && sh.head_dim != 128) || sh.block_size < 8 || (sh.row_stride * item) % 16 != 0 ||
+        int64_t(sh.num_blocks) * sh.block_size > 0x7FFFFFFF || sh.max_seq_len == 0)
+        return plan;
+    const int64_t group = sh.num_q_heads / sh.num_kv_heads, rows = io_bf16 ? 256 : 128;
+    const int64_t by_len = int64_t(sh.batch) * ((int64_t(sh.max_q_len) * group + rows - 1) / rows);
+    const int64_t by_rows = sh.rows * group / rows + (sh.rows < sh.batch ? sh.rows : sh.batch);
+    const int64_t units = (by_len < by_rows ? by_len : by_rows) * sh.num_kv_heads;
+    const int tiles = (sh.max_seq_len + kTcKeys - 1) / kTcKeys;
+    // Key ranges per row: the number that makes the launch shortest when an item costs its key tiles plus about three tiles of
+    // start and finish, and the items are dealt out to the SMs in equal rounds.
+    int best = 1;
+    int64_t best_cost = INT64_MAX;
+    for (int n = 1; n <= 64 && (n == 1 || tiles / n >= 2); ++n) {
+        const int per = (tiles + n - 1) / n, count = (tiles + per - 1) / per;
+        if (count > 1 && sh.rows * sh.num_q_heads * count * (sh.head_dim * 4 + 8) > (int64_t(512) << 20)) break;
+        const int64_t cost = ((units * count + sm_count - 1) / sm_count) * (per + 3);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = n;
+        }
+    }
+    plan.chunk_tiles = (tiles + best - 1) / best;
+    plan.max_chunks = (tiles + plan.chunk_tiles - 1) / plan.chunk_tiles;
+    plan.items = units * plan.max_chunks;
+    plan.tc5 = plan.items < 0x7FFFFFFF && int64_t(sh.max_q_len) * group < 0x7FFFFFFF;
+    return plan;
+}
+
+template <int D, bool F32, typename T>
+cudaError_t launch_tc5(const ChunkPlan& plan, const RaggedShape& sh, const void* q, const void* k_pool, const void* v_pool,
+                       const uint32_t* tables, const uint32_t* q_starts, const uint32_t* seq_lens, void* workspace, void* out, int sm_count,
+                       uint32_t* err, cudaStream_t s) {
+    using Cfg = TcCfg<D, F32>;
+    static int configured[64] = {};
+    if (cudaError_t e = ensure_dynamic_smem(paged_chunk_tc5_kernel<D, F32, T>, Cfg::kSmem, configured)) return e;
+    CUtensorMap map_k, map_v;
+    const int64_t pool_rows = int64_t(sh.num_blocks) * sh.block_size, ekv = int64_t(sh.num_kv_heads) * D;
+    const int box = sh.block_size < kTcKeys ? sh.block_size : kTcKeys;
+    if (!make_bf16_rows_map(&map_k, k_pool, pool_rows, ekv, 64, box) || !make_bf16_rows_map(&map_v, v_pool, pool_rows, ekv, 64, box))
+        return cudaErrorInvalidValue;
+    TcShape p;
+    p.sh = sh;
+    p.group = sh.num_q_heads / sh.num_kv_heads;
+    p.chunk_tiles = plan.chunk_tiles;
+    p.max_chunks = plan.max_chunks;
+    p.q_sign = sh.scale > 0.0f ? 1.0f : (sh.scale < 0.0f ? -1.0f : 0.0f);
+    p.scale_log2 = sh.scale == 0.0f ? 1.0f : fabsf(sh.scale) * 1.44269504088896341f;
+    float* part_o = static_cast<float*>(workspace);
+    float2* part_ml = reinterpret_cast<float2*>(part_o + (plan.max_chunks > 1 ? sh.rows * sh.num_q_heads * plan.max_chunks * D : 0));
+    const dim3 grid(static_cast<unsigned>(plan.items < sm_count ? plan.items : sm_count));
+    cudaError_t e = launch_ex(paged_chunk_tc5_kernel<D, F32, T>, grid, dim3(kTcThreads), Cfg::kSmem, s, 1, true, map_k, map_v, p,
+                              static_cast<const T*>(q), static_cast<const uint16_t*>(v_pool), tables, q_starts, seq_lens,
+                              static_cast<T*>(out), part_o, part_ml, err);
+    if (e != cudaSuccess || plan.max_chunks == 1) return e;
+    const dim3 join(static_cast<unsigned>(sh.rows), (sh.num_q_heads + 7) / 8);
+    return launch_ex(paged_chunk_join_kernel<D, T>, join, dim3(256), 0, s, 1, true, p, Cfg::kRows, q_starts, seq_lens, part_o, part_ml,
+                     static_cast<T*>(out));
+}
+
 }  // namespace
 
 cudaError_t rope_paged_kv_append(const RaggedShape& sh, const RopeShape& rope, const void* qkv, int io_bf16, const float* cos_t,
@@ -279,12 +350,23 @@ cudaError_t rope_paged_kv_append(const RaggedShape& sh, const RopeShape& rope, c
                    : launch_append<float, float>(sh, rope, qkv, cos_t, sin_t, positions, tables, q_starts, seq_lens, q_out, k_pool, v_pool, sm_count, err, s);
 }
 
-size_t paged_chunk_workspace_bytes(const RaggedShape&, int, int, int) { return 0; }
+size_t paged_chunk_workspace_bytes(const RaggedShape& sh, int io_bf16, int kv_bf16, int sm_count) {
+    const ChunkPlan plan = plan_chunk(sh, io_bf16, kv_bf16, sm_count);
+    return plan.tc5 && plan.max_chunks > 1 ? size_t(sh.rows) * sh.num_q_heads * plan.max_chunks * (sh.head_dim * 4 + 8) : 0;
+}
 
 cudaError_t paged_chunk_attention(const RaggedShape& sh, const void* q, int io_bf16, const void* k_pool, const void* v_pool, int kv_bf16,
-                                  const uint32_t* tables, const uint32_t* q_starts, const uint32_t* seq_lens, void*, void* out, int,
-                                  uint32_t* err, cudaStream_t s) {
+                                  const uint32_t* tables, const uint32_t* q_starts, const uint32_t* seq_lens, void* workspace, void* out,
+                                  int sm_count, uint32_t* err, cudaStream_t s) {
     if (sh.rows == 0 || sh.batch == 0) return cudaSuccess;
+    const ChunkPlan plan = plan_chunk(sh, io_bf16, kv_bf16, sm_count);
+    if (plan.tc5) {
+        if (sh.head_dim == 128)
+            return io_bf16 ? launch_tc5<128, false, uint16_t>(plan, sh, q, k_pool, v_pool, tables, q_starts, seq_lens, workspace, out, sm_count, err, s)
+                           : launch_tc5<128, true, float>(plan, sh, q, k_pool, v_pool, tables, q_starts, seq_lens, workspace, out, sm_count, err, s);
+        return io_bf16 ? launch_tc5<64, false, uint16_t>(plan, sh, q, k_pool, v_pool, tables, q_starts, seq_lens, workspace, out, sm_count, err, s)
+                       : launch_tc5<64, true, float>(plan, sh, q, k_pool, v_pool, tables, q_starts, seq_lens, workspace, out, sm_count, err, s);
+    }
     const dim3 grid(static_cast<unsigned>(sh.rows), sh.num_q_heads);
     auto go = [&](auto t, auto kv) {
         using T = decltype(t);

@@ -1,0 +1,687 @@
+// Attention of a batch of ragged chunks on the tensor cores (included by paged_chunk.cu): bf16 pools, head_dim 64 or 128, blocks of
+// 8 tokens or more.
+//
+// The query rows of a sequence that share a KV head - G = Hq / Hkv heads of each new token - are one list of rows r = i G + g, so
+// that a tile of 128 accumulator rows is full however few tokens a sequence brings and every K / V tile is fetched once for
+// all of them.  A work item is (sequence, KV head, tile of rows, range of key tiles of 128 keys); it runs on two accumulator
+// slots, each with its own group of four softmax warps (thread = row, so row maxima and sums need no exchange):
+//   - rows > 128: slot s holds rows [128 s, 128 s + 128) and both slots use every key tile;
+//   - rows <= 128, or f32 activations: both slots hold the same rows and share the key tiles (even / odd); their
+//     partial results are joined at the end.
+// While one slot is in its softmax, the tensor cores work for the other one.
+//
+//   S = Q K^T   tcgen05.mma, operands from shared memory (128-byte swizzle, K-major), 128 columns of tensor memory a slot
+//   P = 2^(S c - m c), c = scale log2 e; bf16, written over S
+//   O += P V    tcgen05.mma, P from tensor memory, V from shared memory as it stands in the cache (MN-major), f32 accumulator
+// The running maximum m of a row is raised only when a new score exceeds it by more than 2^8 in the weight: until then the
+// weights are merely larger than one, and O need not be rescaled.
+//
+// f32 activations: q = q1 + q2 + q3 and p = p1 + p2 as bf16 terms (exact to 24 bits and to 16 bits); K and V are bf16, so
+// the products are exact and the accumulators f32.  Three times the tensor work of the first product, twice that of the second.
+//
+// Warps: 0-7 softmax (two groups), 8 TMA producer (one box per cache block and half head through the block table), 9 MMA issue,
+// 10 cleans V (11 idles): an MMA multiplies what it must not see by zero, which does not remove NaN and infinities.  In tiles with
+// masked keys (only the last ones of a sequence; such a tile is announced to warp 10, and by warp 10 to the MMA warp) rows beyond the item's last visible key are zeroed, non-finite elements
+// of rows that some query must not see are replaced by zero, and if there were any the epilogue adds them back to the rows that do see them.
+
+constexpr int kTcSoftmaxWarps = 8;
+constexpr int kTcThreads = 32 * (kTcSoftmaxWarps + 4);
+// Registers a thread: 168 at launch (384 threads); the softmax threads hold a row of 128 scores and take 216, the other four warps
+// give theirs up: 256 x 216 + 128 x 72 = 384 x 168.
+constexpr int kTcKeys = 128;               // keys of a tile
+constexpr int kTcFlagSlots = 16;
+
+template <int D, bool F32>
+struct TcCfg {
+    static constexpr int kQTerms = F32 ? 3 : 1;
+    static constexpr int kPTerms = F32 ? 2 : 1;
+    static constexpr int kTileBytes = kTcKeys * D * 2;                       // a K or V tile
+    static constexpr int kQTileBytes = 128 * D * 2;
+    static constexpr int kQBytes = (F32 ? 3 : 2) * kQTileBytes;              // also holds the 128 D f32 exchanged by the slots
+    static constexpr int kStages = D == 128 ? (F32 ? 4 : 5) : 8;
+    static constexpr int kSmem = kQBytes + kStages * kTileBytes + 2560;
+    static constexpr int kRows = F32 ? 128 : 256;                            // rows of an item
+};
+
+struct TcShape {
+    RaggedShape sh;
+    int group, chunk_tiles, max_chunks;
+    float scale_log2;          // > 0
+    float q_sign;              // queries are multiplied by this: -1 for a negative scale, 0 for scale 0
+};
+
+struct TcItem {
+    int seq, kvh, row0, rows, chunk, nchunks;      // row0: first row of the tile in the sequence's list of rows
+    int t0, nt;                                    // key tiles [t0, t0 + nt)
+    int n, len, start;                             // new tokens, cached tokens, first token row
+    int min_limit, max_limit;                      // visible keys of the first and the last row
+    bool split;
+};
+
+// Walks the items of a launch in increasing order; all lanes of a warp together.
+template <int R, bool F32>
+struct TcWalk {
+    const TcShape& p;
+    const uint32_t* q_starts;
+    const uint32_t* seq_lens;
+    int lane, first = -32, total = 0, incl = 0, items = 0, n = 0, len = 0, start = 0;
+    int64_t base = 0;
+
+    __device__ TcWalk(const TcShape& p_, const uint32_t* a, const uint32_t* b) : p(p_), q_starts(a), seq_lens(b), lane(threadIdx.x & 31) {}
+
+    __device__ __forceinline__ int tiles_of_rows() const { return (n * p.group + R - 1) / R; }
+    __device__ __forceinline__ int chunks_of_len() const { return ((len + kTcKeys - 1) / kTcKeys + p.chunk_tiles - 1) / p.chunk_tiles; }
+
+    __device__ bool next_group(uint32_t* err) {
+        base += total;
+        first += 32;
+        if (first >= p.sh.batch) return false;
+        const int b = first + lane;
+        items = n = len = 0;
+        if (b < p.sh.batch) {
+            const int64_t s = q_starts[b], e = q_starts[b + 1], l = seq_lens[b];
+            if (e < s || e > p.sh.rows || e - s > l || e - s > p.sh.max_q_len || l > p.sh.max_seq_len) {
+                if (err) atomicCAS(err, 0u, static_cast<uint32_t>(kErrRaggedBatch));
+            } else if (e > s) {
+                n = int(e - s);
+                len = int(l);
+                start = int(s);
+                items = tiles_of_rows() * chunks_of_len() * p.sh.num_kv_heads;
+            }
+        }
+        incl = items;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        total = __shfl_sync(0xffffffffu, incl, 31);
+        return true;
+    }
+    // the item `index` (not below the last one asked for); false when there are no more.  nt = 0: nothing to do.
+    __device__ bool get(int64_t index, TcItem& it, uint32_t* err) {
+        while (index >= base + total)
+            if (!next_group(err)) return false;
+        const int local = int(index - base);
+        const uint32_t m = __ballot_sync(0xffffffffu, incl > local);
+        const int src = __ffs(m) - 1;
+        const int within = local - (__shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, items, src));
+        it.seq = first + src;
+        it.n = __shfl_sync(0xffffffffu, n, src);
+        it.len = __shfl_sync(0xffffffffu, len, src);
+        it.start = __shfl_sync(0xffffffffu, start, src);
+        const int rows_all = it.n * p.group;
+        const int nq = (rows_all + R - 1) / R;
+        it.nchunks = ((it.len + kTcKeys - 1) / kTcKeys + p.chunk_tiles - 1) / p.chunk_tiles;
+        it.kvh = within % p.sh.num_kv_heads;
+        const int rest = within / p.sh.num_kv_heads;
+        it.chunk = rest % it.nchunks;
+        const int qt = nq - 1 - rest / it.nchunks;              // the tiles that see most keys first
+        it.row0 = qt * R;
+        it.rows = min(R, rows_all - it.row0);
+        it.min_limit = it.len - it.n + it.row0 / p.group + 1;
+        it.max_limit = it.len - it.n + (it.row0 + it.rows - 1) / p.group + 1;
+        const int tiles = (it.max_limit + kTcKeys - 1) / kTcKeys;
+        it.t0 = it.chunk * p.chunk_tiles;
+        it.nt = max(0, min(tiles, it.t0 + p.chunk_tiles) - it.t0);
+        it.split = F32 || it.rows <= 128;
+        return true;
+    }
+};
+
+// Places of the tiles in the ring: K tiles run `ahead` tiles ahead of the V tiles (1, or 2 when the slots take turns).
+struct TcOrder {
+    uint32_t p0;
+    int n, ahead;
+    __device__ __forceinline__ TcOrder(uint32_t p0_, const TcItem& it) : p0(p0_), n(it.nt), ahead(min(it.split ? 2 : 1, it.nt)) {}
+    __device__ __forceinline__ uint32_t k(int t) const { return t < ahead ? p0 + t : p0 + 2 * t - ahead + 1; }
+    __device__ __forceinline__ uint32_t v(int t) const { return t < n - ahead ? p0 + ahead + 2 * t : p0 + n + t; }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// two f32 -> packed bf16, the first in the low half
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+
+// Shared-memory descriptor of an MN-major operand whose rows (one per K index) are 128 bytes of the M / N dimension, 128-byte
+// swizzled: 8-row groups along K are 1024 bytes apart, the next 64 elements along M / N start `lead` bytes further.
+__device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t smem_addr, uint32_t lead) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(lead >> 4) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+__device__ __forceinline__ void umma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+struct TcShared {
+    uint64_t full[8], empty[8], raw[8];        // raw: a V tile with masked keys has landed and is to be cleaned
+    uint64_t s_full[2], p_full[2], o_full[2], q_full;
+    uint32_t tmem;
+    uint32_t abort;                            // a softmax warp gave up waiting
+    uint32_t nonfinite[kTcFlagSlots];
+    float xm[2][128], xl[2][128];
+};
+static_assert(sizeof(TcShared) <= 2560, "");
+
+template <int D, bool F32, typename T>
+__global__ void __launch_bounds__(kTcThreads, 1)
+paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcShape p,
+                       const T* __restrict__ q, const uint16_t* __restrict__ v_pool, const uint32_t* __restrict__ tables,
+                       const uint32_t* __restrict__ q_starts, const uint32_t* __restrict__ seq_lens, T* __restrict__ out,
+                       float* __restrict__ part_o, float2* __restrict__ part_ml, uint32_t* err) {
+    using Cfg = TcCfg<D, F32>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    unsigned char* q_smem = smem;
+    unsigned char* ring = smem + Cfg::kQBytes;
+    TcShared& sh = *reinterpret_cast<TcShared*>(smem + Cfg::kQBytes + Cfg::kStages * Cfg::kTileBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t q_addr = smem_u32(q_smem), ring_addr = smem_u32(ring);
+    constexpr int kNst = Cfg::kStages;
+    constexpr int kHalves = D / 64;
+    constexpr int kHalfBytes = kTcKeys * 128;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kNst; ++i) {
+            mbar_init(smem_u32(&sh.full[i]), 1);
+            mbar_init(smem_u32(&sh.empty[i]), 1);
+            mbar_init(smem_u32(&sh.raw[i]), 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(smem_u32(&sh.s_full[s]), 1);
+            mbar_init(smem_u32(&sh.p_full[s]), 4);
+            mbar_init(smem_u32(&sh.o_full[s]), 1);
+        }
+        mbar_init(smem_u32(&sh.q_full), kTcSoftmaxWarps);
+        sh.abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 8 && lane == 0) {
+        tma_prefetch_desc(&map_k);
+        tma_prefetch_desc(&map_v);
+    }
+    // The tensor memory is taken after the wait: a block of the kernel before that has yet to take its own must not find it gone.
+    pdl_wait();
+    if (warp == 9) {
+        tmem_alloc(smem_u32(&sh.tmem), 512);
+        tmem_relinquish();
+    }
+    tc5_fence_before();
+    __syncthreads();
+    tc5_fence_after();
+    const uint32_t tmem = sh.tmem;
+    pdl_launch_dependents();
+
+    TcWalk<Cfg::kRows, F32> walk(p, q_starts, seq_lens);
+    TcItem it;
+    const int block = p.sh.block_size;
+
+    if (warp >= kTcSoftmaxWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 8) {
+        // ------------------------------------------------------------ TMA producer: lane i fetches the i-th cache block of a tile
+        uint32_t pos = 0, issued = 0, raw_last = 0, raw_phase = 0;      // per stage: its last tile went to `raw`; parity of those
+        bool ok = true;
+        const int box = min(block, kTcKeys);
+        for (int64_t index = blockIdx.x; ok && walk.get(index, it, err); index += gridDim.x) {
+            if (it.nt == 0) continue;
+            const TcOrder order(pos, it);
+            const uint32_t* table = tables + int64_t(it.seq) * p.sh.max_blocks_per_seq;
+            const int end = min(it.max_limit, (it.t0 + it.nt) * kTcKeys);
+            const int masked_from = it.min_limit / kTcKeys;
+            auto fetch = [&](const CUtensorMap& map, int t, uint32_t at, bool values) {
+                const int stage = at % kNst, k0 = (it.t0 + t) * kTcKeys;
+                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.empty[stage]), ((at / kNst) & 1) ^ 1, err, kErrProducerWait))) return false;
+                issued = at + 1;
+                const int boxes = (min(kTcKeys, end - k0) + box - 1) / box;
+                const bool masked = values && it.t0 + t >= masked_from;
+                const uint32_t bar = smem_u32(masked ? &sh.raw[stage] : &sh.full[stage]);
+                if (masked) { raw_last |= 1u << stage; raw_phase ^= 1u << stage; }
+                else raw_last &= ~(1u << stage);
+                if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box * D * 2);
+                __syncwarp();
+                if (lane < boxes) {
+                    const int key = k0 + lane * box;
+                    uint32_t blk = table[key / block];
+                    if (blk >= uint32_t(p.sh.num_blocks)) {
+                        atomicCAS(err, 0u, static_cast<uint32_t>(kErrAttnBlockId));
+                        blk = 0;
+                    }
+                    const int y = int(blk) * block + key % block;
+                    const uint32_t dst = ring_addr + stage * Cfg::kTileBytes + lane * box * 128;
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h) tma_load_2d(dst + h * kHalfBytes, &map, bar, it.kvh * D + h * 64, y);
+                }
+                return true;
+            };
+            for (int t = 0; ok && t < order.ahead; ++t) ok = fetch(map_k, t, order.k(t), false);
+            for (int t = 0; ok && t < it.nt; ++t) {
+                ok = fetch(map_v, t, order.v(t), true);
+                if (ok && t + order.ahead < it.nt) ok = fetch(map_k, t + order.ahead, order.k(t + order.ahead), false);
+            }
+            pos += 2 * it.nt;
+        }
+        if (!ok)      // the consumer is gone: let this warp's own copies land before the memory is given back
+            for (uint32_t at = issued > kNst ? issued - kNst : 0; at < issued; ++at) {
+                const uint32_t stage = at % kNst;
+                if ((raw_last >> stage) & 1) mbar_wait(smem_u32(&sh.raw[stage]), ((raw_phase >> stage) & 1) ^ 1, err, kErrProducerWait);
+                else mbar_wait(smem_u32(&sh.full[stage]), (at / kNst) & 1, err, kErrProducerWait);
+            }
+    } else if (warp == 9) {
+        // ------------------------------------------------------------ MMA issue (one thread)
+        constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((kTcKeys >> 3) << 17) | ((128 >> 4) << 24);
+        constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((D >> 3) << 17) | ((128 >> 4) << 24);
+        uint32_t pos = 0, p_phase[2] = {0, 0}, q_phase = 0;
+        bool ok = true;
+        for (int64_t index = blockIdx.x; walk.get(index, it, nullptr); index += gridDim.x) {
+            if (it.nt == 0) continue;
+            const TcOrder order(pos, it);
+            pos += 2 * it.nt;
+            if (lane == 0 && ok) {
+                const int n = it.nt;
+                ok = mbar_wait(smem_u32(&sh.q_full), q_phase & 1, err, kErrMmaWait);
+                ++q_phase;
+                tc5_fence_after();
+                auto scores = [&](int s, int t, bool last_use) {
+                    const uint32_t at = order.k(t), stage = at % kNst;
+                    if (!mbar_wait(smem_u32(&sh.full[stage]), (at / kNst) & 1, err, kErrMmaWait)) return false;
+                    tc5_fence_after();
+                    const uint32_t k_tile = ring_addr + stage * Cfg::kTileBytes;
+#pragma unroll
+                    for (int term = 0; term < Cfg::kQTerms; ++term) {
+                        const uint32_t a = q_addr + (F32 ? term : (it.split ? 0 : s)) * Cfg::kQTileBytes;
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            const uint32_t off = (kk / 4) * kHalfBytes + (kk % 4) * 32;
+                            umma_bf16_ss(tmem + s * 128, umma_desc_k128(a + off), umma_desc_k128(k_tile + off), kIdescS, term + kk > 0);
+                        }
+                    }
+                    if (last_use) tc5_commit(smem_u32(&sh.empty[stage]));
+                    tc5_commit(smem_u32(&sh.s_full[s]));
+                    return true;
+                };
+                auto values = [&](int s, int t, bool first, bool last_use, bool last) {
+                    const uint32_t at = order.v(t), stage = at % kNst;
+                    if (!mbar_wait(smem_u32(&sh.full[stage]), (at / kNst) & 1, err, kErrMmaWait)) return false;
+                    if (!mbar_wait(smem_u32(&sh.p_full[s]), p_phase[s] & 1, err, kErrMmaWait)) return false;
+                    ++p_phase[s];
+                    tc5_fence_after();
+                    const uint32_t v_tile = ring_addr + stage * Cfg::kTileBytes;
+#pragma unroll
+                    for (int term = 0; term < Cfg::kPTerms; ++term)
+#pragma unroll
+                        for (int kk = 0; kk < kTcKeys / 16; ++kk)
+                            umma_bf16_ts(tmem + 256 + s * 128, tmem + s * 128 + term * 64 + kk * 8,
+                                         umma_desc_mn128(v_tile + kk * 2048, kHalfBytes), kIdescO, !(first && term + kk == 0));
+                    if (last_use) tc5_commit(smem_u32(&sh.empty[stage]));
+                    if (last) tc5_commit(smem_u32(&sh.o_full[s]));
+                    return true;
+                };
+                if (it.split) {
+                    ok = ok && scores(0, 0, true);
+                    if (n > 1) ok = ok && scores(1, 1, true);
+                    for (int t = 0; ok && t < n; ++t) {
+                        ok = values(t & 1, t, t < 2, true, t + 2 >= n);
+                        if (ok && t + 2 < n) ok = scores(t & 1, t + 2, true);
+                    }
+                } else {
+                    ok = ok && scores(0, 0, false) && scores(1, 0, true);
+                    for (int t = 0; ok && t < n; ++t)
+                        for (int s = 0; ok && s < 2; ++s) {
+                            ok = values(s, t, t == 0, s == 1, t + 1 == n);
+                            if (ok && t + 1 < n) ok = scores(s, t + 1, s == 1);
+                        }
+                }
+            }
+            __syncwarp();
+        }
+    } else if (warp == 10) {
+        // ------------------------------------------------------------ V tiles with masked keys
+        uint32_t pos = 0, count = 0, raw_phase = 0;
+        bool ok = true;
+        for (int64_t index = blockIdx.x; ok && walk.get(index, it, nullptr); index += gridDim.x) {
+            if (it.nt == 0) continue;
+            const TcOrder order(pos, it);
+            pos += 2 * it.nt;
+            const uint32_t slot = count++ % kTcFlagSlots;
+            if (lane == 0) sh.nonfinite[slot] = 0;
+            __syncwarp();
+            const int masked_from = it.min_limit / kTcKeys;
+            for (int t = max(0, masked_from - it.t0); ok && t < it.nt; ++t) {
+                const uint32_t at = order.v(t), stage = at % kNst;
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.raw[stage]), (raw_phase >> stage) & 1, err, kErrAttnLoadWait));
+                if (!ok) break;
+                raw_phase ^= 1u << stage;
+                const int k0 = (it.t0 + t) * kTcKeys;
+                unsigned char* tile = ring + stage * Cfg::kTileBytes;
+                bool found = false;
+                // rows some query must not see, then rows nobody sees; 8 pieces of 16 bytes are a row of a half
+                const int r0 = max(0, it.min_limit - k0), r1 = min(kTcKeys, it.max_limit - k0);
+                for (int c = r0 * 8 + lane; c < kTcKeys * 8; c += 32) {
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h) {
+                        uint4* piece = reinterpret_cast<uint4*>(tile + h * kHalfBytes + c * 16);
+                        if (c >= r1 * 8) {
+                            *piece = make_uint4(0, 0, 0, 0);
+                            continue;
+                        }
+                        uint4 v = *piece;
+                        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+                        bool bad = false;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if ((w[k] & 0x7F80u) == 0x7F80u) { w[k] &= 0xFFFF0000u; bad = true; }
+                            if ((w[k] & 0x7F800000u) == 0x7F800000u) { w[k] &= 0x0000FFFFu; bad = true; }
+                        }
+                        if (bad) { *piece = v; found = true; }
+                    }
+                }
+                if (found) sh.nonfinite[slot] = 1;
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.full[stage]));
+            }
+        }
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        // ------------------------------------------------------------ softmax: group `wg` of four warps, thread = row
+        const int wg = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t lane_base = uint32_t(warp & 3) << 21;               // 32 lanes a warp, lane field in the upper half of the address
+        const uint32_t t_s = tmem + wg * 128 + lane_base, t_o = tmem + 256 + wg * 128 + lane_base;
+        const float c = p.scale_log2;
+        uint32_t s_phase = 0, o_phase = 0, count = 0;
+        bool ok = true;
+        for (int64_t index = blockIdx.x; ok && walk.get(index, it, nullptr); index += gridDim.x) {
+            if (it.nt == 0) continue;
+            const uint32_t slot = count++ % kTcFlagSlots;
+            const int r = (it.split ? 0 : wg * 128) + row;                 // row of the item
+            const bool live = r < it.rows;
+            const int list = it.row0 + r, token = list / p.group, head = it.kvh * p.group + list % p.group;
+            const int limit = live ? it.len - it.n + token + 1 : 0;
+            const int64_t out_row = (int64_t(it.start) + token) * p.sh.num_q_heads + head;
+
+            // queries into shared memory, 128-byte swizzled; a shared tile is written by both groups, half a row each
+            {
+                const T* src = q + (int64_t(it.start) + token) * p.sh.row_stride + int64_t(head) * D;
+                const int pieces = D / 8, per = it.split ? pieces / 2 : pieces;
+                unsigned char* dst = q_smem + (it.split ? 0 : wg) * Cfg::kQTileBytes;
+#pragma unroll 4
+                for (int j = 0; j < per; ++j) {
+                    const int piece = (it.split ? wg * per : 0) + j;
+                    const int at = (piece / 8) * kHalfBytes + row * 128 + (((piece % 8) ^ (row & 7)) << 4);
+                    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                    if (live) {
+                        load_f32<T, 8>(src + piece * 8, x);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) x[k] *= p.q_sign;
+                    }
+#pragma unroll
+                    for (int term = 0; term < Cfg::kQTerms; ++term) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            w[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+                            x[2 * k] -= bf16_lo(w[k]);
+                            x[2 * k + 1] -= bf16_hi(w[k]);
+                        }
+                        *reinterpret_cast<uint4*>(dst + term * Cfg::kQTileBytes + at) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                fence_proxy_async();
+                tc5_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.q_full));
+            }
+
+            float m = -INFINITY, l = 0.0f;
+            const int masked_from = it.min_limit / kTcKeys, step = it.split ? 2 : 1;
+            int done = 0;
+            for (int t = it.split ? wg : 0; t < it.nt; t += step, ++done) {
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.s_full[wg]), s_phase & 1, err, kErrEpilogueWait));
+                if (!ok) break;
+                ++s_phase;
+                tc5_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) tmem_ld_32x32(t_s + g * 32, s[g]);
+                tmem_ld_wait();
+                if (it.t0 + t >= masked_from) {
+                    const int visible = limit - (it.t0 + t) * kTcKeys;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (g * 32 + k >= visible) s[g][k] = 0xFF800000u;
+                }
+                float mx[4];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    mx[g] = __uint_as_float(s[g][0]);
+#pragma unroll
+                    for (int k = 1; k < 32; ++k) mx[g] = fmaxf(mx[g], __uint_as_float(s[g][k]));
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if (done == 0) {
+                    m = top;
+                } else if (__any_sync(0xffffffffu, (top - m) * c > 8.0f)) {
+                    const float m_new = fmaxf(m, top);
+                    const float f = m_new == m ? 1.0f : ex2((m - m_new) * c);
+                    m = m_new;
+                    l *= f;
+#pragma unroll
+                    for (int g = 0; g < D / 32; ++g) {
+                        uint32_t o[32];
+                        tmem_ld_32x32(t_o + g * 32, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                        tmem_st_32x32(t_o + g * 32, o);
+                    }
+                }
+                const float mc = m == -INFINITY ? 0.0f : m * c;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int g = 0; g < 4; g += 2) {
+                    uint32_t w1[32], w2[32];
+#pragma unroll
+                    for (int k = 0; k < 64; k += 2) {
+                        const float a = ex2(fmaf(__uint_as_float(s[g + k / 32][k % 32]), c, -mc));
+                        const float b = ex2(fmaf(__uint_as_float(s[g + k / 32][k % 32 + 1]), c, -mc));
+                        sum[(k / 2) & 3] += a + b;
+                        w1[k / 2] = pack_bf16(a, b);
+                        if constexpr (F32) w2[k / 2] = pack_bf16(a - bf16_lo(w1[k / 2]), b - bf16_hi(w1[k / 2]));
+                    }
+                    tmem_st_32x32(t_s + g * 16, w1);
+                    if constexpr (F32) tmem_st_32x32(t_s + 64 + g * 16, w2);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_st_wait();
+                tc5_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[wg]));
+            }
+            if (ok && done > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.o_full[wg]), o_phase & 1, err, kErrEpilogueWait));
+                ++o_phase;
+                tc5_fence_after();
+            }
+            if (!ok && lane == 0) sh.abort = 1;      // both groups still meet at this item's barriers, then both leave
+
+            // ---- results.  `emit` finishes 32 columns of a row
+            const bool direct = it.nchunks == 1;
+            bool patch = false;
+            auto emit = [&](int col, float (&o)[32], float factor) {
+                if (patch) {      // non-finite values that the MMAs did not get, for the rows that see them
+                    const int from = max(it.min_limit, it.t0 * kTcKeys), to = min(limit, (it.t0 + it.nt) * kTcKeys);
+                    for (int j = from; j < to; ++j) {
+                        const uint32_t blk = tables[int64_t(it.seq) * p.sh.max_blocks_per_seq + j / block];
+                        if (blk >= uint32_t(p.sh.num_blocks)) continue;
+                        const uint16_t* v = v_pool + (int64_t(blk) * block + j % block) * (int64_t(p.sh.num_kv_heads) * D) + it.kvh * D + col;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if ((v[k] & 0x7F80u) == 0x7F80u) o[k] += bf16_bits_to_f32(v[k]);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] *= factor;
+                if (!live) return;
+                if (direct) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {
+                        float y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = o[k + e];
+                        store_f32<T, 8>(out + out_row * D + col + k, y);
+                    }
+                } else {
+                    float* dst = part_o + (out_row * p.max_chunks + it.chunk) * D + col;
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(dst + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                }
+            };
+            if (!it.split) {
+                const float inv = direct ? 1.0f / l : 1.0f;
+                patch = sh.nonfinite[slot] != 0;        // set before the products that o_full stands for
+                for (int g = 0; g < D / 32; ++g) {
+                    uint32_t raw[32];
+                    float o[32];
+                    tmem_ld_32x32(t_o + g * 32, raw);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(raw[k]);
+                    emit(g * 32, o, inv);
+                }
+                if (!direct && live) part_ml[out_row * p.max_chunks + it.chunk] = make_float2(m * c, l);
+                tc5_fence_before();
+                bar_sync(1, kTcSoftmaxWarps * 32);      // both groups are done with their query tiles
+            } else {
+                sh.xm[wg][row] = m;
+                sh.xl[wg][row] = l;
+                bar_sync(1, kTcSoftmaxWarps * 32);      // every product that reads the query tile is complete: it may be overwritten
+                patch = sh.nonfinite[slot] != 0;
+                const float m0 = sh.xm[0][row], m1 = sh.xm[1][row], mt = fmaxf(m0, m1);
+                const float f0 = m0 == -INFINITY ? 0.0f : ex2((m0 - mt) * c), f1 = m1 == -INFINITY ? 0.0f : ex2((m1 - mt) * c);
+                const float lt = fmaf(sh.xl[0][row], f0, sh.xl[1][row] * f1);
+                float* xo = reinterpret_cast<float*>(q_smem);
+                constexpr int kCols = D / 2;            // group g finishes the columns [g D/2, (g + 1) D/2)
+                const int other = wg ^ 1;
+                const float mine = wg == 0 ? f0 : f1, theirs = wg == 0 ? f1 : f0;
+#pragma unroll
+                for (int g = 0; g < kCols / 32; ++g) {
+                    uint32_t raw[32];
+                    if (done > 0) {
+                        tmem_ld_32x32(t_o + other * kCols + g * 32, raw);
+                        tmem_ld_wait();
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) xo[(other * kCols + g * 32 + k) * 128 + row] = done > 0 ? __uint_as_float(raw[k]) : 0.0f;
+                }
+                bar_sync(1, kTcSoftmaxWarps * 32);
+                const float inv = direct ? 1.0f / lt : 1.0f;
+#pragma unroll
+                for (int g = 0; g < kCols / 32; ++g) {
+                    uint32_t raw[32];
+                    float o[32];
+                    if (done > 0) {
+                        tmem_ld_32x32(t_o + wg * kCols + g * 32, raw);
+                        tmem_ld_wait();
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                        o[k] = fmaf(done > 0 ? __uint_as_float(raw[k]) : 0.0f, mine, xo[(wg * kCols + g * 32 + k) * 128 + row] * theirs);
+                    emit(wg * kCols + g * 32, o, inv);
+                }
+                if (!direct && live && wg == 0) part_ml[out_row * p.max_chunks + it.chunk] = make_float2(mt * c, lt);
+                tc5_fence_before();
+                bar_sync(1, kTcSoftmaxWarps * 32);      // the exchanged halves have been read
+            }
+            if (*reinterpret_cast<volatile uint32_t*>(&sh.abort)) break;
+        }
+    }
+    // every copy has landed and every product is complete before the memory is given back
+    __syncthreads();
+    if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// Joins the key ranges of a row: one warp per (token row, query head).
+template <int D, typename T>
+__global__ void __launch_bounds__(256)
+paged_chunk_join_kernel(const __grid_constant__ TcShape p, int tile_rows, const uint32_t* __restrict__ q_starts,
+                        const uint32_t* __restrict__ seq_lens, const float* __restrict__ part_o, const float2* __restrict__ part_ml,
+                        T* __restrict__ out) {
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = blockIdx.x;
+    const int seq = sequence_of_row(q_starts, p.sh.batch, row);
+    if (seq >= p.sh.batch) return;
+    const int64_t s = q_starts[seq], e = q_starts[seq + 1], len = seq_lens[seq];
+    if (e > p.sh.rows || e - s > len || e - s > p.sh.max_q_len || len > p.sh.max_seq_len) return;      // reported by the first kernel
+    const int n = int(e - s), token = int(row - s);
+    const int chunks = ((int(len) + kTcKeys - 1) / kTcKeys + p.chunk_tiles - 1) / p.chunk_tiles;
+    if (chunks == 1) return;                                                                            // written already
+    for (int head = blockIdx.y * 8 + warp; head < p.sh.num_q_heads; head += gridDim.y * 8) {
+        const int r = token * p.group + head % p.group, last = min((r / tile_rows + 1) * tile_rows, n * p.group) - 1;
+        const int limit = int(len) - n + last / p.group + 1;                                            // of the item's last row
+        const int used = ((limit + kTcKeys - 1) / kTcKeys + p.chunk_tiles - 1) / p.chunk_tiles;
+        const int64_t base = (row * p.sh.num_q_heads + head) * p.max_chunks;
+        float m = -INFINITY;
+        for (int i = lane; i < used; i += 32) m = fmaxf(m, part_ml[base + i].x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        float l = 0.0f;
+        constexpr int V = D / 32;
+        float acc[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+        for (int i = 0; i < used; ++i) {
+            const float2 ml = part_ml[base + i];
+            if (ml.x == -INFINITY && ml.y == 0.0f) continue;           // no visible key in this range
+            const float w = ml.x == -INFINITY ? 1.0f : ex2(ml.x - m);
+            l = fmaf(ml.y, w, l);
+            float o[V];
+            load_f32<float, V>(part_o + (base + i) * D + lane * V, o);
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] = fmaf(o[k], w, acc[k]);
+        }
+        const float inv = 1.0f / l;
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] *= inv;
+        store_f32<T, V>(out + (row * p.sh.num_q_heads + head) * D + lane * V, acc);
+    }
+}
