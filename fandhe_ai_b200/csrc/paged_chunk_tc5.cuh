@@ -303,72 +303,77 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 else mbar_wait(smem_u32(&sh.full[stage]), (at / kNst) & 1, err, kErrProducerWait);
             }
     } else if (warp == 9) {
-        // ------------------------------------------------------------ MMA issue (one thread)
+        // ------------------------------------------------------------ MMA issue (one elected thread)
         constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((kTcKeys >> 3) << 17) | ((128 >> 4) << 24);
         constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((D >> 3) << 17) | ((128 >> 4) << 24);
         uint32_t pos = 0, p_phase[2] = {0, 0}, q_phase = 0;
         bool ok = true;
-        for (int64_t index = blockIdx.x; walk.get(index, it, nullptr); index += gridDim.x) {
+        auto wait = [&](uint32_t bar, uint32_t parity) { return bool(__all_sync(0xffffffffu, mbar_wait(bar, parity, err, kErrMmaWait))); };
+        for (int64_t index = blockIdx.x; ok && walk.get(index, it, nullptr); index += gridDim.x) {
             if (it.nt == 0) continue;
             const TcOrder order(pos, it);
             pos += 2 * it.nt;
-            if (lane == 0 && ok) {
-                const int n = it.nt;
-                ok = mbar_wait(smem_u32(&sh.q_full), q_phase & 1, err, kErrMmaWait);
-                ++q_phase;
+            const int n = it.nt;
+            const bool split = it.split;
+            ok = wait(smem_u32(&sh.q_full), q_phase & 1);
+            ++q_phase;
+            tc5_fence_after();
+            auto scores = [&](int s, int t, bool last_use) {
+                const uint32_t at = order.k(t), stage = at % kNst;
+                if (!wait(smem_u32(&sh.full[stage]), (at / kNst) & 1)) return false;
                 tc5_fence_after();
-                auto scores = [&](int s, int t, bool last_use) {
-                    const uint32_t at = order.k(t), stage = at % kNst;
-                    if (!mbar_wait(smem_u32(&sh.full[stage]), (at / kNst) & 1, err, kErrMmaWait)) return false;
-                    tc5_fence_after();
-                    const uint32_t k_tile = ring_addr + stage * Cfg::kTileBytes;
+                const uint64_t k_desc = umma_desc_k128(ring_addr + stage * Cfg::kTileBytes);
+                const uint64_t q_desc = umma_desc_k128(q_addr + (F32 || split ? 0 : s) * Cfg::kQTileBytes);
+                const uint32_t d = tmem + s * 128;
+                if (elect_one()) {
 #pragma unroll
-                    for (int term = 0; term < Cfg::kQTerms; ++term) {
-                        const uint32_t a = q_addr + (F32 ? term : (it.split ? 0 : s)) * Cfg::kQTileBytes;
+                    for (int term = 0; term < Cfg::kQTerms; ++term)
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk) {
-                            const uint32_t off = (kk / 4) * kHalfBytes + (kk % 4) * 32;
-                            umma_bf16_ss(tmem + s * 128, umma_desc_k128(a + off), umma_desc_k128(k_tile + off), kIdescS, term + kk > 0);
+                            const uint32_t off = ((kk / 4) * kHalfBytes + (kk % 4) * 32) >> 4;
+                            umma_bf16_ss(d, q_desc + off + ((term * Cfg::kQTileBytes) >> 4), k_desc + off, kIdescS, term + kk > 0);
                         }
-                    }
                     if (last_use) tc5_commit(smem_u32(&sh.empty[stage]));
                     tc5_commit(smem_u32(&sh.s_full[s]));
-                    return true;
-                };
-                auto values = [&](int s, int t, bool first, bool last_use, bool last) {
-                    const uint32_t at = order.v(t), stage = at % kNst;
-                    if (!mbar_wait(smem_u32(&sh.full[stage]), (at / kNst) & 1, err, kErrMmaWait)) return false;
-                    if (!mbar_wait(smem_u32(&sh.p_full[s]), p_phase[s] & 1, err, kErrMmaWait)) return false;
-                    ++p_phase[s];
-                    tc5_fence_after();
-                    const uint32_t v_tile = ring_addr + stage * Cfg::kTileBytes;
+                }
+                __syncwarp();
+                return true;
+            };
+            auto values = [&](int s, int t, bool first, bool last_use, bool last) {
+                const uint32_t at = order.v(t), stage = at % kNst;
+                if (!wait(smem_u32(&sh.full[stage]), (at / kNst) & 1)) return false;
+                if (!wait(smem_u32(&sh.p_full[s]), p_phase[s] & 1)) return false;
+                ++p_phase[s];
+                tc5_fence_after();
+                const uint64_t v_desc = umma_desc_mn128(ring_addr + stage * Cfg::kTileBytes, kHalfBytes);
+                const uint32_t d = tmem + 256 + s * 128, a = tmem + s * 128;
+                if (elect_one()) {
 #pragma unroll
                     for (int term = 0; term < Cfg::kPTerms; ++term)
 #pragma unroll
                         for (int kk = 0; kk < kTcKeys / 16; ++kk)
-                            umma_bf16_ts(tmem + 256 + s * 128, tmem + s * 128 + term * 64 + kk * 8,
-                                         umma_desc_mn128(v_tile + kk * 2048, kHalfBytes), kIdescO, !(first && term + kk == 0));
+                            umma_bf16_ts(d, a + term * 64 + kk * 8, v_desc + ((kk * 2048) >> 4), kIdescO, !(first && term + kk == 0));
                     if (last_use) tc5_commit(smem_u32(&sh.empty[stage]));
                     if (last) tc5_commit(smem_u32(&sh.o_full[s]));
-                    return true;
-                };
-                if (it.split) {
-                    ok = ok && scores(0, 0, true);
-                    if (n > 1) ok = ok && scores(1, 1, true);
-                    for (int t = 0; ok && t < n; ++t) {
-                        ok = values(t & 1, t, t < 2, true, t + 2 >= n);
-                        if (ok && t + 2 < n) ok = scores(t & 1, t + 2, true);
-                    }
-                } else {
-                    ok = ok && scores(0, 0, false) && scores(1, 0, true);
-                    for (int t = 0; ok && t < n; ++t)
-                        for (int s = 0; ok && s < 2; ++s) {
-                            ok = values(s, t, t == 0, s == 1, t + 1 == n);
-                            if (ok && t + 1 < n) ok = scores(s, t + 1, s == 1);
-                        }
                 }
+                __syncwarp();
+                return true;
+            };
+            if (split) {
+                ok = ok && scores(0, 0, true);
+                if (n > 1) ok = ok && scores(1, 1, true);
+                for (int t = 0; ok && t < n; ++t) {
+                    ok = values(t & 1, t, t < 2, true, t + 2 >= n);
+                    if (ok && t + 2 < n) ok = scores(t & 1, t + 2, true);
+                }
+            } else {
+                ok = ok && scores(0, 0, false) && scores(1, 0, true);
+                for (int t = 0; ok && t < n; ++t)
+                    for (int s = 0; ok && s < 2; ++s) {
+                        ok = values(s, t, t == 0, s == 1, t + 1 == n);
+                        if (ok && t + 1 < n) ok = scores(s, t + 1, s == 1);
+                    }
             }
-            __syncwarp();
         }
     } else if (warp == 10) {
         // ------------------------------------------------------------ V tiles with masked keys
