@@ -4,6 +4,8 @@
 // Sequence b brings the token rows [q_starts[b], q_starts[b + 1]); it holds seq_lens[b] cached tokens of which those rows are the
 // last, so row r of it stands at position seq_lens[b] - (q_starts[b + 1] - r).  All three arrays live on the device; nothing in
 // them is trusted: an index out of range sets the error word and touches nothing.
+#include <type_traits>
+
 #include "kernels.cuh"
 #include "launch.cuh"
 #include "ptx.cuh"

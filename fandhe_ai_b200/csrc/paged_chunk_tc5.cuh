@@ -16,11 +16,16 @@
 // The running maximum m of a row is raised only when a new score exceeds it by more than 2^8 in the weight: until then the
 // weights are merely larger than one, and O need not be rescaled.
 //
-// f32 activations: q = q1 + q2 + q3 and p = p1 + p2 as bf16 terms (exact to 24 bits and to 16 bits); K and V are bf16, so
-// the products are exact and the accumulators f32.  Three times the tensor work of the first product, twice that of the second.
+// f32 activations: q = q1 + q2 + q3 and p = p1 + p2 + p3 as bf16 terms, exact to 24 bits; K and V are bf16, so the products are
+// exact and the accumulators f32.  Three times the tensor work; but an item of at most 32 rows stands its terms in the
+// three quarters of one tile of accumulator rows ("stacked"): one product gives the partial scores of all terms, which the
+// three warps of a group exchange, and one product the three partial results, which are added at the end.
+//
+// The softmax weights go to the MMA warp in two halves of 64 keys, so that the second product starts while the second
+// half is still in the exponential.
 //
 // Warps: 0-7 softmax (two groups), 8 TMA producer (one box per cache block and half head through the block table), 9 MMA issue,
-// 10 cleans V (11 idles): an MMA multiplies what it must not see by zero, which does not remove NaN and infinities.  In tiles with
+// 10 cleans V, 11 deals out the items (decoded once, into shared memory): an MMA multiplies what it must not see by zero, which does not remove NaN and infinities.  In tiles with
 // masked keys (only the last ones of a sequence; such a tile is announced to warp 10, and by warp 10 to the MMA warp) rows beyond the item's last visible key are zeroed, non-finite elements
 // of rows that some query must not see are replaced by zero, and if there were any the epilogue adds them back to the rows that do see them.
 
@@ -29,17 +34,21 @@ constexpr int kTcThreads = 32 * (kTcSoftmaxWarps + 4);
 // Registers a thread: 168 at launch (384 threads); the softmax threads hold a row of 128 scores and take 216, the other four warps
 // give theirs up: 256 x 216 + 128 x 72 = 384 x 168.
 constexpr int kTcKeys = 128;               // keys of a tile
-constexpr int kTcFlagSlots = 16;
+constexpr int kTcItemSlots = 4;            // items known ahead
 
 template <int D, bool F32>
 struct TcCfg {
     static constexpr int kQTerms = F32 ? 3 : 1;
-    static constexpr int kPTerms = F32 ? 2 : 1;
+    static constexpr int kPTerms = F32 ? 3 : 1;
     static constexpr int kTileBytes = kTcKeys * D * 2;                       // a K or V tile
     static constexpr int kQTileBytes = 128 * D * 2;
-    static constexpr int kQBytes = (F32 ? 3 : 2) * kQTileBytes;              // also holds the 128 D f32 exchanged by the slots
+    // query tiles; also holds what the groups exchange: 128 D f32 at the end of an item, and for stacked items
+    // partial scores (behind the first tile) and 2 x 96 x D f32 at the end
+    static constexpr int kXchgBytes = F32 ? 3 * 64 * 32 * 4 : 0;             // partial scores of a group
+    static constexpr int kQTilesBytes = (F32 ? 3 : 2) * kQTileBytes;
+    static constexpr int kQBytes = kQTilesBytes > kQTileBytes + 2 * kXchgBytes ? kQTilesBytes : kQTileBytes + 2 * kXchgBytes;
     static constexpr int kStages = D == 128 ? (F32 ? 4 : 5) : 8;
-    static constexpr int kSmem = kQBytes + kStages * kTileBytes + 2560;
+    static constexpr int kSmem = kQBytes + kStages * kTileBytes + 3072;
     static constexpr int kRows = F32 ? 128 : 256;                            // rows of an item
 };
 
@@ -55,7 +64,8 @@ struct TcItem {
     int t0, nt;                                    // key tiles [t0, t0 + nt)
     int n, len, start;                             // new tokens, cached tokens, first token row
     int min_limit, max_limit;                      // visible keys of the first and the last row
-    bool split;
+    bool split, stack;                             // the slots share the rows; the three terms share the accumulator rows
+    uint32_t nonfinite;                            // set when cleaning met non-finite values
 };
 
 // Walks the items of a launch in increasing order; all lanes of a warp together.
@@ -125,6 +135,8 @@ struct TcWalk {
         it.t0 = it.chunk * p.chunk_tiles;
         it.nt = max(0, min(tiles, it.t0 + p.chunk_tiles) - it.t0);
         it.split = F32 || it.rows <= 128;
+        it.stack = F32 && it.rows <= 32;
+        it.nonfinite = 0;
         return true;
     }
 };
@@ -151,6 +163,24 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+
+// Two f32 operations in one instruction
+struct F2 {
+    unsigned long long v;
+    __device__ __forceinline__ F2() {}
+    __device__ __forceinline__ F2(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+    __device__ __forceinline__ void get(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
 
 // Shared-memory descriptor of an MN-major operand whose rows (one per K index) are 128 bytes of the M / N dimension, 128-byte
 // swizzled: 8-row groups along K are 1024 bytes apart, the next 64 elements along M / N start `lead` bytes further.
@@ -186,18 +216,41 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
         "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
+// First column (of a slot's 128) of the bf16 weights of half `h` and term `term`.  Three terms of 64 keys take 96 columns, so
+// the second half's last two terms are written over the first half's once that has been multiplied.
+__device__ __forceinline__ uint32_t weight_columns(int h, int term, bool terms3) {
+    if (!terms3) return h * 32;
+    return h == 0 ? term * 32 : (term == 0 ? 96 : (term - 1) * 32);
+}
+
 struct TcShared {
     uint64_t full[8], empty[8], raw[8];        // raw: a V tile with masked keys has landed and is to be cleaned
-    uint64_t s_full[2], p_full[2], o_full[2], q_full;
+    uint64_t s_full[2], p_full[2][2], p_free[2], o_full[2], q_full;
     uint32_t tmem;
     uint32_t abort;                            // a softmax warp gave up waiting
-    uint32_t nonfinite[kTcFlagSlots];
+    uint64_t item_full[kTcItemSlots], item_empty[kTcItemSlots];
+    TcItem items[kTcItemSlots];                // nt < 0: no more
     float xm[2][128], xl[2][128];
 };
-static_assert(sizeof(TcShared) <= 2560, "");
+static_assert(sizeof(TcShared) <= 3072, "");
 
 template <int D, bool F32, typename T>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -224,10 +277,16 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(smem_u32(&sh.s_full[s]), 1);
-            mbar_init(smem_u32(&sh.p_full[s]), 4);
+            mbar_init(smem_u32(&sh.p_full[s][0]), 4);
+            mbar_init(smem_u32(&sh.p_full[s][1]), 4);
+            mbar_init(smem_u32(&sh.p_free[s]), 1);
             mbar_init(smem_u32(&sh.o_full[s]), 1);
         }
         mbar_init(smem_u32(&sh.q_full), kTcSoftmaxWarps);
+        for (int i = 0; i < kTcItemSlots; ++i) {
+            mbar_init(smem_u32(&sh.item_full[i]), 1);
+            mbar_init(smem_u32(&sh.item_empty[i]), kTcSoftmaxWarps + 3);
+        }
         sh.abort = 0;
         fence_barrier_init();
     }
@@ -247,9 +306,17 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const uint32_t tmem = sh.tmem;
     pdl_launch_dependents();
 
-    TcWalk<Cfg::kRows, F32> walk(p, q_starts, seq_lens);
-    TcItem it;
     const int block = p.sh.block_size;
+    // the k-th item, for every warp but the one that deals them out; null: no more (or the wait ran out)
+    auto next_item = [&](uint32_t k) -> TcItem* {
+        const uint32_t slot = k % kTcItemSlots;
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.item_full[slot]), (k / kTcItemSlots) & 1, err, kErrProducerWait))) return nullptr;
+        return sh.items[slot].nt < 0 ? nullptr : &sh.items[slot];
+    };
+    auto release_item = [&](uint32_t k) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.item_empty[k % kTcItemSlots]));
+    };
 
     if (warp >= kTcSoftmaxWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -258,8 +325,10 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         uint32_t pos = 0, issued = 0, raw_last = 0, raw_phase = 0;      // per stage: its last tile went to `raw`; parity of those
         bool ok = true;
         const int box = min(block, kTcKeys);
-        for (int64_t index = blockIdx.x; ok && walk.get(index, it, err); index += gridDim.x) {
-            if (it.nt == 0) continue;
+        uint32_t k_item = 0;
+        for (TcItem* item; ok && (item = next_item(k_item)) != nullptr; ++k_item) {
+            const TcItem it = *item;
+            release_item(k_item);
             const TcOrder order(pos, it);
             const uint32_t* table = tables + int64_t(it.seq) * p.sh.max_blocks_per_seq;
             const int end = min(it.max_limit, (it.t0 + it.nt) * kTcKeys);
@@ -309,12 +378,13 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         uint32_t pos = 0, p_phase[2] = {0, 0}, q_phase = 0;
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) { return bool(__all_sync(0xffffffffu, mbar_wait(bar, parity, err, kErrMmaWait))); };
-        for (int64_t index = blockIdx.x; ok && walk.get(index, it, nullptr); index += gridDim.x) {
-            if (it.nt == 0) continue;
-            const TcOrder order(pos, it);
-            pos += 2 * it.nt;
-            const int n = it.nt;
-            const bool split = it.split;
+        uint32_t k_item = 0;
+        for (TcItem* item; ok && (item = next_item(k_item)) != nullptr; ++k_item) {
+            const TcOrder order(pos, *item);
+            const int n = item->nt;
+            const bool split = item->split, stack = item->stack;
+            release_item(k_item);
+            pos += 2 * n;
             ok = wait(smem_u32(&sh.q_full), q_phase & 1);
             ++q_phase;
             tc5_fence_after();
@@ -325,38 +395,53 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 const uint64_t k_desc = umma_desc_k128(ring_addr + stage * Cfg::kTileBytes);
                 const uint64_t q_desc = umma_desc_k128(q_addr + (F32 || split ? 0 : s) * Cfg::kQTileBytes);
                 const uint32_t d = tmem + s * 128;
-                if (elect_one()) {
+                // (no condition may stand inside the elected thread's block: it would cost hundreds of clocks a product)
+                auto multiply = [&](auto terms) {
+                    if (elect_one()) {
 #pragma unroll
-                    for (int term = 0; term < Cfg::kQTerms; ++term)
+                        for (int term = 0; term < decltype(terms)::value; ++term)
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk) {
-                            const uint32_t off = ((kk / 4) * kHalfBytes + (kk % 4) * 32) >> 4;
-                            umma_bf16_ss(d, q_desc + off + ((term * Cfg::kQTileBytes) >> 4), k_desc + off, kIdescS, term + kk > 0);
-                        }
-                    if (last_use) tc5_commit(smem_u32(&sh.empty[stage]));
-                    tc5_commit(smem_u32(&sh.s_full[s]));
-                }
+                            for (int kk = 0; kk < D / 16; ++kk) {
+                                const uint32_t off = ((kk / 4) * kHalfBytes + (kk % 4) * 32) >> 4;
+                                umma_bf16_ss(d, q_desc + off + ((term * Cfg::kQTileBytes) >> 4), k_desc + off, kIdescS, term + kk > 0);
+                            }
+                        if (last_use) tc5_commit(smem_u32(&sh.empty[stage]));
+                        tc5_commit(smem_u32(&sh.s_full[s]));
+                    }
+                };
+                if (F32 && stack) multiply(std::integral_constant<int, 1>());
+                else multiply(std::integral_constant<int, Cfg::kQTerms>());
                 __syncwarp();
                 return true;
             };
             auto values = [&](int s, int t, bool first, bool last_use, bool last) {
                 const uint32_t at = order.v(t), stage = at % kNst;
                 if (!wait(smem_u32(&sh.full[stage]), (at / kNst) & 1)) return false;
-                if (!wait(smem_u32(&sh.p_full[s]), p_phase[s] & 1)) return false;
-                ++p_phase[s];
-                tc5_fence_after();
-                const uint64_t v_desc = umma_desc_mn128(ring_addr + stage * Cfg::kTileBytes, kHalfBytes);
-                const uint32_t d = tmem + 256 + s * 128, a = tmem + s * 128;
-                if (elect_one()) {
+                const uint32_t v_tile = ring_addr + stage * Cfg::kTileBytes, d = tmem + 256 + s * 128, a = tmem + s * 128;
+                const uint64_t v_desc = umma_desc_mn128(v_tile, kHalfBytes);
 #pragma unroll
-                    for (int term = 0; term < Cfg::kPTerms; ++term)
+                for (int h = 0; h < 2; ++h) {      // the weights arrive in halves of 64 keys
+                    if (!wait(smem_u32(&sh.p_full[s][h]), p_phase[s] & 1)) return false;
+                    tc5_fence_after();
+                    auto multiply = [&](auto terms) {
+                        constexpr int kTerms = decltype(terms)::value;
+                        if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < kTcKeys / 16; ++kk)
-                            umma_bf16_ts(d, a + term * 64 + kk * 8, v_desc + ((kk * 2048) >> 4), kIdescO, !(first && term + kk == 0));
-                    if (last_use) tc5_commit(smem_u32(&sh.empty[stage]));
-                    if (last) tc5_commit(smem_u32(&sh.o_full[s]));
+                            for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+                                for (int kk = 0; kk < 4; ++kk)
+                                    umma_bf16_ts(d, a + weight_columns(h, term, kTerms == 3) + kk * 8, v_desc + (((h * 4 + kk) * 2048) >> 4),
+                                                 kIdescO, !(first && h + term + kk == 0));
+                            if (h == 0 && kTerms == 3) tc5_commit(smem_u32(&sh.p_free[s]));
+                            if (h == 1 && last_use) tc5_commit(smem_u32(&sh.empty[stage]));
+                            if (h == 1 && last) tc5_commit(smem_u32(&sh.o_full[s]));
+                        }
+                    };
+                    if (F32 && stack) multiply(std::integral_constant<int, 1>());
+                    else multiply(std::integral_constant<int, Cfg::kPTerms>());
+                    __syncwarp();
                 }
-                __syncwarp();
+                ++p_phase[s];
                 return true;
             };
             if (split) {
@@ -377,15 +462,12 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
     } else if (warp == 10) {
         // ------------------------------------------------------------ V tiles with masked keys
-        uint32_t pos = 0, count = 0, raw_phase = 0;
+        uint32_t pos = 0, raw_phase = 0, k_item = 0;
         bool ok = true;
-        for (int64_t index = blockIdx.x; ok && walk.get(index, it, nullptr); index += gridDim.x) {
-            if (it.nt == 0) continue;
+        for (TcItem* item; ok && (item = next_item(k_item)) != nullptr; release_item(k_item++)) {
+            const TcItem& it = *item;
             const TcOrder order(pos, it);
             pos += 2 * it.nt;
-            const uint32_t slot = count++ % kTcFlagSlots;
-            if (lane == 0) sh.nonfinite[slot] = 0;
-            __syncwarp();
             const int masked_from = it.min_limit / kTcKeys;
             for (int t = max(0, masked_from - it.t0); ok && t < it.nt; ++t) {
                 const uint32_t at = order.v(t), stage = at % kNst;
@@ -416,12 +498,31 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         if (bad) { *piece = v; found = true; }
                     }
                 }
-                if (found) sh.nonfinite[slot] = 1;
+                if (found) item->nonfinite = 1;
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sh.full[stage]));
             }
         }
+    } else {
+        // ------------------------------------------------------------ items
+        TcWalk<Cfg::kRows, F32> walk(p, q_starts, seq_lens);
+        TcItem it;
+        uint32_t k = 0;
+        auto deal = [&]() {
+            const uint32_t slot = k % kTcItemSlots;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.item_empty[slot]), ((k / kTcItemSlots) & 1) ^ 1, err, kErrProducerWait))) return false;
+            if (lane == 0) sh.items[slot] = it;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.item_full[slot]));
+            ++k;
+            return true;
+        };
+        bool ok = true;
+        for (int64_t index = blockIdx.x; ok && walk.get(index, it, err); index += gridDim.x)
+            if (it.nt > 0) ok = deal();
+        it.nt = -1;
+        if (ok) deal();
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -430,13 +531,15 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         const uint32_t lane_base = uint32_t(warp & 3) << 21;               // 32 lanes a warp, lane field in the upper half of the address
         const uint32_t t_s = tmem + wg * 128 + lane_base, t_o = tmem + 256 + wg * 128 + lane_base;
         const float c = p.scale_log2;
-        uint32_t s_phase = 0, o_phase = 0, count = 0;
+        uint32_t s_phase = 0, f_phase = 0, o_phase = 0, k_item = 0;      // f_phase: tiles whose first half is waited for (p_free)
         bool ok = true;
-        for (int64_t index = blockIdx.x; ok && walk.get(index, it, nullptr); index += gridDim.x) {
-            if (it.nt == 0) continue;
-            const uint32_t slot = count++ % kTcFlagSlots;
-            const int r = (it.split ? 0 : wg * 128) + row;                 // row of the item
+        for (TcItem* item; ok && (item = next_item(k_item)) != nullptr; release_item(k_item++)) {
+            const TcItem& it = *item;
+            const bool stack = F32 && it.stack;
+            const int r = stack ? row & 31 : (it.split ? 0 : wg * 128) + row;      // row of the item
             const bool live = r < it.rows;
+            // a warp without rows only keeps the barriers going: its accumulator rows hold garbage that nobody reads
+            const bool busy = __any_sync(0xffffffffu, live) && !(stack && (warp & 3) == 3);
             const int list = it.row0 + r, token = list / p.group, head = it.kvh * p.group + list % p.group;
             const int limit = live ? it.len - it.n + token + 1 : 0;
             const int64_t out_row = (int64_t(it.start) + token) * p.sh.num_q_heads + head;
@@ -451,7 +554,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     const int piece = (it.split ? wg * per : 0) + j;
                     const int at = (piece / 8) * kHalfBytes + row * 128 + (((piece % 8) ^ (row & 7)) << 4);
                     float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                    if (live) {
+                    if (live && busy) {
                         load_f32<T, 8>(src + piece * 8, x);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) x[k] *= p.q_sign;
@@ -465,7 +568,8 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                             x[2 * k] -= bf16_lo(w[k]);
                             x[2 * k + 1] -= bf16_hi(w[k]);
                         }
-                        *reinterpret_cast<uint4*>(dst + term * Cfg::kQTileBytes + at) = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (!stack) *reinterpret_cast<uint4*>(dst + term * Cfg::kQTileBytes + at) = make_uint4(w[0], w[1], w[2], w[3]);
+                        else if (term == (warp & 3)) *reinterpret_cast<uint4*>(dst + at) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
                 fence_proxy_async();
@@ -475,31 +579,59 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
 
             float m = -INFINITY, l = 0.0f;
-            const int masked_from = it.min_limit / kTcKeys, step = it.split ? 2 : 1;
+            const int masked_from = it.min_limit / kTcKeys - it.t0, step = it.split ? 2 : 1, nt = it.nt, k0 = it.t0 * kTcKeys;
             int done = 0;
-            for (int t = it.split ? wg : 0; t < it.nt; t += step, ++done) {
+            for (int t = it.split ? wg : 0; t < nt; t += step, ++done) {
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.s_full[wg]), s_phase & 1, err, kErrEpilogueWait));
                 if (!ok) break;
-                ++s_phase;
-                tc5_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int g = 0; g < 4; ++g) tmem_ld_32x32(t_s + g * 32, s[g]);
-                tmem_ld_wait();
-                if (it.t0 + t >= masked_from) {
-                    const int visible = limit - (it.t0 + t) * kTcKeys;
-#pragma unroll
-                    for (int g = 0; g < 4; ++g)
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (g * 32 + k >= visible) s[g][k] = 0xFF800000u;
+                if (!busy) {
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_u32(&sh.p_full[wg][0]));
+                        mbar_arrive(smem_u32(&sh.p_full[wg][1]));
+                    }
+                    ++s_phase;
+                    f_phase += !stack;
+                    continue;
                 }
+                tc5_fence_after();
+                float s[128];
                 float mx[4];
+                {
+                    uint32_t raw[4][32];
+                    tmem_ld_32x32(t_s, raw[0]);
+                    tmem_ld_32x32(t_s + 32, raw[1]);
+                    tmem_ld_32x32(t_s + 64, raw[2]);
+                    tmem_ld_32x32(t_s + 96, raw[3]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 128; ++k) s[k] = __uint_as_float(raw[k / 32][k % 32]);
+                }
+                if constexpr (F32) {
+                    if (stack) {      // scores are the sum of the three terms' partial scores, added in the same order by all three warps
+                        float* xs = reinterpret_cast<float*>(q_smem + Cfg::kQTileBytes + wg * Cfg::kXchgBytes);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                            for (int k = 0; k < 64; ++k) xs[((warp & 3) * 64 + k) * 32 + lane] = s[h * 64 + k];
+                            bar_sync(2 + wg, 96);
+#pragma unroll
+                            for (int k = 0; k < 64; ++k) s[h * 64 + k] = (xs[(128 + k) * 32 + lane] + xs[(64 + k) * 32 + lane]) + xs[k * 32 + lane];
+                            bar_sync(2 + wg, 96);
+                        }
+                    }
+                }
+                if (t >= masked_from) {
+                    const int visible = limit - k0 - t * kTcKeys;
+#pragma unroll
+                    for (int k = 0; k < 128; ++k)
+                        if (k >= visible) s[k] = -INFINITY;
+                }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    mx[g] = __uint_as_float(s[g][0]);
+                    mx[g] = fmaxf(s[g], s[g + 4]);
 #pragma unroll
-                    for (int k = 1; k < 32; ++k) mx[g] = fmaxf(mx[g], __uint_as_float(s[g][k]));
+                    for (int k = 8; k < 128; k += 8) mx[g] = fmaxf(fmaxf(mx[g], s[k + g]), s[k + 4 + g]);
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 if (done == 0) {
@@ -510,36 +642,68 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     m = m_new;
                     l *= f;
 #pragma unroll
-                    for (int g = 0; g < D / 32; ++g) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(t_o + g * 32, o);
+                    for (int g = 0; g < D / 16; ++g) {
+                        uint32_t o[16];
+                        tmem_ld_32x16(t_o + g * 16, o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                        tmem_st_32x32(t_o + g * 32, o);
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                        tmem_st_32x16(t_o + g * 16, o);
                     }
                 }
                 const float mc = m == -INFINITY ? 0.0f : m * c;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const F2 c2(c, c), mc2(-mc, -mc);
+                F2 sum[2] = {F2(0.0f, 0.0f), F2(0.0f, 0.0f)};
 #pragma unroll
-                for (int g = 0; g < 4; g += 2) {
-                    uint32_t w1[32], w2[32];
+                for (int h = 0; h < 2; ++h) {
+                    constexpr int kParts = F32 ? 3 : 1;
 #pragma unroll
-                    for (int k = 0; k < 64; k += 2) {
-                        const float a = ex2(fmaf(__uint_as_float(s[g + k / 32][k % 32]), c, -mc));
-                        const float b = ex2(fmaf(__uint_as_float(s[g + k / 32][k % 32 + 1]), c, -mc));
-                        sum[(k / 2) & 3] += a + b;
-                        w1[k / 2] = pack_bf16(a, b);
-                        if constexpr (F32) w2[k / 2] = pack_bf16(a - bf16_lo(w1[k / 2]), b - bf16_hi(w1[k / 2]));
+                    for (int g = 0; g < 2; ++g) {          // 32 keys, 16 columns a term
+                        uint32_t w[kParts][16];
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) {
+                            const int at = h * 64 + g * 32 + k;
+                            float a, b;
+                            fma2(F2(s[at], s[at + 1]), c2, mc2).get(a, b);
+                            a = ex2(a);
+                            b = ex2(b);
+                            sum[(k / 2) & 1] = add2(sum[(k / 2) & 1], F2(a, b));
+                            w[0][k / 2] = pack_bf16(a, b);
+                            if constexpr (F32) {
+                                const float a2 = a - bf16_lo(w[0][k / 2]), b2 = b - bf16_hi(w[0][k / 2]);
+                                w[1][k / 2] = pack_bf16(a2, b2);
+                                w[2][k / 2] = pack_bf16(a2 - bf16_lo(w[1][k / 2]), b2 - bf16_hi(w[1][k / 2]));
+                            }
+                        }
+                        if constexpr (F32) {
+                            if (stack) {
+                                if ((warp & 3) == 0) tmem_st_32x16(t_s + h * 32 + g * 16, w[0]);
+                                else if ((warp & 3) == 1) tmem_st_32x16(t_s + h * 32 + g * 16, w[1]);
+                                else tmem_st_32x16(t_s + h * 32 + g * 16, w[2]);
+                            } else {
+                                tmem_st_32x16(t_s + weight_columns(h, 0, true) + g * 16, w[0]);
+                                if (h == 1 && g == 0) {      // the columns of the first half's last two terms
+                                    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.p_free[wg]), f_phase & 1, err, kErrEpilogueWait)) && ok;
+                                    tc5_fence_after();
+                                }
+                                tmem_st_32x16(t_s + weight_columns(h, 1, true) + g * 16, w[1]);
+                                tmem_st_32x16(t_s + weight_columns(h, 2, true) + g * 16, w[2]);
+                            }
+                        } else {
+                            tmem_st_32x16(t_s + h * 32 + g * 16, w[0]);
+                        }
                     }
-                    tmem_st_32x32(t_s + g * 16, w1);
-                    if constexpr (F32) tmem_st_32x32(t_s + 64 + g * 16, w2);
+                    tmem_st_wait();
+                    tc5_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[wg][h]));
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_st_wait();
-                tc5_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[wg]));
+                ++s_phase;
+                f_phase += !stack;
+                float a, b;
+                add2(sum[0], sum[1]).get(a, b);
+                l += a + b;
+                if (!ok) break;
             }
             if (ok && done > 0) {
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.o_full[wg]), o_phase & 1, err, kErrEpilogueWait));
@@ -548,10 +712,11 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
             if (!ok && lane == 0) sh.abort = 1;      // both groups still meet at this item's barriers, then both leave
 
-            // ---- results.  `emit` finishes 32 columns of a row
+            // ---- results.  `emit` finishes some columns of a row
             const bool direct = it.nchunks == 1;
             bool patch = false;
-            auto emit = [&](int col, float (&o)[32], float factor) {
+            auto emit = [&](int col, auto& o, float factor) {
+                constexpr int N = sizeof(o) / sizeof(float);
                 if (patch) {      // non-finite values that the MMAs did not get, for the rows that see them
                     const int from = max(it.min_limit, it.t0 * kTcKeys), to = min(limit, (it.t0 + it.nt) * kTcKeys);
                     for (int j = from; j < to; ++j) {
@@ -559,16 +724,16 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         if (blk >= uint32_t(p.sh.num_blocks)) continue;
                         const uint16_t* v = v_pool + (int64_t(blk) * block + j % block) * (int64_t(p.sh.num_kv_heads) * D) + it.kvh * D + col;
 #pragma unroll
-                        for (int k = 0; k < 32; ++k)
+                        for (int k = 0; k < N; ++k)
                             if ((v[k] & 0x7F80u) == 0x7F80u) o[k] += bf16_bits_to_f32(v[k]);
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] *= factor;
+                for (int k = 0; k < N; ++k) o[k] *= factor;
                 if (!live) return;
                 if (direct) {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
+                    for (int k = 0; k < N; k += 8) {
                         float y[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) y[e] = o[k + e];
@@ -577,13 +742,13 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 } else {
                     float* dst = part_o + (out_row * p.max_chunks + it.chunk) * D + col;
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(dst + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(dst + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                 }
             };
             if (!it.split) {
                 const float inv = direct ? 1.0f / l : 1.0f;
-                patch = sh.nonfinite[slot] != 0;        // set before the products that o_full stands for
-                for (int g = 0; g < D / 32; ++g) {
+                patch = *reinterpret_cast<volatile uint32_t*>(&item->nonfinite) != 0;        // set before the products that o_full stands for
+                for (int g = 0; g < (busy ? D / 32 : 0); ++g) {
                     uint32_t raw[32];
                     float o[32];
                     tmem_ld_32x32(t_o + g * 32, raw);
@@ -596,43 +761,73 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 tc5_fence_before();
                 bar_sync(1, kTcSoftmaxWarps * 32);      // both groups are done with their query tiles
             } else {
-                sh.xm[wg][row] = m;
-                sh.xl[wg][row] = l;
+                const int lane_row = stack ? lane : row;
+                if (!stack || (warp & 3) == 0) {
+                    sh.xm[wg][row] = m;
+                    sh.xl[wg][row] = l;
+                }
                 bar_sync(1, kTcSoftmaxWarps * 32);      // every product that reads the query tile is complete: it may be overwritten
-                patch = sh.nonfinite[slot] != 0;
-                const float m0 = sh.xm[0][row], m1 = sh.xm[1][row], mt = fmaxf(m0, m1);
+                patch = *reinterpret_cast<volatile uint32_t*>(&item->nonfinite) != 0;
+                const float m0 = sh.xm[0][lane_row], m1 = sh.xm[1][lane_row], mt = fmaxf(m0, m1);
                 const float f0 = m0 == -INFINITY ? 0.0f : ex2((m0 - mt) * c), f1 = m1 == -INFINITY ? 0.0f : ex2((m1 - mt) * c);
-                const float lt = fmaf(sh.xl[0][row], f0, sh.xl[1][row] * f1);
-                float* xo = reinterpret_cast<float*>(q_smem);
-                constexpr int kCols = D / 2;            // group g finishes the columns [g D/2, (g + 1) D/2)
-                const int other = wg ^ 1;
-                const float mine = wg == 0 ? f0 : f1, theirs = wg == 0 ? f1 : f0;
-#pragma unroll
-                for (int g = 0; g < kCols / 32; ++g) {
-                    uint32_t raw[32];
-                    if (done > 0) {
-                        tmem_ld_32x32(t_o + other * kCols + g * 32, raw);
-                        tmem_ld_wait();
-                    }
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) xo[(other * kCols + g * 32 + k) * 128 + row] = done > 0 ? __uint_as_float(raw[k]) : 0.0f;
-                }
-                bar_sync(1, kTcSoftmaxWarps * 32);
+                const float lt = fmaf(sh.xl[0][lane_row], f0, sh.xl[1][lane_row] * f1);
                 const float inv = direct ? 1.0f / lt : 1.0f;
+                float* xo = reinterpret_cast<float*>(q_smem);
+                if (stack) {
+                    if (busy) {
 #pragma unroll
-                for (int g = 0; g < kCols / 32; ++g) {
-                    uint32_t raw[32];
-                    float o[32];
-                    if (done > 0) {
-                        tmem_ld_32x32(t_o + wg * kCols + g * 32, raw);
-                        tmem_ld_wait();
+                        for (int g = 0; g < D / 32; ++g) {
+                            uint32_t raw[32];
+                            if (done > 0) {
+                                tmem_ld_32x32(t_o + g * 32, raw);
+                                tmem_ld_wait();
+                            }
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) xo[(wg * D + g * 32 + k) * 96 + row] = done > 0 ? __uint_as_float(raw[k]) : 0.0f;
+                        }
                     }
+                    bar_sync(1, kTcSoftmaxWarps * 32);
+                    constexpr int kCols = D / 8;        // columns of a warp
+                    float o[kCols];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        o[k] = fmaf(done > 0 ? __uint_as_float(raw[k]) : 0.0f, mine, xo[(wg * kCols + g * 32 + k) * 128 + row] * theirs);
-                    emit(wg * kCols + g * 32, o, inv);
+                    for (int k = 0; k < kCols; ++k) {
+                        const float* x0 = xo + (warp * kCols + k) * 96 + lane;
+                        const float* x1 = x0 + D * 96;
+                        o[k] = fmaf((x0[64] + x0[32]) + x0[0], f0, ((x1[64] + x1[32]) + x1[0]) * f1);
+                    }
+                    emit(warp * kCols, o, inv);
+                } else {
+                    constexpr int kCols = D / 2;        // group g finishes the columns [g D/2, (g + 1) D/2)
+                    const int other = wg ^ 1;
+                    const float mine = wg == 0 ? f0 : f1, theirs = wg == 0 ? f1 : f0;
+#pragma unroll
+                    for (int g = 0; g < kCols / 32; ++g) {
+                        if (!busy) break;
+                        uint32_t raw[32];
+                        if (done > 0) {
+                            tmem_ld_32x32(t_o + other * kCols + g * 32, raw);
+                            tmem_ld_wait();
+                        }
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) xo[(other * kCols + g * 32 + k) * 128 + row] = done > 0 ? __uint_as_float(raw[k]) : 0.0f;
+                    }
+                    bar_sync(1, kTcSoftmaxWarps * 32);
+#pragma unroll
+                    for (int g = 0; g < kCols / 32; ++g) {
+                        if (!busy) break;
+                        uint32_t raw[32];
+                        float o[32];
+                        if (done > 0) {
+                            tmem_ld_32x32(t_o + wg * kCols + g * 32, raw);
+                            tmem_ld_wait();
+                        }
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            o[k] = fmaf(done > 0 ? __uint_as_float(raw[k]) : 0.0f, mine, xo[(wg * kCols + g * 32 + k) * 128 + row] * theirs);
+                        emit(wg * kCols + g * 32, o, inv);
+                    }
                 }
-                if (!direct && live && wg == 0) part_ml[out_row * p.max_chunks + it.chunk] = make_float2(mt * c, lt);
+                if (!direct && live && warp == (stack ? 0 : warp & 3)) part_ml[out_row * p.max_chunks + it.chunk] = make_float2(mt * c, lt);
                 tc5_fence_before();
                 bar_sync(1, kTcSoftmaxWarps * 32);      // the exchanged halves have been read
             }
