@@ -17,16 +17,18 @@
 // weights are merely larger than one, and O need not be rescaled.
 //
 // f32 activations: q = q1 + q2 + q3 and p = p1 + p2 + p3 as bf16 terms, exact to 24 bits; K and V are bf16, so the products are
-// exact and the accumulators f32.  Three times the tensor work; but an item of at most 32 rows stands its terms in the
-// three quarters of one tile of accumulator rows ("stacked"): one product gives the partial scores of all terms, which the
-// three warps of a group exchange, and one product the three partial results, which are added at the end.
+// exact and the accumulators f32.  Three times the tensor work; but an item of at most 32 rows ("stacked") has its queries
+// three times in the tile of accumulator rows, so that three warps of a group hold the same scores, and each contributes one term
+// of the weights: one product gives the three partial results, which are added at the end.
 //
 // The softmax weights go to the MMA warp in two halves of 64 keys, so that the second product starts while the second
 // half is still in the exponential.
 //
-// Warps: 0-7 softmax (two groups), 8 TMA producer (one box per cache block and half head through the block table), 9 MMA issue,
-// 10 cleans V, 11 deals out the items (decoded once, into shared memory): an MMA multiplies what it must not see by zero, which does not remove NaN and infinities.  In tiles with
-// masked keys (only the last ones of a sequence; such a tile is announced to warp 10, and by warp 10 to the MMA warp) rows beyond the item's last visible key are zeroed, non-finite elements
+// Warps: 0-7 softmax (two groups); 8 deals out the items (decoded once, into shared memory) and fetches their tiles by TMA (one
+// box per cache block and half head, through the block table); 9 and 10 issue the products of one slot each, which keeps the
+// chain scores -> softmax -> values of a slot free of the other slot's waits; 11 cleans V: an MMA multiplies what it must not
+// see by zero, which does not remove NaN and infinities.  In tiles with
+// masked keys (only the last ones of a sequence; such a tile is announced to warp 11, and by it to the MMA warps) rows beyond the item's last visible key are zeroed, non-finite elements
 // of rows that some query must not see are replaced by zero, and if there were any the epilogue adds them back to the rows that do see them.
 
 constexpr int kTcSoftmaxWarps = 8;
@@ -42,11 +44,7 @@ struct TcCfg {
     static constexpr int kPTerms = F32 ? 3 : 1;
     static constexpr int kTileBytes = kTcKeys * D * 2;                       // a K or V tile
     static constexpr int kQTileBytes = 128 * D * 2;
-    // query tiles; also holds what the groups exchange: 128 D f32 at the end of an item, and for stacked items
-    // partial scores (behind the first tile) and 2 x 96 x D f32 at the end
-    static constexpr int kXchgBytes = F32 ? 3 * 64 * 32 * 4 : 0;             // partial scores of a group
-    static constexpr int kQTilesBytes = (F32 ? 3 : 2) * kQTileBytes;
-    static constexpr int kQBytes = kQTilesBytes > kQTileBytes + 2 * kXchgBytes ? kQTilesBytes : kQTileBytes + 2 * kXchgBytes;
+    static constexpr int kQBytes = (F32 ? 3 : 2) * kQTileBytes;              // also holds what the groups exchange at the end of an item
     static constexpr int kStages = D == 128 ? (F32 ? 4 : 5) : 8;
     static constexpr int kSmem = kQBytes + kStages * kTileBytes + 3072;
     static constexpr int kRows = F32 ? 128 : 256;                            // rows of an item
@@ -234,11 +232,19 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-// First column (of a slot's 128) of the bf16 weights of half `h` and term `term`.  Three terms of 64 keys take 96 columns, so
-// the second half's last two terms are written over the first half's once that has been multiplied.
-__device__ __forceinline__ uint32_t weight_columns(int h, int term, bool terms3) {
+// First column, counted from a slot's scores, of the bf16 weights of half `h` and term `term`.  Three terms of 64 keys take 96 of the
+// 128 columns; the second half's last two terms go to columns that a 64-wide accumulator leaves free, or with D = 128 over the first
+// half's once that has been multiplied (p_free).
+template <int D>
+__device__ __forceinline__ constexpr uint32_t weight_columns(int h, int term, bool terms3) {
     if (!terms3) return h * 32;
-    return h == 0 ? term * 32 : (term == 0 ? 96 : (term - 1) * 32);
+    if (h == 0) return term * 32;
+    return term == 0 ? 96 : (D == 64 ? 256 + 64 : 0) + (term - 1) * 32;
+}
+// Two f32 in truncated bf16 (their upper halves), the first in the low half; the remainders are exact
+__device__ __forceinline__ uint32_t cut_bf16(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
+__device__ __forceinline__ F2 cut_rest(float lo, float hi) {
+    return fma2(F2(__uint_as_float(__float_as_uint(lo) & 0xFFFF0000u), __uint_as_float(__float_as_uint(hi) & 0xFFFF0000u)), F2(-1.0f, -1.0f), F2(lo, hi));
 }
 
 struct TcShared {
@@ -272,7 +278,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if (threadIdx.x == 0) {
         for (int i = 0; i < kNst; ++i) {
             mbar_init(smem_u32(&sh.full[i]), 1);
-            mbar_init(smem_u32(&sh.empty[i]), 1);
+            mbar_init(smem_u32(&sh.empty[i]), 2);      // both slots, or one slot twice
             mbar_init(smem_u32(&sh.raw[i]), 1);
         }
         for (int s = 0; s < 2; ++s) {
@@ -325,10 +331,22 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         uint32_t pos = 0, issued = 0, raw_last = 0, raw_phase = 0;      // per stage: its last tile went to `raw`; parity of those
         bool ok = true;
         const int box = min(block, kTcKeys);
+        TcWalk<Cfg::kRows, F32> walk(p, q_starts, seq_lens);
+        TcItem it;
         uint32_t k_item = 0;
-        for (TcItem* item; ok && (item = next_item(k_item)) != nullptr; ++k_item) {
-            const TcItem it = *item;
-            release_item(k_item);
+        auto deal = [&]() {
+            const uint32_t slot = k_item % kTcItemSlots;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.item_empty[slot]), ((k_item / kTcItemSlots) & 1) ^ 1, err, kErrProducerWait))) return false;
+            if (lane == 0) sh.items[slot] = it;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.item_full[slot]));
+            ++k_item;
+            return true;
+        };
+        for (int64_t index = blockIdx.x; ok && walk.get(index, it, err); index += gridDim.x) {
+            if (it.nt == 0) continue;
+            ok = deal();
+            if (!ok) break;
             const TcOrder order(pos, it);
             const uint32_t* table = tables + int64_t(it.seq) * p.sh.max_blocks_per_seq;
             const int end = min(it.max_limit, (it.t0 + it.nt) * kTcKeys);
@@ -365,102 +383,99 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
             pos += 2 * it.nt;
         }
+        if (ok) {
+            it.nt = -1;
+            deal();
+        }
         if (!ok)      // the consumer is gone: let this warp's own copies land before the memory is given back
             for (uint32_t at = issued > kNst ? issued - kNst : 0; at < issued; ++at) {
                 const uint32_t stage = at % kNst;
                 if ((raw_last >> stage) & 1) mbar_wait(smem_u32(&sh.raw[stage]), ((raw_phase >> stage) & 1) ^ 1, err, kErrProducerWait);
                 else mbar_wait(smem_u32(&sh.full[stage]), (at / kNst) & 1, err, kErrProducerWait);
             }
-    } else if (warp == 9) {
-        // ------------------------------------------------------------ MMA issue (one elected thread)
+    } else if (warp <= 10) {
+        // ------------------------------------------------------------ MMA issue for slot `s` (one elected thread)
         constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((kTcKeys >> 3) << 17) | ((128 >> 4) << 24);
         constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((D >> 3) << 17) | ((128 >> 4) << 24);
-        uint32_t pos = 0, p_phase[2] = {0, 0}, q_phase = 0;
+        const int s = warp - 9;
+        const uint32_t d_s = tmem + s * 128, d_o = tmem + 256 + s * 128;
+        uint32_t pos = 0, p_phase = 0, k_item = 0;
         bool ok = true;
-        auto wait = [&](uint32_t bar, uint32_t parity) { return bool(__all_sync(0xffffffffu, mbar_wait(bar, parity, err, kErrMmaWait))); };
-        uint32_t k_item = 0;
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return bool(__all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, err, kErrMmaWait))); };
         for (TcItem* item; ok && (item = next_item(k_item)) != nullptr; ++k_item) {
             const TcOrder order(pos, *item);
             const int n = item->nt;
-            const bool split = item->split, stack = item->stack;
+            const bool split = item->split, stack = F32 && item->stack;
             release_item(k_item);
             pos += 2 * n;
-            ok = wait(smem_u32(&sh.q_full), q_phase & 1);
-            ++q_phase;
+            ok = wait(&sh.q_full, k_item & 1);
             tc5_fence_after();
-            auto scores = [&](int s, int t, bool last_use) {
-                const uint32_t at = order.k(t), stage = at % kNst;
-                if (!wait(smem_u32(&sh.full[stage]), (at / kNst) & 1)) return false;
-                tc5_fence_after();
-                const uint64_t k_desc = umma_desc_k128(ring_addr + stage * Cfg::kTileBytes);
-                const uint64_t q_desc = umma_desc_k128(q_addr + (F32 || split ? 0 : s) * Cfg::kQTileBytes);
-                const uint32_t d = tmem + s * 128;
-                // (no condition may stand inside the elected thread's block: it would cost hundreds of clocks a product)
-                auto multiply = [&](auto terms) {
+            const uint64_t q_desc = umma_desc_k128(q_addr + (F32 || split ? 0 : s) * Cfg::kQTileBytes);
+            const int step = split ? 2 : 1;
+            // a stage is free when both slots are done with it; a slot that has it for itself says so twice
+            auto release = [&](uint32_t stage) {
+                tc5_commit(smem_u32(&sh.empty[stage]));
+                if (split) tc5_commit(smem_u32(&sh.empty[stage]));
+            };
+            for (int t = split ? s : 0; ok && t < n; t += step) {
+                {
+                    const uint32_t at = order.k(t), stage = at % kNst;
+                    ok = wait(&sh.full[stage], (at / kNst) & 1);
+                    if (!ok) break;
+                    tc5_fence_after();
+                    const uint64_t k_desc = umma_desc_k128(ring_addr + stage * Cfg::kTileBytes);
                     if (elect_one()) {
 #pragma unroll
-                        for (int term = 0; term < decltype(terms)::value; ++term)
+                        for (int term = 0; term < Cfg::kQTerms; ++term)
 #pragma unroll
                             for (int kk = 0; kk < D / 16; ++kk) {
                                 const uint32_t off = ((kk / 4) * kHalfBytes + (kk % 4) * 32) >> 4;
-                                umma_bf16_ss(d, q_desc + off + ((term * Cfg::kQTileBytes) >> 4), k_desc + off, kIdescS, term + kk > 0);
+                                umma_bf16_ss(d_s, q_desc + off + ((term * Cfg::kQTileBytes) >> 4), k_desc + off, kIdescS, term + kk > 0);
                             }
-                        if (last_use) tc5_commit(smem_u32(&sh.empty[stage]));
                         tc5_commit(smem_u32(&sh.s_full[s]));
+                        release(stage);
                     }
-                };
-                if (F32 && stack) multiply(std::integral_constant<int, 1>());
-                else multiply(std::integral_constant<int, Cfg::kQTerms>());
-                __syncwarp();
-                return true;
-            };
-            auto values = [&](int s, int t, bool first, bool last_use, bool last) {
-                const uint32_t at = order.v(t), stage = at % kNst;
-                if (!wait(smem_u32(&sh.full[stage]), (at / kNst) & 1)) return false;
-                const uint32_t v_tile = ring_addr + stage * Cfg::kTileBytes, d = tmem + 256 + s * 128, a = tmem + s * 128;
-                const uint64_t v_desc = umma_desc_mn128(v_tile, kHalfBytes);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {      // the weights arrive in halves of 64 keys
-                    if (!wait(smem_u32(&sh.p_full[s][h]), p_phase[s] & 1)) return false;
-                    tc5_fence_after();
-                    auto multiply = [&](auto terms) {
-                        constexpr int kTerms = decltype(terms)::value;
-                        if (elect_one()) {
-#pragma unroll
-                            for (int term = 0; term < kTerms; ++term)
-#pragma unroll
-                                for (int kk = 0; kk < 4; ++kk)
-                                    umma_bf16_ts(d, a + weight_columns(h, term, kTerms == 3) + kk * 8, v_desc + (((h * 4 + kk) * 2048) >> 4),
-                                                 kIdescO, !(first && h + term + kk == 0));
-                            if (h == 0 && kTerms == 3) tc5_commit(smem_u32(&sh.p_free[s]));
-                            if (h == 1 && last_use) tc5_commit(smem_u32(&sh.empty[stage]));
-                            if (h == 1 && last) tc5_commit(smem_u32(&sh.o_full[s]));
-                        }
-                    };
-                    if (F32 && stack) multiply(std::integral_constant<int, 1>());
-                    else multiply(std::integral_constant<int, Cfg::kPTerms>());
                     __syncwarp();
                 }
-                ++p_phase[s];
-                return true;
-            };
-            if (split) {
-                ok = ok && scores(0, 0, true);
-                if (n > 1) ok = ok && scores(1, 1, true);
-                for (int t = 0; ok && t < n; ++t) {
-                    ok = values(t & 1, t, t < 2, true, t + 2 >= n);
-                    if (ok && t + 2 < n) ok = scores(t & 1, t + 2, true);
-                }
-            } else {
-                ok = ok && scores(0, 0, false) && scores(1, 0, true);
-                for (int t = 0; ok && t < n; ++t)
-                    for (int s = 0; ok && s < 2; ++s) {
-                        ok = values(s, t, t == 0, s == 1, t + 1 == n);
-                        if (ok && t + 1 < n) ok = scores(s, t + 1, s == 1);
+                const uint32_t at = order.v(t), stage = at % kNst;
+                ok = wait(&sh.full[stage], (at / kNst) & 1);
+                const uint64_t v_desc = umma_desc_mn128(ring_addr + stage * Cfg::kTileBytes, kHalfBytes);
+                const uint32_t keep = t >= step;            // not the first product of this item
+                const bool last = t + step >= n;
+                auto multiply = [&](auto half, auto terms) {
+                    constexpr int kTerms = decltype(terms)::value, H = decltype(half)::value;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk)
+                                umma_bf16_ts(d_o, d_s + weight_columns<D>(H, term, kTerms == 3) + kk * 8, v_desc + (((H * 4 + kk) * 2048) >> 4), kIdescO,
+                                             H + term + kk > 0 ? 1u : keep);
+                        if (H == 0 && kTerms == 3 && D == 128) tc5_commit(smem_u32(&sh.p_free[s]));
+                        if (H == 1) {
+                            if (last) tc5_commit(smem_u32(&sh.o_full[s]));
+                            release(stage);
+                        }
                     }
+                    __syncwarp();
+                };
+                using One = std::integral_constant<int, 1>;
+                using Zero = std::integral_constant<int, 0>;
+                using All = std::integral_constant<int, Cfg::kPTerms>;
+                ok = ok && wait(&sh.p_full[s][0], p_phase & 1);
+                if (!ok) break;
+                tc5_fence_after();
+                if (F32 && stack) multiply(Zero(), One());
+                else multiply(Zero(), All());
+                ok = wait(&sh.p_full[s][1], p_phase & 1);
+                if (!ok) break;
+                tc5_fence_after();
+                if (F32 && stack) multiply(One(), One());
+                else multiply(One(), All());
+                ++p_phase;
             }
         }
-    } else if (warp == 10) {
+    } else {
         // ------------------------------------------------------------ V tiles with masked keys
         uint32_t pos = 0, raw_phase = 0, k_item = 0;
         bool ok = true;
@@ -479,24 +494,27 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 bool found = false;
                 // rows some query must not see, then rows nobody sees; 8 pieces of 16 bytes are a row of a half
                 const int r0 = max(0, it.min_limit - k0), r1 = min(kTcKeys, it.max_limit - k0);
-                for (int c = r0 * 8 + lane; c < kTcKeys * 8; c += 32) {
 #pragma unroll
-                    for (int h = 0; h < kHalves; ++h) {
-                        uint4* piece = reinterpret_cast<uint4*>(tile + h * kHalfBytes + c * 16);
-                        if (c >= r1 * 8) {
-                            *piece = make_uint4(0, 0, 0, 0);
-                            continue;
-                        }
-                        uint4 v = *piece;
-                        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-                        bool bad = false;
+                for (int h = 0; h < kHalves; ++h) {
+                    uint4* pieces = reinterpret_cast<uint4*>(tile + h * kHalfBytes);
+                    for (int c0 = r0 * 8; c0 < r1 * 8; c0 += 256) {
+                        uint4 v[8];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if ((w[k] & 0x7F80u) == 0x7F80u) { w[k] &= 0xFFFF0000u; bad = true; }
-                            if ((w[k] & 0x7F800000u) == 0x7F800000u) { w[k] &= 0x0000FFFFu; bad = true; }
+                        for (int k = 0; k < 8; ++k) v[k] = c0 + k * 32 + lane < r1 * 8 ? pieces[c0 + k * 32 + lane] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            uint32_t* w = reinterpret_cast<uint32_t*>(&v[k]);
+                            bool bad = false;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if ((w[e] & 0x7F80u) == 0x7F80u) { w[e] &= 0xFFFF0000u; bad = true; }
+                                if ((w[e] & 0x7F800000u) == 0x7F800000u) { w[e] &= 0x0000FFFFu; bad = true; }
+                            }
+                            if (bad) { pieces[c0 + k * 32 + lane] = v[k]; found = true; }
                         }
-                        if (bad) { *piece = v; found = true; }
                     }
+#pragma unroll 8
+                    for (int c = r1 * 8 + lane; c < kTcKeys * 8; c += 32) pieces[c] = make_uint4(0, 0, 0, 0);
                 }
                 if (found) item->nonfinite = 1;
                 fence_proxy_async();
@@ -504,25 +522,6 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 if (lane == 0) mbar_arrive(smem_u32(&sh.full[stage]));
             }
         }
-    } else {
-        // ------------------------------------------------------------ items
-        TcWalk<Cfg::kRows, F32> walk(p, q_starts, seq_lens);
-        TcItem it;
-        uint32_t k = 0;
-        auto deal = [&]() {
-            const uint32_t slot = k % kTcItemSlots;
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.item_empty[slot]), ((k / kTcItemSlots) & 1) ^ 1, err, kErrProducerWait))) return false;
-            if (lane == 0) sh.items[slot] = it;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sh.item_full[slot]));
-            ++k;
-            return true;
-        };
-        bool ok = true;
-        for (int64_t index = blockIdx.x; ok && walk.get(index, it, err); index += gridDim.x)
-            if (it.nt > 0) ok = deal();
-        it.nt = -1;
-        if (ok) deal();
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -544,32 +543,50 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             const int limit = live ? it.len - it.n + token + 1 : 0;
             const int64_t out_row = (int64_t(it.start) + token) * p.sh.num_q_heads + head;
 
-            // queries into shared memory, 128-byte swizzled; a shared tile is written by both groups, half a row each
+            // Queries into shared memory, 128-byte swizzled.  A warp reads whole rows (a lane 8 elements of one), several before it
+            // uses the first; a tile that both slots use is shared out over all eight warps.
             {
-                const T* src = q + (int64_t(it.start) + token) * p.sh.row_stride + int64_t(head) * D;
-                const int pieces = D / 8, per = it.split ? pieces / 2 : pieces;
-                unsigned char* dst = q_smem + (it.split ? 0 : wg) * Cfg::kQTileBytes;
-#pragma unroll 4
-                for (int j = 0; j < per; ++j) {
-                    const int piece = (it.split ? wg * per : 0) + j;
-                    const int at = (piece / 8) * kHalfBytes + row * 128 + (((piece % 8) ^ (row & 7)) << 4);
-                    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                    if (live && busy) {
-                        load_f32<T, 8>(src + piece * 8, x);
+                constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces, kBatch = F32 ? 2 : 8;
+                const int per = stack ? 4 : (it.split ? 16 : 32), base = (it.split ? warp : warp & 3) * per;
+                const int first = (it.split ? 0 : wg * 128) + base, count = min(per, it.rows - first);      // rows of this warp (<= 0: none)
+                // place of the row base + lane; rows that the item does not have read its first row and are set to zero
+                const int at = it.row0 + (lane < count ? first + lane : 0), tok = at / p.group;
+                const int64_t from = (int64_t(it.start) + tok) * p.sh.row_stride + int64_t(it.kvh * p.group + at - tok * p.group) * D;
+                const int piece = lane % kPieces;
+                unsigned char* dst = q_smem + (it.split ? 0 : wg) * Cfg::kQTileBytes + (piece / 8) * kHalfBytes;
+                for (int j0 = lane / kPieces; j0 < per; j0 += kBatch * kAtOnce) {
+                    using Raw = Pack<T, 8>;
+                    Raw raw[kBatch];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) x[k] *= p.q_sign;
+                    for (int b = 0; b < kBatch; ++b) {
+                        const int64_t f = __shfl_sync(0xffffffffu, static_cast<long long>(from), (j0 + b * kAtOnce) & 31);
+                        const uint4* src = reinterpret_cast<const uint4*>(q + f + piece * 8);
+#pragma unroll
+                        for (int k = 0; k < int(sizeof(Raw) / 16); ++k) reinterpret_cast<uint4*>(&raw[b])[k] = __ldg(src + k);
                     }
 #pragma unroll
-                    for (int term = 0; term < Cfg::kQTerms; ++term) {
-                        uint32_t w[4];
+                    for (int b = 0; b < kBatch; ++b) {
+                        const int j = j0 + b * kAtOnce, to = base + j, sw = ((piece % 8) ^ (to & 7)) << 4;
+                        const float sign = j < count ? p.q_sign : 0.0f;
+                        float x[8];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            w[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
-                            x[2 * k] -= bf16_lo(w[k]);
-                            x[2 * k + 1] -= bf16_hi(w[k]);
+                        for (int k = 0; k < 8; ++k) x[k] = j < count ? as_f32(raw[b].v[k]) * sign : 0.0f;
+#pragma unroll
+                        for (int term = 0; term < Cfg::kQTerms; ++term) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                w[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+                                x[2 * k] -= bf16_lo(w[k]);
+                                x[2 * k + 1] -= bf16_hi(w[k]);
+                            }
+                            unsigned char* tile = dst + term * Cfg::kQTileBytes;
+                            if (j < per) *reinterpret_cast<uint4*>(tile + to * 128 + sw) = make_uint4(w[0], w[1], w[2], w[3]);
+                            if (stack && j < per) {
+                                *reinterpret_cast<uint4*>(tile + (32 + to) * 128 + sw) = make_uint4(w[0], w[1], w[2], w[3]);
+                                *reinterpret_cast<uint4*>(tile + (64 + to) * 128 + sw) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
                         }
-                        if (!stack) *reinterpret_cast<uint4*>(dst + term * Cfg::kQTileBytes + at) = make_uint4(w[0], w[1], w[2], w[3]);
-                        else if (term == (warp & 3)) *reinterpret_cast<uint4*>(dst + at) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
                 fence_proxy_async();
@@ -595,108 +612,157 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     continue;
                 }
                 tc5_fence_after();
-                float s[128];
-                float mx[4];
-                {
-                    uint32_t raw[4][32];
-                    tmem_ld_32x32(t_s, raw[0]);
-                    tmem_ld_32x32(t_s + 32, raw[1]);
-                    tmem_ld_32x32(t_s + 64, raw[2]);
-                    tmem_ld_32x32(t_s + 96, raw[3]);
-                    tmem_ld_wait();
+                const bool masked = t >= masked_from;                          // the same for all lanes, as the collective loads and stores need
+                const int visible = limit - k0 - t * kTcKeys;
+                // Running maximum; true when O was rescaled.  m may stay behind by 2^8 in the weight.
+                auto raise = [&](float top) {
+                    if (done == 0) {
+                        m = top;
+                    } else if (__any_sync(0xffffffffu, (top - m) * c > 8.0f)) {
+                        const float m_new = fmaxf(m, top);
+                        const float f = m_new == m ? 1.0f : ex2((m - m_new) * c);
+                        m = m_new;
+                        l *= f;
 #pragma unroll
-                    for (int k = 0; k < 128; ++k) s[k] = __uint_as_float(raw[k / 32][k % 32]);
-                }
-                if constexpr (F32) {
-                    if (stack) {      // scores are the sum of the three terms' partial scores, added in the same order by all three warps
-                        float* xs = reinterpret_cast<float*>(q_smem + Cfg::kQTileBytes + wg * Cfg::kXchgBytes);
+                        for (int g = 0; g < D / 16; ++g) {
+                            uint32_t o[16];
+                            tmem_ld_32x16(t_o + g * 16, o);
+                            tmem_ld_wait();
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                            for (int k = 0; k < 64; ++k) xs[((warp & 3) * 64 + k) * 32 + lane] = s[h * 64 + k];
-                            bar_sync(2 + wg, 96);
-#pragma unroll
-                            for (int k = 0; k < 64; ++k) s[h * 64 + k] = (xs[(128 + k) * 32 + lane] + xs[(64 + k) * 32 + lane]) + xs[k * 32 + lane];
-                            bar_sync(2 + wg, 96);
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            tmem_st_32x16(t_o + g * 16, o);
                         }
                     }
-                }
-                if (t >= masked_from) {
-                    const int visible = limit - k0 - t * kTcKeys;
-#pragma unroll
-                    for (int k = 0; k < 128; ++k)
-                        if (k >= visible) s[k] = -INFINITY;
-                }
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    mx[g] = fmaxf(s[g], s[g + 4]);
-#pragma unroll
-                    for (int k = 8; k < 128; k += 8) mx[g] = fmaxf(fmaxf(mx[g], s[k + g]), s[k + 4 + g]);
-                }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                if (done == 0) {
-                    m = top;
-                } else if (__any_sync(0xffffffffu, (top - m) * c > 8.0f)) {
-                    const float m_new = fmaxf(m, top);
-                    const float f = m_new == m ? 1.0f : ex2((m - m_new) * c);
-                    m = m_new;
-                    l *= f;
-#pragma unroll
-                    for (int g = 0; g < D / 16; ++g) {
-                        uint32_t o[16];
-                        tmem_ld_32x16(t_o + g * 16, o);
+                };
+                F2 sum[2] = {F2(0.0f, 0.0f), F2(0.0f, 0.0f)};
+                if constexpr (!F32) {
+                    float s[128];      // the whole row stays in registers
+                    {
+                        uint32_t raw[4][32];
+                        tmem_ld_32x32(t_s, raw[0]);
+                        tmem_ld_32x32(t_s + 32, raw[1]);
+                        tmem_ld_32x32(t_s + 64, raw[2]);
+                        tmem_ld_32x32(t_s + 96, raw[3]);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                        tmem_st_32x16(t_o + g * 16, o);
+                        for (int k = 0; k < 128; ++k) s[k] = __uint_as_float(raw[k / 32][k % 32]);
                     }
-                }
-                const float mc = m == -INFINITY ? 0.0f : m * c;
-                const F2 c2(c, c), mc2(-mc, -mc);
-                F2 sum[2] = {F2(0.0f, 0.0f), F2(0.0f, 0.0f)};
+                    if (masked) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    constexpr int kParts = F32 ? 3 : 1;
+                        for (int k = 0; k < 128; ++k)
+                            if (k >= visible) s[k] = -INFINITY;
+                    }
+                    float mx[4];
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {          // 32 keys, 16 columns a term
-                        uint32_t w[kParts][16];
+                    for (int g = 0; g < 4; ++g) {
+                        mx[g] = fmaxf(s[g], s[g + 4]);
 #pragma unroll
-                        for (int k = 0; k < 32; k += 2) {
-                            const int at = h * 64 + g * 32 + k;
-                            float a, b;
-                            fma2(F2(s[at], s[at + 1]), c2, mc2).get(a, b);
-                            a = ex2(a);
-                            b = ex2(b);
-                            sum[(k / 2) & 1] = add2(sum[(k / 2) & 1], F2(a, b));
-                            w[0][k / 2] = pack_bf16(a, b);
-                            if constexpr (F32) {
-                                const float a2 = a - bf16_lo(w[0][k / 2]), b2 = b - bf16_hi(w[0][k / 2]);
-                                w[1][k / 2] = pack_bf16(a2, b2);
-                                w[2][k / 2] = pack_bf16(a2 - bf16_lo(w[1][k / 2]), b2 - bf16_hi(w[1][k / 2]));
+                        for (int k = 8; k < 128; k += 8) mx[g] = fmaxf(fmaxf(mx[g], s[k + g]), s[k + 4 + g]);
+                    }
+                    raise(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+                    const float mc = m == -INFINITY ? 0.0f : m * c;
+                    const F2 c2(c, c), mc2(-mc, -mc);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int k = 0; k < 32; k += 2) {
+                                const int at = h * 64 + g * 32 + k;
+                                float a, b;
+                                fma2(F2(s[at], s[at + 1]), c2, mc2).get(a, b);
+                                a = ex2(a);
+                                b = ex2(b);
+                                sum[(k / 2) & 1] = add2(sum[(k / 2) & 1], F2(a, b));
+                                w[k / 2] = pack_bf16(a, b);
                             }
+                            tmem_st_32x16(t_s + h * 32 + g * 16, w);
                         }
-                        if constexpr (F32) {
+                        tmem_st_wait();
+                        tc5_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[wg][h]));
+                    }
+                } else {
+                    // The scores are read twice, 32 at a time: a row of them and its three terms do not fit the registers together.
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t raw[2][32];
+                        tmem_ld_32x32(t_s + h * 64, raw[0]);
+                        tmem_ld_32x32(t_s + h * 64 + 32, raw[1]);
+                        tmem_ld_wait();
+                        if (masked) {
+#pragma unroll
+                            for (int k = 0; k < 64; ++k)
+                                if (h * 64 + k >= visible) raw[k / 32][k % 32] = 0xFF800000u;
+                        }
+                        if (masked) {
+                            tmem_st_32x32(t_s + h * 64, raw[0]);
+                            tmem_st_32x32(t_s + h * 64 + 32, raw[1]);
+                        }
+                        float mx[4];
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            mx[g] = __uint_as_float(raw[0][g]);
+#pragma unroll
+                            for (int k = 4; k < 64; k += 4) mx[g] = fmaxf(mx[g], __uint_as_float(raw[(k + g) / 32][(k + g) % 32]));
+                        }
+                        top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+                    }
+                    tmem_st_wait();
+                    raise(top);
+                    const float mc = m == -INFINITY ? 0.0f : m * c;
+                    const F2 c2(c, c), mc2(-mc, -mc);
+                    // a half's terms are stored when its own scores, and those that they overwrite, are in registers
+                    uint32_t sc[4][32];
+                    tmem_ld_32x32(t_s, sc[0]);
+                    tmem_ld_32x32(t_s + 32, sc[1]);
+                    tmem_ld_32x32(t_s + 64, sc[2]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (h == 1) {
+                            tmem_ld_32x32(t_s + 96, sc[3]);
+                            tmem_ld_wait();
+                        }
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {          // 32 keys, 16 columns a term
+                            const uint32_t (&now)[32] = sc[h * 2 + g];
+                            uint32_t w[3][16];
+#pragma unroll
+                            for (int k = 0; k < 32; k += 2) {
+                                float a, b;
+                                fma2(F2(__uint_as_float(now[k]), __uint_as_float(now[k + 1])), c2, mc2).get(a, b);
+                                a = ex2(a);
+                                b = ex2(b);
+                                sum[(k / 2) & 1] = add2(sum[(k / 2) & 1], F2(a, b));
+                                w[0][k / 2] = cut_bf16(a, b);
+                                cut_rest(a, b).get(a, b);
+                                w[1][k / 2] = cut_bf16(a, b);
+                                cut_rest(a, b).get(a, b);
+                                w[2][k / 2] = cut_bf16(a, b);
+                            }
                             if (stack) {
                                 if ((warp & 3) == 0) tmem_st_32x16(t_s + h * 32 + g * 16, w[0]);
                                 else if ((warp & 3) == 1) tmem_st_32x16(t_s + h * 32 + g * 16, w[1]);
                                 else tmem_st_32x16(t_s + h * 32 + g * 16, w[2]);
                             } else {
-                                tmem_st_32x16(t_s + weight_columns(h, 0, true) + g * 16, w[0]);
-                                if (h == 1 && g == 0) {      // the columns of the first half's last two terms
+                                tmem_st_32x16(t_s + weight_columns<D>(h, 0, true) + g * 16, w[0]);
+                                if (D == 128 && h == 1 && g == 0) {      // the columns of the first half's last two terms
                                     ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.p_free[wg]), f_phase & 1, err, kErrEpilogueWait)) && ok;
                                     tc5_fence_after();
                                 }
-                                tmem_st_32x16(t_s + weight_columns(h, 1, true) + g * 16, w[1]);
-                                tmem_st_32x16(t_s + weight_columns(h, 2, true) + g * 16, w[2]);
+                                tmem_st_32x16(t_s + weight_columns<D>(h, 1, true) + g * 16, w[1]);
+                                tmem_st_32x16(t_s + weight_columns<D>(h, 2, true) + g * 16, w[2]);
                             }
-                        } else {
-                            tmem_st_32x16(t_s + h * 32 + g * 16, w[0]);
                         }
+                        tmem_st_wait();
+                        tc5_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[wg][h]));
                     }
-                    tmem_st_wait();
-                    tc5_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[wg][h]));
                 }
                 ++s_phase;
                 f_phase += !stack;
@@ -712,13 +778,15 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
             if (!ok && lane == 0) sh.abort = 1;      // both groups still meet at this item's barriers, then both leave
 
-            // ---- results.  `emit` finishes some columns of a row
+            // ---- results.  Rows go through shared memory (the query tiles are done with), so that a warp writes whole rows:
+            // row r of a staging area of W-element rows keeps its 16-byte piece j at piece j ^ (r & 7).
             const bool direct = it.nchunks == 1;
             bool patch = false;
-            auto emit = [&](int col, auto& o, float factor) {
+            // finishes N columns of the row with this place and reach: non-finite values that the MMAs did not get, where the row sees them
+            auto finish = [&](int64_t to_row, int reach, int col, auto& o) {
                 constexpr int N = sizeof(o) / sizeof(float);
-                if (patch) {      // non-finite values that the MMAs did not get, for the rows that see them
-                    const int from = max(it.min_limit, it.t0 * kTcKeys), to = min(limit, (it.t0 + it.nt) * kTcKeys);
+                if (patch) {
+                    const int from = max(it.min_limit, k0), to = min(reach, k0 + nt * kTcKeys);
                     for (int j = from; j < to; ++j) {
                         const uint32_t blk = tables[int64_t(it.seq) * p.sh.max_blocks_per_seq + j / block];
                         if (blk >= uint32_t(p.sh.num_blocks)) continue;
@@ -728,36 +796,65 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                             if ((v[k] & 0x7F80u) == 0x7F80u) o[k] += bf16_bits_to_f32(v[k]);
                     }
                 }
+                if (direct) store_f32<T, N>(out + to_row * D + col, o);
+                else store_f32<float, N>(part_o + (to_row * p.max_chunks + it.chunk) * D + col, o);
+            };
+            auto row_of = [&](int j) { return static_cast<int64_t>(__shfl_sync(0xffffffffu, static_cast<long long>(out_row), j)); };
+            auto reach_of = [&](int j) { return __shfl_sync(0xffffffffu, limit, j); };
+            // The rows [j, j + 32 / kLanes, ...) of a warp's 32, kLanes lanes of N columns to a row: all in flight together.  `get`
+            // reads the staged columns of a row.
+            auto write_rows = [&](auto lanes, auto columns, int col0, auto get) {
+                constexpr int kLanes = decltype(lanes)::value, N = decltype(columns)::value, kAtOnce = 32 / kLanes, kSteps = 32 / kAtOnce;
+                constexpr int kBatch = kSteps < 8 ? kSteps : 8;
+                const int col = lane % kLanes * N;
+#pragma unroll 1
+                for (int j0 = 0; j0 < 32; j0 += kBatch * kAtOnce) {
+                    float o[kBatch][N];
 #pragma unroll
-                for (int k = 0; k < N; ++k) o[k] *= factor;
-                if (!live) return;
-                if (direct) {
+                    for (int b = 0; b < kBatch; ++b) get(j0 + b * kAtOnce + lane / kLanes, col, o[b]);
 #pragma unroll
-                    for (int k = 0; k < N; k += 8) {
-                        float y[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = o[k + e];
-                        store_f32<T, 8>(out + out_row * D + col + k, y);
+                    for (int b = 0; b < kBatch; ++b) {
+                        const int j = j0 + b * kAtOnce + lane / kLanes, reach = reach_of(j);
+                        const int64_t to_row = row_of(j);
+                        if (reach > 0) finish(to_row, reach, col0 + col, o[b]);
                     }
-                } else {
-                    float* dst = part_o + (out_row * p.max_chunks + it.chunk) * D + col;
-#pragma unroll
-                    for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(dst + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                 }
             };
+            auto staged = [&](unsigned char* area, int width, int rr, int col) -> float4* {
+                return reinterpret_cast<float4*>(area + (size_t(rr) * width + (((col >> 2) ^ (rr & 7)) << 2)) * 4);
+            };
             if (!it.split) {
-                const float inv = direct ? 1.0f / l : 1.0f;
-                patch = *reinterpret_cast<volatile uint32_t*>(&item->nonfinite) != 0;        // set before the products that o_full stands for
-                for (int g = 0; g < (busy ? D / 32 : 0); ++g) {
-                    uint32_t raw[32];
-                    float o[32];
-                    tmem_ld_32x32(t_o + g * 32, raw);
-                    tmem_ld_wait();
+                if constexpr (!F32) {
+                    patch = *reinterpret_cast<volatile uint32_t*>(&item->nonfinite) != 0;      // set before the products that o_full stands for
+                    const float inv = direct ? 1.0f / l : 1.0f;
+                    // 32 rows of 64 columns at a time in this warp's part of its group's query tile (D = 64: of 32 columns)
+                    constexpr int kCols = D / 2;
+                    unsigned char* area = q_smem + wg * Cfg::kQTileBytes + (warp & 3) * (Cfg::kQTileBytes / 4);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(raw[k]);
-                    emit(g * 32, o, inv);
+                    for (int part = 0; part < 2; ++part) {
+                        if (busy) {
+#pragma unroll
+                            for (int g = 0; g < kCols / 32; ++g) {
+                                uint32_t raw[32];
+                                tmem_ld_32x32(t_o + part * kCols + g * 32, raw);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int k = 0; k < 32; k += 4)
+                                    *staged(area, kCols, lane, g * 32 + k) =
+                                        make_float4(__uint_as_float(raw[k]) * inv, __uint_as_float(raw[k + 1]) * inv,
+                                                    __uint_as_float(raw[k + 2]) * inv, __uint_as_float(raw[k + 3]) * inv);
+                            }
+                        }
+                        __syncwarp();
+                        if (busy)
+                            write_rows(std::integral_constant<int, kCols / 8>(), std::integral_constant<int, 8>(), part * kCols, [&](int j, int col, float (&o)[8]) {
+                            const float4 x = *staged(area, kCols, j, col), y = *staged(area, kCols, j, col + 4);
+                            o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w; o[4] = y.x; o[5] = y.y; o[6] = y.z; o[7] = y.w;
+                        });
+                        __syncwarp();
+                    }
+                    if (!direct && live) part_ml[out_row * p.max_chunks + it.chunk] = make_float2(m * c, l);
                 }
-                if (!direct && live) part_ml[out_row * p.max_chunks + it.chunk] = make_float2(m * c, l);
                 tc5_fence_before();
                 bar_sync(1, kTcSoftmaxWarps * 32);      // both groups are done with their query tiles
             } else {
@@ -772,7 +869,8 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 const float f0 = m0 == -INFINITY ? 0.0f : ex2((m0 - mt) * c), f1 = m1 == -INFINITY ? 0.0f : ex2((m1 - mt) * c);
                 const float lt = fmaf(sh.xl[0][lane_row], f0, sh.xl[1][lane_row] * f1);
                 const float inv = direct ? 1.0f / lt : 1.0f;
-                float* xo = reinterpret_cast<float*>(q_smem);
+                const float mine = (wg == 0 ? f0 : f1) * inv;
+                if (!direct && live && warp == (stack ? 0 : warp & 3)) part_ml[out_row * p.max_chunks + it.chunk] = make_float2(mt * c, lt);
                 if (stack) {
                     if (busy) {
 #pragma unroll
@@ -783,51 +881,76 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                                 tmem_ld_wait();
                             }
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) xo[(wg * D + g * 32 + k) * 96 + row] = done > 0 ? __uint_as_float(raw[k]) : 0.0f;
+                            for (int k = 0; k < 32; k += 4)
+                                *staged(q_smem, D, wg * 96 + row, g * 32 + k) =
+                                    done > 0 ? make_float4(__uint_as_float(raw[k]) * mine, __uint_as_float(raw[k + 1]) * mine,
+                                                           __uint_as_float(raw[k + 2]) * mine, __uint_as_float(raw[k + 3]) * mine)
+                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         }
                     }
                     bar_sync(1, kTcSoftmaxWarps * 32);
-                    constexpr int kCols = D / 8;        // columns of a warp
-                    float o[kCols];
+                    constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;
 #pragma unroll
-                    for (int k = 0; k < kCols; ++k) {
-                        const float* x0 = xo + (warp * kCols + k) * 96 + lane;
-                        const float* x1 = x0 + D * 96;
-                        o[k] = fmaf((x0[64] + x0[32]) + x0[0], f0, ((x1[64] + x1[32]) + x1[0]) * f1);
+                    for (int j = 0; j < 4; j += kAtOnce) {
+                        const int rr = warp * 4 + j + lane / kLanes, col = lane % kLanes * 4, reach = reach_of(rr);
+                        const int64_t to_row = row_of(rr);
+                        if (reach == 0) continue;
+                        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int x = 5; x >= 0; --x) {      // the small terms first
+                            const float4 v = *staged(q_smem, D, (x & 1) * 96 + (x >> 1) * 32 + rr, col);
+                            o[0] += v.x; o[1] += v.y; o[2] += v.z; o[3] += v.w;
+                        }
+                        finish(to_row, reach, col, o);
                     }
-                    emit(warp * kCols, o, inv);
                 } else {
-                    constexpr int kCols = D / 2;        // group g finishes the columns [g D/2, (g + 1) D/2)
+                    // group g finishes the columns [g D/2, (g + 1) D/2): the other group's half through shared memory, scaled
+                    constexpr int kCols = D / 2;
                     const int other = wg ^ 1;
-                    const float mine = wg == 0 ? f0 : f1, theirs = wg == 0 ? f1 : f0;
+                    if (busy) {
 #pragma unroll
-                    for (int g = 0; g < kCols / 32; ++g) {
-                        if (!busy) break;
-                        uint32_t raw[32];
-                        if (done > 0) {
-                            tmem_ld_32x32(t_o + other * kCols + g * 32, raw);
-                            tmem_ld_wait();
+                        for (int g = 0; g < kCols / 32; ++g) {
+                            uint32_t raw[32];
+                            if (done > 0) {
+                                tmem_ld_32x32(t_o + other * kCols + g * 32, raw);
+                                tmem_ld_wait();
+                            }
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4)
+                                *staged(q_smem + other * 128 * kCols * 4, kCols, row, g * 32 + k) =
+                                    done > 0 ? make_float4(__uint_as_float(raw[k]) * mine, __uint_as_float(raw[k + 1]) * mine,
+                                                           __uint_as_float(raw[k + 2]) * mine, __uint_as_float(raw[k + 3]) * mine)
+                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         }
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) xo[(other * kCols + g * 32 + k) * 128 + row] = done > 0 ? __uint_as_float(raw[k]) : 0.0f;
                     }
                     bar_sync(1, kTcSoftmaxWarps * 32);
+                    unsigned char* area = q_smem + wg * 128 * kCols * 4;
+                    if (busy && done > 0) {
 #pragma unroll
-                    for (int g = 0; g < kCols / 32; ++g) {
-                        if (!busy) break;
-                        uint32_t raw[32];
-                        float o[32];
-                        if (done > 0) {
+                        for (int g = 0; g < kCols / 32; ++g) {
+                            uint32_t raw[32];
                             tmem_ld_32x32(t_o + wg * kCols + g * 32, raw);
                             tmem_ld_wait();
-                        }
 #pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            o[k] = fmaf(done > 0 ? __uint_as_float(raw[k]) : 0.0f, mine, xo[(wg * kCols + g * 32 + k) * 128 + row] * theirs);
-                        emit(wg * kCols + g * 32, o, inv);
+                            for (int k = 0; k < 32; k += 4) {
+                                float4* at = staged(area, kCols, row, g * 32 + k);
+                                const float4 x = *at;
+                                *at = make_float4(fmaf(__uint_as_float(raw[k]), mine, x.x), fmaf(__uint_as_float(raw[k + 1]), mine, x.y),
+                                                  fmaf(__uint_as_float(raw[k + 2]), mine, x.z), fmaf(__uint_as_float(raw[k + 3]), mine, x.w));
+                            }
+                        }
                     }
+                    __syncwarp();
+                    constexpr int N = F32 ? 4 : 8;
+                    if (busy)
+                        write_rows(std::integral_constant<int, kCols / N>(), std::integral_constant<int, N>(), wg * kCols, [&](int j, int col, float (&o)[N]) {
+#pragma unroll
+                            for (int k = 0; k < N; k += 4) {
+                                const float4 x = *staged(area, kCols, (warp & 3) * 32 + j, col + k);
+                                o[k] = x.x; o[k + 1] = x.y; o[k + 2] = x.z; o[k + 3] = x.w;
+                            }
+                        });
                 }
-                if (!direct && live && warp == (stack ? 0 : warp & 3)) part_ml[out_row * p.max_chunks + it.chunk] = make_float2(mt * c, lt);
                 tc5_fence_before();
                 bar_sync(1, kTcSoftmaxWarps * 32);      // the exchanged halves have been read
             }
