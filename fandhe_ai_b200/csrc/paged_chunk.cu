@@ -36,7 +36,11 @@ __device__ __forceinline__ T from_f32(float v);
 template <>
 __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <>
-__device__ __forceinline__ uint16_t from_f32<uint16_t>(float v) { return static_cast<uint16_t>(f32_to_bf16_bits(v)); }
+__device__ __forceinline__ uint16_t from_f32<uint16_t>(float v) {      // round to nearest even
+    uint16_t r;
+    asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
+    return r;
+}
 
 template <typename T, int N>
 __device__ __forceinline__ void load_f32(const T* p, float (&x)[N]) {
@@ -54,8 +58,14 @@ __device__ __forceinline__ void store_f32(T* p, const float (&x)[N]) {
 #pragma unroll
     for (int g = 0; g < N; g += W) {
         Pack<T, W> raw;
+        if constexpr (sizeof(T) == 2 && W % 2 == 0) {
 #pragma unroll
-        for (int k = 0; k < W; ++k) raw.v[k] = from_f32<T>(x[g + k]);
+            for (int k = 0; k < W; k += 2)
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(reinterpret_cast<uint32_t*>(&raw)[k / 2]) : "f"(x[g + k + 1]), "f"(x[g + k]));
+        } else {
+#pragma unroll
+            for (int k = 0; k < W; ++k) raw.v[k] = from_f32<T>(x[g + k]);
+        }
         *reinterpret_cast<Pack<T, W>*>(p + g) = raw;
     }
 }

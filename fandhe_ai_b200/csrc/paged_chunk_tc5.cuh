@@ -21,8 +21,8 @@
 // three times in the tile of accumulator rows, so that three warps of a group hold the same scores, and each contributes one term
 // of the weights: one product gives the three partial results, which are added at the end.
 //
-// The softmax weights go to the MMA warp in two halves of 64 keys, so that the second product starts while the second
-// half is still in the exponential.
+// The softmax weights go to the MMA warp in two parts, so that the second product starts while the rest is still in the
+// exponential: 96 and 32 keys (little is left to multiply after the last weight), or with three terms 64 and 64.
 //
 // Warps: 0-7 softmax (two groups); 8 deals out the items (decoded once, into shared memory) and fetches their tiles by TMA (one
 // box per cache block and half head, through the block table); 9 and 10 issue the products of one slot each, which keeps the
@@ -162,6 +162,16 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
 
+__device__ __forceinline__ float max_nan(float a, float b) {       // NaN if one of them is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
 // Two f32 operations in one instruction
 struct F2 {
     unsigned long long v;
@@ -230,14 +240,12 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-// First column, counted from a slot's scores, of the bf16 weights of half `h` and term `term`.  Three terms of 64 keys take 96 of the
+// First column, counted from a slot's scores, of the bf16 weights of half `h` and term `term` (one term: columns 0 to 63).  Three terms of 64 keys take 96 of the
 // 128 columns; the second half's last two terms go to columns that a 64-wide accumulator leaves free, or with D = 128 over the first
 // half's once that has been multiplied (p_free).
 template <int D>
-__device__ __forceinline__ constexpr uint32_t weight_columns(int h, int term, bool terms3) {
-    if (!terms3) return h * 32;
+__device__ __forceinline__ constexpr uint32_t weight_columns(int h, int term) {
     if (h == 0) return term * 32;
     return term == 0 ? 96 : (D == 64 ? 256 + 64 : 0) + (term - 1) * 32;
 }
@@ -249,9 +257,10 @@ __device__ __forceinline__ F2 cut_rest(float lo, float hi) {
 
 struct TcShared {
     uint64_t full[8], empty[8], raw[8];        // raw: a V tile with masked keys has landed and is to be cleaned
-    uint64_t s_full[2], p_full[2][2], p_free[2], o_full[2], q_full;
+    uint64_t s_full[2], p_full[2][2], p_free[2], o_full[2], q_full[2];
+    uint32_t turn[4];                          // taken by one of the two softmax warps of a scheduler
+    uint64_t meet_all, meet[2];                // the softmax warps meet: all of them, one group
     uint32_t tmem;
-    uint32_t abort;                            // a softmax warp gave up waiting
     uint64_t item_full[kTcItemSlots], item_empty[kTcItemSlots];
     TcItem items[kTcItemSlots];                // nt < 0: no more
     float xm[2][128], xl[2][128];
@@ -287,13 +296,15 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             mbar_init(smem_u32(&sh.p_full[s][1]), 4);
             mbar_init(smem_u32(&sh.p_free[s]), 1);
             mbar_init(smem_u32(&sh.o_full[s]), 1);
+            mbar_init(smem_u32(&sh.q_full[s]), 4);
+            mbar_init(smem_u32(&sh.meet[s]), 4);
         }
-        mbar_init(smem_u32(&sh.q_full), kTcSoftmaxWarps);
+        mbar_init(smem_u32(&sh.meet_all), kTcSoftmaxWarps);
+        for (int i = 0; i < 4; ++i) sh.turn[i] = 0;
         for (int i = 0; i < kTcItemSlots; ++i) {
             mbar_init(smem_u32(&sh.item_full[i]), 1);
             mbar_init(smem_u32(&sh.item_empty[i]), kTcSoftmaxWarps + 3);
         }
-        sh.abort = 0;
         fence_barrier_init();
     }
     if (warp == 8 && lane == 0) {
@@ -408,7 +419,8 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             const bool split = item->split, stack = F32 && item->stack;
             release_item(k_item);
             pos += 2 * n;
-            ok = wait(&sh.q_full, k_item & 1);
+            // (the other group's part last: it is at most one item behind once this group has stored its part)
+            ok = wait(&sh.q_full[s], k_item & 1) && (!split || wait(&sh.q_full[s ^ 1], k_item & 1));
             tc5_fence_after();
             const uint64_t q_desc = umma_desc_k128(q_addr + (F32 || split ? 0 : s) * Cfg::kQTileBytes);
             const int step = split ? 2 : 1;
@@ -448,9 +460,12 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
                         for (int term = 0; term < kTerms; ++term)
 #pragma unroll
-                            for (int kk = 0; kk < 4; ++kk)
-                                umma_bf16_ts(d_o, d_s + weight_columns<D>(H, term, kTerms == 3) + kk * 8, v_desc + (((H * 4 + kk) * 2048) >> 4), kIdescO,
-                                             H + term + kk > 0 ? 1u : keep);
+                            for (int kk = 0; kk < kTcKeys / 16; ++kk) {
+                                constexpr int kFirst = F32 ? 4 : 6;            // products of 16 keys in the first part
+                                if ((kk < kFirst) != (H == 0)) continue;
+                                const uint32_t cols = kTerms == 3 ? weight_columns<D>(H, term) + (kk - H * kFirst) * 8 : kk * 8;
+                                umma_bf16_ts(d_o, d_s + cols, v_desc + ((kk * 2048) >> 4), kIdescO, term + kk > 0 ? 1u : keep);
+                            }
                         if (H == 0 && kTerms == 3 && D == 128) tc5_commit(smem_u32(&sh.p_free[s]));
                         if (H == 1) {
                             if (last) tc5_commit(smem_u32(&sh.o_full[s]));
@@ -530,8 +545,34 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         const uint32_t lane_base = uint32_t(warp & 3) << 21;               // 32 lanes a warp, lane field in the upper half of the address
         const uint32_t t_s = tmem + wg * 128 + lane_base, t_o = tmem + 256 + wg * 128 + lane_base;
         const float c = p.scale_log2;
-        uint32_t s_phase = 0, f_phase = 0, o_phase = 0, k_item = 0;      // f_phase: tiles whose first half is waited for (p_free)
-        bool ok = true;
+        uint32_t s_phase = 0, f_phase = 0, o_phase = 0, k_item = 0, all_phase = 0, wg_phase = 0;      // f_phase: tiles whose first half is waited for (p_free)
+        bool ok = true, was_split = true;
+        // (mbarriers instead of named barriers: their waits end when somebody has given up)
+        auto meet_all = [&]() {
+            tc5_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.meet_all));
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.meet_all), all_phase++ & 1, err, kErrEpilogueWait)) && ok;
+            tc5_fence_after();
+        };
+        auto meet_group = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.meet[wg]));
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.meet[wg]), wg_phase++ & 1, err, kErrEpilogueWait)) && ok;
+        };
+        // Warps w and w + 4 share an exponential unit.  Left alone they fall into step - both exponentiate while the tensor cores
+        // wait, then both wait - so one lets the other finish first.  A courtesy with a limit: nothing depends on it.
+        bool my_turn = false;
+        auto take_turn = [&]() {
+            if (lane == 0) {
+                for (int i = 0; i < 48 && !my_turn; ++i) my_turn = atomicExch(&sh.turn[warp & 3], 1u) == 0u;
+            }
+            __syncwarp();
+        };
+        auto end_turn = [&]() {
+            if (lane == 0 && my_turn) atomicExch(&sh.turn[warp & 3], 0u);
+            my_turn = false;
+        };
         for (TcItem* item; ok && (item = next_item(k_item)) != nullptr; release_item(k_item++)) {
             const TcItem& it = *item;
             const bool stack = F32 && it.stack;
@@ -542,6 +583,13 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             const int list = it.row0 + r, token = list / p.group, head = it.kvh * p.group + list % p.group;
             const int limit = live ? it.len - it.n + token + 1 : 0;
             const int64_t out_row = (int64_t(it.start) + token) * p.sh.num_q_heads + head;
+
+            // The query tiles are free: a group that has its slot to itself waits for its own warps only, and so works through its
+            // items independently of the other group.
+            if (!it.split) meet_group();
+            else if (!was_split) meet_all();
+            was_split = it.split;
+            if (!ok) break;
 
             // Queries into shared memory, 128-byte swizzled.  A warp reads whole rows (a lane 8 elements of one), several before it
             // uses the first; a tile that both slots use is shared out over all eight warps.
@@ -592,7 +640,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 fence_proxy_async();
                 tc5_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.q_full));
+                if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[wg]));
             }
 
             float m = -INFINITY, l = 0.0f;
@@ -618,8 +666,8 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 auto raise = [&](float top) {
                     if (done == 0) {
                         m = top;
-                    } else if (__any_sync(0xffffffffu, (top - m) * c > 8.0f)) {
-                        const float m_new = fmaxf(m, top);
+                    } else if (__any_sync(0xffffffffu, !((top - m) * c <= 8.0f))) {
+                        const float m_new = max_nan(m, top);
                         const float f = m_new == m ? 1.0f : ex2((m - m_new) * c);
                         m = m_new;
                         l *= f;
@@ -655,34 +703,35 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     float mx[4];
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        mx[g] = fmaxf(s[g], s[g + 4]);
+                        mx[g] = max_nan(s[g], s[g + 4]);
 #pragma unroll
-                        for (int k = 8; k < 128; k += 8) mx[g] = fmaxf(fmaxf(mx[g], s[k + g]), s[k + 4 + g]);
+                        for (int k = 8; k < 128; k += 8) mx[g] = max_nan(mx[g], s[k + g], s[k + 4 + g]);
                     }
-                    raise(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-                    const float mc = m == -INFINITY ? 0.0f : m * c;
+                    raise(max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])));
+                    const float mc = m == -INFINITY ? 0.0f : (m == INFINITY ? __int_as_float(0x7FC00000) : m * c);      // a score of +inf: NaN, as inf - inf is
                     const F2 c2(c, c), mc2(-mc, -mc);
+                    take_turn();
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    for (int g = 0; g < 4; ++g) {      // 32 keys, 16 columns
+                        uint32_t w[16];
 #pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            uint32_t w[16];
-#pragma unroll
-                            for (int k = 0; k < 32; k += 2) {
-                                const int at = h * 64 + g * 32 + k;
-                                float a, b;
-                                fma2(F2(s[at], s[at + 1]), c2, mc2).get(a, b);
-                                a = ex2(a);
-                                b = ex2(b);
-                                sum[(k / 2) & 1] = add2(sum[(k / 2) & 1], F2(a, b));
-                                w[k / 2] = pack_bf16(a, b);
-                            }
-                            tmem_st_32x16(t_s + h * 32 + g * 16, w);
+                        for (int k = 0; k < 32; k += 2) {
+                            const int at = g * 32 + k;
+                            float a, b;
+                            fma2(F2(s[at], s[at + 1]), c2, mc2).get(a, b);
+                            a = ex2(a);
+                            b = ex2(b);
+                            sum[(k / 2) & 1] = add2(sum[(k / 2) & 1], F2(a, b));
+                            w[k / 2] = pack_bf16(a, b);
                         }
-                        tmem_st_wait();
-                        tc5_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[wg][h]));
+                        tmem_st_32x16(t_s + g * 16, w);
+                        if (g == 3) end_turn();
+                        if (g >= 2) {                  // 96 keys are handed over, then the other 32
+                            tmem_st_wait();
+                            tc5_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[wg][g - 2]));
+                        }
                     }
                 } else {
                     // The scores are read twice, 32 at a time: a row of them and its three terms do not fit the registers together.
@@ -705,15 +754,16 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         float mx[4];
 #pragma unroll
                         for (int g = 0; g < 4; ++g) {
-                            mx[g] = __uint_as_float(raw[0][g]);
+                            mx[g] = max_nan(__uint_as_float(raw[0][g]), __uint_as_float(raw[0][g + 4]));
 #pragma unroll
-                            for (int k = 4; k < 64; k += 4) mx[g] = fmaxf(mx[g], __uint_as_float(raw[(k + g) / 32][(k + g) % 32]));
+                            for (int k = 8; k < 64; k += 8)
+                                mx[g] = max_nan(mx[g], __uint_as_float(raw[(k + g) / 32][(k + g) % 32]), __uint_as_float(raw[(k + g + 4) / 32][(k + g + 4) % 32]));
                         }
-                        top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+                        top = max_nan(top, max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])));
                     }
                     tmem_st_wait();
                     raise(top);
-                    const float mc = m == -INFINITY ? 0.0f : m * c;
+                    const float mc = m == -INFINITY ? 0.0f : (m == INFINITY ? __int_as_float(0x7FC00000) : m * c);      // a score of +inf: NaN, as inf - inf is
                     const F2 c2(c, c), mc2(-mc, -mc);
                     // a half's terms are stored when its own scores, and those that they overwrite, are in registers
                     uint32_t sc[4][32];
@@ -749,13 +799,13 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                                 else if ((warp & 3) == 1) tmem_st_32x16(t_s + h * 32 + g * 16, w[1]);
                                 else tmem_st_32x16(t_s + h * 32 + g * 16, w[2]);
                             } else {
-                                tmem_st_32x16(t_s + weight_columns<D>(h, 0, true) + g * 16, w[0]);
+                                tmem_st_32x16(t_s + weight_columns<D>(h, 0) + g * 16, w[0]);
                                 if (D == 128 && h == 1 && g == 0) {      // the columns of the first half's last two terms
                                     ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.p_free[wg]), f_phase & 1, err, kErrEpilogueWait)) && ok;
                                     tc5_fence_after();
                                 }
-                                tmem_st_32x16(t_s + weight_columns<D>(h, 1, true) + g * 16, w[1]);
-                                tmem_st_32x16(t_s + weight_columns<D>(h, 2, true) + g * 16, w[2]);
+                                tmem_st_32x16(t_s + weight_columns<D>(h, 1) + g * 16, w[1]);
+                                tmem_st_32x16(t_s + weight_columns<D>(h, 2) + g * 16, w[2]);
                             }
                         }
                         tmem_st_wait();
@@ -776,7 +826,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 ++o_phase;
                 tc5_fence_after();
             }
-            if (!ok && lane == 0) sh.abort = 1;      // both groups still meet at this item's barriers, then both leave
+            if (!ok) break;
 
             // ---- results.  Rows go through shared memory (the query tiles are done with), so that a warp writes whole rows:
             // row r of a staging area of W-element rows keeps its 16-byte piece j at piece j ^ (r & 7).
@@ -856,14 +906,14 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     if (!direct && live) part_ml[out_row * p.max_chunks + it.chunk] = make_float2(m * c, l);
                 }
                 tc5_fence_before();
-                bar_sync(1, kTcSoftmaxWarps * 32);      // both groups are done with their query tiles
             } else {
                 const int lane_row = stack ? lane : row;
                 if (!stack || (warp & 3) == 0) {
                     sh.xm[wg][row] = m;
                     sh.xl[wg][row] = l;
                 }
-                bar_sync(1, kTcSoftmaxWarps * 32);      // every product that reads the query tile is complete: it may be overwritten
+                meet_all();      // every product that reads the query tile is complete: it may be overwritten
+                if (!ok) break;
                 patch = *reinterpret_cast<volatile uint32_t*>(&item->nonfinite) != 0;
                 const float m0 = sh.xm[0][lane_row], m1 = sh.xm[1][lane_row], mt = fmaxf(m0, m1);
                 const float f0 = m0 == -INFINITY ? 0.0f : ex2((m0 - mt) * c), f1 = m1 == -INFINITY ? 0.0f : ex2((m1 - mt) * c);
@@ -888,7 +938,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         }
                     }
-                    bar_sync(1, kTcSoftmaxWarps * 32);
+                    meet_all();
                     constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;
 #pragma unroll
                     for (int j = 0; j < 4; j += kAtOnce) {
@@ -923,7 +973,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         }
                     }
-                    bar_sync(1, kTcSoftmaxWarps * 32);
+                    meet_all();
                     unsigned char* area = q_smem + wg * 128 * kCols * 4;
                     if (busy && done > 0) {
 #pragma unroll
@@ -951,10 +1001,8 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                             }
                         });
                 }
-                tc5_fence_before();
-                bar_sync(1, kTcSoftmaxWarps * 32);      // the exchanged halves have been read
+                meet_all();      // the exchanged halves have been read
             }
-            if (*reinterpret_cast<volatile uint32_t*>(&sh.abort)) break;
         }
     }
     // every copy has landed and every product is complete before the memory is given back
@@ -994,8 +1042,8 @@ paged_chunk_join_kernel(const __grid_constant__ TcShape p, int tile_rows, const 
         for (int k = 0; k < V; ++k) acc[k] = 0.0f;
         for (int i = 0; i < used; ++i) {
             const float2 ml = part_ml[base + i];
-            if (ml.x == -INFINITY && ml.y == 0.0f) continue;           // no visible key in this range
-            const float w = ml.x == -INFINITY ? 1.0f : ex2(ml.x - m);
+            if (ml.x == -INFINITY) continue;           // no visible key in this range, or only scores of -inf
+            const float w = ex2(ml.x - m);
             l = fmaf(ml.y, w, l);
             float o[V];
             load_f32<float, V>(part_o + (base + i) * D + lane * V, o);
