@@ -32,7 +32,27 @@ constexpr int kCandidates = 512;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxPerCta = 49152;      // 192 KB of f32 logits per thread block
 
+// 2^(j / 64)
+__constant__ double kRoots[64] = {
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
+
 struct Shared {
+    double roots[64];                         // the table again, where threads may look up different entries
     uint64_t exchange[2][kMaxCluster][4];     // [phase][source rank][value], written by the peers
     uint64_t warp_sum[kWarps][4];
     uint32_t hist[kBins];
@@ -84,18 +104,37 @@ __device__ __forceinline__ float logit_f32<uint16_t>(uint16_t v) { return bf16_b
 
 struct Row {
     float max_x, bin_scale;
-    double inv_t, scale;      // 1 / T, 2^shift
+    double max_d, arg_scale;      // 64 log2(e) / T
+    const double* roots;
+    int shift, dead_bin;          // from this bin on a weight rounds to zero
 
     __device__ __forceinline__ int bin(float x) const {       // kBins for -inf
         const float d = max_x - x;
-        if (d == 0.0f) return 0;
-        if (x == -INFINITY) return kBins;
-        return static_cast<int>(fminf(d * bin_scale, static_cast<float>(kBins - 1)));
+        const int b = d == 0.0f ? 0 : static_cast<int>(fminf(d * bin_scale, static_cast<float>(kBins - 1)));
+        return x == -INFINITY ? kBins : b;
     }
-    __device__ __forceinline__ double weight_f64(float x) const {
-        return exp((static_cast<double>(x) - static_cast<double>(max_x)) * inv_t);
+    // 2^(y / 64), y = n + r, |r| <= 1/2: the table's 2^((n mod 64) / 64), the Taylor polynomial of 2^(r / 64) (its remainder is below
+    // 2^-54), and n / 64 in the exponent.  About 2^-50 relative, as the f64 subtraction and quotient it starts from.
+    __device__ __forceinline__ double scaled_weight(float x, int up) const {
+        const double magic = 6755399441055744.0;      // 1.5 * 2^52: adding it rounds to an integer and leaves that in the low word
+        const double y = (static_cast<double>(x) - max_d) * arg_scale;
+        const double z = y + magic;
+        const int n = __double2loint(z);
+        const double r = y - (z - magic);
+        double q = fma(r, 1.2417843701716925e-12, 5.732851688640402e-10);
+        q = fma(q, r, 2.1173137155464776e-07);
+        q = fma(q, r, 5.86490495505617e-05);
+        q = fma(q, r, 0.010830424696249145);
+        q = fma(q, r, 1.0);
+        q *= roots[n & 63];
+        return __hiloint2double(__double2hiint(q) + ((n >> 6) + up) * (1 << 20), __double2loint(q));
     }
-    __device__ __forceinline__ uint64_t weight(float x) const { return static_cast<uint64_t>(__double2ull_rn(weight_f64(x) * scale)); }
+    // the weight as an integer, 2^shift for the maximum
+    __device__ __forceinline__ uint64_t weight(float x, int b) const {
+        if (b >= dead_bin) return 0;
+        const double w = scaled_weight(x, shift) + 4503599627370496.0;      // 2^52: rounds, and the mantissa is the integer
+        return static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
+    }
 };
 
 // Sums (or with kMax: maxima) of N values over the cluster; `mine` receives nothing, `out` the totals, and
@@ -185,6 +224,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
     }
     for (int i = done + tid; i < n; i += kThreads) take(i, logit_f32<T>(src[i]));
     for (int b = tid; b < kBins; b += kThreads) sh.hist[b] = 0;
+    if (tid < 64) sh.roots[tid] = kRoots[tid];
     if (tid == 0) sh.n_cand = 0;
     if (nranks > 1) cluster_sync_all();      // the peers are running: their shared memory may be written
     const uint64_t best_bad[2] = {best, bad};
@@ -211,9 +251,13 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         const uint32_t key = static_cast<uint32_t>(top[0] >> 32);
         r.max_x = __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
         r.bin_scale = fminf(46.166241308f / t, FLT_MAX);      // 32 log2(e) / T
-        r.inv_t = 1.0 / static_cast<double>(t);
-        r.scale = static_cast<double>(1ull << p.shift);
+        r.max_d = static_cast<double>(r.max_x);
+        r.arg_scale = 92.33248261893424 / static_cast<double>(t);      // 64 log2(e) / T
+        r.roots = sh.roots;
+        r.shift = p.shift;
+        r.dead_bin = min(kBins - 1, 32 * (p.shift + 2));
     }
+    const double unit = static_cast<double>(1ull << p.shift);
     const int run = p.run, lo = tid * run, hi = min(n, lo + run);
     auto index = [&](int i) { return uint32_t(first) + i; };
 
@@ -235,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         }
         __syncthreads();
         if (weights)
-            for (int i = tid; i < at; i += kThreads) sh.all_w[i] = r.weight(sh.all_x[i]);
+            for (int i = tid; i < at; i += kThreads) sh.all_w[i] = r.weight(sh.all_x[i], r.bin(sh.all_x[i]));
         cluster_sync_all();                  // the peers have read this block's list: it may be refilled
         if (tid == 0) { sh.n_cand = 0; sh.best = ~0ull; }
         __syncthreads();
@@ -254,7 +298,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
             uint64_t s[1] = {0}, sum[1];
             for (int i = lo; i < hi; ++i) {
                 const float x = xs[i];
-                if (r.bin(x) == b && order_pair(x, index(i)) >= mid && under.keeps(b, x, index(i))) s[0] += by_weight ? r.weight(x) : 1ull;
+                if (r.bin(x) == b && order_pair(x, index(i)) >= mid && under.keeps(b, x, index(i))) s[0] += by_weight ? r.weight(x, b) : 1ull;
             }
             cluster_reduce<1, false>(sh, phase, rank, nranks, s, sum);
             if (static_cast<double>(base + sum[0]) >= enough) a = mid;
@@ -263,10 +307,25 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         return a;
     };
 
-    // ---- the bins of the row
-    for (int i = lo; i < hi; ++i) {
-        const int b = r.bin(xs[i]);
-        if (b < kBins) atomicAdd(&sh.hist[b], 1u);
+    // ---- the bins of the row; top-p over the whole row also wants the row's sum
+    const bool limited = k > 0 && k < p.vocab;
+    uint64_t row_sum = 0;
+    if (tp < 1.0f && !limited) {
+#pragma unroll 3
+        for (int i = lo; i < hi; ++i) {
+            const float x = xs[i];
+            const int b = r.bin(x);
+            if (b < kBins) {
+                atomicAdd(&sh.hist[b], 1u);
+                row_sum += r.weight(x, b);
+            }
+        }
+    } else {
+#pragma unroll 3
+        for (int i = lo; i < hi; ++i) {
+            const int b = r.bin(xs[i]);
+            if (b < kBins) atomicAdd(&sh.hist[b], 1u);
+        }
     }
     if (nranks > 1) {
         cluster_sync_all();
@@ -374,49 +433,62 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         }
         __syncthreads();
         int bp = min(int(sh.found[3]), bhi);
-        double target = 0.0;
-        uint64_t above = 0;
         const Cut k_cut = cut;
-        for (;;) {
-            uint64_t s[3] = {0, 0, 0}, sum[3];
+        // sums of the tokens of S1 in the bins [from, to), and in bin `to`
+        auto sums = [&](int from, int to, uint64_t (&sum)[3]) {
+            uint64_t s[3] = {0, 0, limited ? 0 : row_sum};
+#pragma unroll 3
             for (int i = lo; i < hi; ++i) {
                 const float x = xs[i];
                 const int b = r.bin(x);
-                if (b == kBins || !k_cut.keeps(b, x, index(i))) continue;
-                const uint64_t w = r.weight(x);
-                s[0] += w;
-                if (b < bp) s[1] += w;
-                else if (b == bp) s[2] += w;
+                if (b < from || (limited ? b > k_cut.bin : b > to) || b == kBins) continue;
+                if (limited && b == k_cut.bin && !k_cut.keeps(b, x, index(i))) continue;
+                const uint64_t w = r.weight(x, b);
+                if (limited) s[2] += w;
+                if (b < to) s[0] += w;
+                else if (b == to) s[1] += w;
             }
             cluster_reduce<3, false>(sh, phase, rank, nranks, s, sum);
-            target = double(tp) * double(sum[0]);
-            above = sum[1];
-            if (double(above) >= target && bp > blo) {               // the border lies above this bin
+        };
+        uint64_t sum[3];
+        sums(0, bp, sum);
+        const double target = double(tp) * double(sum[2]);
+        uint64_t above = sum[0], inside = sum[1];
+        for (;;) {
+            int next;
+            if (double(above) >= target && bp > blo) {               // the border lies above this bin: towards it by the estimates
                 bhi = bp - 1;
-                // walk towards it by the estimated masses
-                float gap = float((double(above) - target) / r.scale);
-                int b = bhi;
-                while (b > blo) {
-                    const float est_b = float(sh.total[b]) * exp2f(-(float(b) + 0.5f) * (1.0f / 32.0f));
+                float gap = float((double(above) - target) / unit);
+                for (next = bhi; next > blo; --next) {
+                    const float est_b = float(sh.total[next]) * exp2f(-(float(next) + 0.5f) * (1.0f / 32.0f));
                     if (gap < est_b) break;
                     gap -= est_b;
-                    --b;
                 }
-                bp = b;
-            } else if (double(above + sum[2]) < target && bp < bhi) {  // ... below it
+                uint64_t more[3];
+                sums(next, bp, more);                                 // what lies between comes off
+                above -= more[0];
+            } else if (double(above + inside) < target && bp < bhi) {  // ... below it
                 blo = bp + 1;
-                float gap = float((target - double(above + sum[2])) / r.scale);
-                int b = blo;
-                while (b < bhi) {
-                    const float est_b = float(sh.total[b]) * exp2f(-(float(b) + 0.5f) * (1.0f / 32.0f));
+                float gap = float((target - double(above + inside)) / unit);
+                for (next = blo; next < bhi; ++next) {
+                    const float est_b = float(sh.total[next]) * exp2f(-(float(next) + 0.5f) * (1.0f / 32.0f));
                     if (gap <= est_b) break;
                     gap -= est_b;
-                    ++b;
                 }
-                bp = b;
+                above += inside;
+                uint64_t more[3];
+                sums(bp + 1, next, more);
+                above += more[0];
+                inside = more[1];
+                bp = next;
+                continue;
             } else {
                 break;
             }
+            uint64_t more[3];
+            sums(next, next, more);
+            inside = more[1];
+            bp = next;
         }
         cut.bin = bp;
         if (sh.total[bp] <= kCandidates) {
@@ -439,12 +511,12 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
 
     // ---- the draw: sums of the kept weights in index order
     uint64_t s[2] = {0, 0}, sum[2];
-    const double floor_w = double(mp) * r.scale;
+    const double floor_w = double(mp) * unit;
     auto kept_weight = [&](int i, uint64_t* w) -> bool {
         const float x = xs[i];
         const int b = r.bin(x);
-        if (b == kBins || !cut.keeps(b, x, index(i))) return false;
-        *w = r.weight(x);
+        if (b > cut.bin || b == kBins || (b == cut.bin && !cut.keeps(b, x, index(i)))) return false;
+        *w = r.weight(x, b);
         return double(*w) >= floor_w || index(i) == best_i;
     };
     for (int i = lo; i < hi; ++i) {
@@ -477,7 +549,8 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
                 before += by ? 1 : w;
                 if (double(before) > goal) {
                     ids[row] = int(index(i));
-                    if (prob) prob[row] = float(r.weight_f64(xs[i]) * r.scale / double(sum[0]));
+                    const bool dead = (r.max_x - xs[i]) * r.bin_scale > 32000.0f;      // 2^-1000 of the maximum
+                    if (prob) prob[row] = dead ? 0.0f : float(r.scaled_weight(xs[i], 0) * unit / double(sum[0]));
                     if (kept) kept[row] = int(sum[1]);
                     break;
                 }
@@ -501,7 +574,7 @@ cudaError_t sample_tokens(const SampleShape& want, const void* logits, int bf16,
     p.per_cta = (((p.vocab + c - 1) / c) + 7) / 8 * 8;
     if (p.per_cta > kMaxPerCta) return cudaErrorInvalidValue;
     p.run = ((p.per_cta + kThreads - 1) / kThreads) | 1;      // odd: the threads' runs start in different banks
-    int bits = 1;
+    int bits = 12;                                              // weights below 2^52, see Row::weight
     while ((int64_t(1) << bits) < p.vocab) ++bits;
     p.shift = 62 - bits;
     const int smem = int(sizeof(Shared)) + p.per_cta * 4;
