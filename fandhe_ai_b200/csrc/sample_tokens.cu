@@ -14,9 +14,11 @@
 // One cluster of C thread blocks owns a row and keeps it in its shared memory, so that the logits are read from HBM once
 // however many passes the filters take.  Selection needs no sort: tokens fall into 2048 bins of (max - x) / T (a monotone
 // function, 1/32 of a doubling of the weight per bin), the bin a border falls into is found from the counts, and only the
-// few tokens of that bin are ranked exactly.  A bin that holds more than kCandidates tokens (flat or heavily tied rows) is
+// few tokens of that bin are ranked exactly.  Tokens that the counts already rule out are left behind: the others ("survivors",
+// usually a few hundred) move to a list in index order, and what follows works on that.  A bin that holds more than kCandidates tokens (flat or heavily tied rows) is
 // resolved by bisection over the ordered pair (logit, index) instead.
 #include <cfloat>
+#include <type_traits>
 
 #include "kernels.cuh"
 #include "launch.cuh"
@@ -29,6 +31,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kCandidates = 512;
+constexpr int kSurvivors = 2048;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxPerCta = 49152;      // 192 KB of f32 logits per thread block
 
@@ -64,8 +67,10 @@ struct Shared {
     uint64_t all_w[kCandidates];
     uint32_t scan_count[kWarps];
     float scan_mass[kWarps];
+    float list_x[kSurvivors];
+    uint16_t list_i[kSurvivors];              // place in this block's share
     uint32_t n_cand;
-    uint32_t found[4];
+    uint32_t found[6];
     unsigned long long best;
 };
 
@@ -131,9 +136,8 @@ struct Row {
     }
     // the weight as an integer, 2^shift for the maximum
     __device__ __forceinline__ uint64_t weight(float x, int b) const {
-        if (b >= dead_bin) return 0;
-        const double w = scaled_weight(x, shift) + 4503599627370496.0;      // 2^52: rounds, and the mantissa is the integer
-        return static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
+        const double w = scaled_weight(b >= dead_bin ? max_x : x, shift) + 4503599627370496.0;      // 2^52: rounds, and the mantissa is the integer
+        return b >= dead_bin ? 0 : static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
     }
 };
 
@@ -211,10 +215,12 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         const uint64_t pr = order_pair(x, uint32_t(first) + i);
         if (x != -INFINITY && pr > best) best = pr;
     };
+    if (nranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     constexpr int kVec = 16 / sizeof(T);
     int done = 0;
     if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
         done = n / kVec * kVec;
+#pragma unroll 4
         for (int g = tid; g < n / kVec; g += kThreads) {
             const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(src) + g);
             const T* v = reinterpret_cast<const T*>(&raw);
@@ -226,7 +232,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
     for (int b = tid; b < kBins; b += kThreads) sh.hist[b] = 0;
     if (tid < 64) sh.roots[tid] = kRoots[tid];
     if (tid == 0) sh.n_cand = 0;
-    if (nranks > 1) cluster_sync_all();      // the peers are running: their shared memory may be written
+    if (nranks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // the peers are running: their shared memory may be written
     const uint64_t best_bad[2] = {best, bad};
     uint64_t top[2];
     cluster_reduce<2, true>(sh, phase, rank, nranks, best_bad, top);
@@ -258,8 +264,11 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         r.dead_bin = min(kBins - 1, 32 * (p.shift + 2));
     }
     const double unit = static_cast<double>(1ull << p.shift);
-    const int run = p.run, lo = tid * run, hi = min(n, lo + run);
-    auto index = [&](int i) { return uint32_t(first) + i; };
+    const int run = p.run;
+    int lo = tid * run, hi = min(n, lo + run);      // this thread's elements: of the block's share, or of the list
+    bool listed = false;
+    auto X = [&](int i) { return listed ? sh.list_x[i] : xs[i]; };
+    auto index = [&](int i) { return uint32_t(first) + (listed ? uint32_t(sh.list_i[i]) : uint32_t(i)); };
 
     // gathers the candidates of all blocks; returns their number (known not to exceed kCandidates)
     auto gather = [&](bool weights) -> int {
@@ -297,7 +306,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
             const uint64_t mid = a + ((z - a) >> 1) + 1;
             uint64_t s[1] = {0}, sum[1];
             for (int i = lo; i < hi; ++i) {
-                const float x = xs[i];
+                const float x = X(i);
                 if (r.bin(x) == b && order_pair(x, index(i)) >= mid && under.keeps(b, x, index(i))) s[0] += by_weight ? r.weight(x, b) : 1ull;
             }
             cluster_reduce<1, false>(sh, phase, rank, nranks, s, sum);
@@ -310,23 +319,28 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
     // ---- the bins of the row; top-p over the whole row also wants the row's sum
     const bool limited = k > 0 && k < p.vocab;
     uint64_t row_sum = 0;
-    if (tp < 1.0f && !limited) {
-#pragma unroll 3
-        for (int i = lo; i < hi; ++i) {
-            const float x = xs[i];
-            const int b = r.bin(x);
-            if (b < kBins) {
-                atomicAdd(&sh.hist[b], 1u);
-                row_sum += r.weight(x, b);
+    auto bins = [&](auto weighed) {
+        for (int i0 = lo; i0 < lo + run; i0 += 4) {      // four at a time, without branches around the arithmetic
+            float x[4];
+            int b[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                x[q] = i0 + q < hi ? xs[i0 + q] : -INFINITY;
+                b[q] = r.bin(x[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (b[q] < kBins) atomicAdd(&sh.hist[b[q]], 1u);
+            if (decltype(weighed)::value) {
+                uint64_t w[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) w[q] = r.weight(x[q], b[q]);
+                row_sum += (w[0] + w[1]) + (w[2] + w[3]);
             }
         }
-    } else {
-#pragma unroll 3
-        for (int i = lo; i < hi; ++i) {
-            const int b = r.bin(xs[i]);
-            if (b < kBins) atomicAdd(&sh.hist[b], 1u);
-        }
-    }
+    };
+    if (tp < 1.0f && !limited) bins(std::true_type());
+    else bins(std::false_type());
     if (nranks > 1) {
         cluster_sync_all();
         const int slice = kBins / int(nranks);
@@ -380,9 +394,11 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
     }
     Cut cut{kBins, 0};
 
-    // ---- top-k: the bin in which the k-th token lies, then its rank inside the bin
+    // ---- where the borders lie by the counts: the bin of the k-th token, and the bin in which the estimated mass reaches top_p
+    const bool cut_k = limited && uint32_t(k) < all_count;
     float k_mass = all_mass;
-    if (k > 0 && uint32_t(k) < all_count) {
+    if (tid == 0) sh.found[3] = uint32_t(kBins - 1);
+    if (cut_k) {
         uint32_t cb = count_before;
         float mb = mass_before;
 #pragma unroll
@@ -395,14 +411,79 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
             cb += c4[q];
             mb += m4[q];
         }
+    }
+    __syncthreads();
+    const int bk = cut_k ? int(sh.found[0]) : kBins - 1;
+    if (cut_k) k_mass = __uint_as_float(sh.found[2]);
+    int bp = bk;
+    if (tp < 1.0f) {
+        const float est = tp * k_mass;
+        float mb = mass_before;
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+            if (mb < est && est <= mb + m4[q]) atomicMin(&sh.found[3], uint32_t(tid * kPer + q));
+            mb += m4[q];
+        }
         __syncthreads();
-        const int bk = int(sh.found[0]);
+        bp = min(int(sh.found[3]), bk);
+    }
+    // ---- the survivors: S1 lies in the bins up to bk; without top-k, S2 up to bp (give or take: should its border turn out to lie
+    // further, the whole share is gone through again), and S3 up to where a weight falls below min_p
+    int last_bin = kBins - 1;
+    if (cut_k) last_bin = bk;
+    else if (tp < 1.0f) last_bin = limited ? kBins - 1 : min(bp + 2, kBins - 1);      // (fewer tokens than top_k: their sum is still to come)
+    else if (mp > 0.0f) last_bin = min(static_cast<int>(-32.0f * log2f(fminf(mp, 1.0f))) + 2, kBins - 1);
+    if (last_bin < kBins - 1 && run <= 64) {
+        uint64_t mine = 0;
+        for (int i0 = lo; i0 < lo + run; i0 += 4) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float x = i0 + q < hi ? xs[i0 + q] : -INFINITY;
+                if (r.bin(x) <= last_bin) mine |= 1ull << (i0 + q - lo);
+            }
+        }
+        const int count = __popcll(mine);
+        int upto = count;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += up;
+        }
+        if (lane == 31) sh.warp_sum[warp][0] = uint64_t(upto);
+        __syncthreads();
+        int total = 0, at = upto - count;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) at += int(sh.warp_sum[w][0]);
+            total += int(sh.warp_sum[w][0]);
+        }
+        __syncthreads();
+        if (total <= kSurvivors) {
+            while (mine) {
+                const int j = __ffsll(static_cast<long long>(mine)) - 1;
+                mine &= mine - 1;
+                sh.list_x[at] = xs[lo + j];
+                sh.list_i[at++] = uint16_t(lo + j);
+            }
+            __syncthreads();
+            listed = true;
+            const int per = (total + kThreads - 1) / kThreads;
+            lo = min(total, tid * per);
+            hi = min(total, lo + per);
+        }
+    }
+    auto unlist = [&]() {
+        listed = false;
+        lo = tid * run;
+        hi = min(n, lo + run);
+    };
+
+    // ---- top-k: the k-th token's rank inside its bin
+    if (cut_k) {
         const uint32_t want = sh.found[1];
-        k_mass = __uint_as_float(sh.found[2]);
         cut.bin = bk;
         if (sh.total[bk] <= kCandidates) {
             for (int i = lo; i < hi; ++i)
-                if (r.bin(xs[i]) == bk) add_candidate(xs[i], index(i));
+                if (r.bin(X(i)) == bk) add_candidate(X(i), index(i));
             const int m = gather(false);
             for (int i = tid; i < m; i += kThreads) {
                 const uint64_t mine = order_pair(sh.all_x[i], sh.all_i[i]);
@@ -419,27 +500,14 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
 
     // ---- top-p: exact sums around the estimated bin until the border lies inside it, then the border inside the bin
     if (tp < 1.0f) {
-        int blo = 0, bhi = cut.bin < kBins ? cut.bin : kBins - 1;
-        const float est = tp * k_mass;
-        if (tid == 0) sh.found[3] = uint32_t(bhi);
-        __syncthreads();
-        {
-            float mb = mass_before;
-#pragma unroll
-            for (int q = 0; q < kPer; ++q) {
-                if (mb < est && est <= mb + m4[q]) atomicMin(&sh.found[3], uint32_t(tid * kPer + q));
-                mb += m4[q];
-            }
-        }
-        __syncthreads();
-        int bp = min(int(sh.found[3]), bhi);
+        int blo = 0, bhi = bk;
         const Cut k_cut = cut;
         // sums of the tokens of S1 in the bins [from, to), and in bin `to`
         auto sums = [&](int from, int to, uint64_t (&sum)[3]) {
             uint64_t s[3] = {0, 0, limited ? 0 : row_sum};
 #pragma unroll 3
             for (int i = lo; i < hi; ++i) {
-                const float x = xs[i];
+                const float x = X(i);
                 const int b = r.bin(x);
                 if (b < from || (limited ? b > k_cut.bin : b > to) || b == kBins) continue;
                 if (limited && b == k_cut.bin && !k_cut.keeps(b, x, index(i))) continue;
@@ -476,6 +544,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
                     gap -= est_b;
                 }
                 above += inside;
+                if (listed && next > last_bin) unlist();
                 uint64_t more[3];
                 sums(bp + 1, next, more);
                 above += more[0];
@@ -493,7 +562,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         cut.bin = bp;
         if (sh.total[bp] <= kCandidates) {
             for (int i = lo; i < hi; ++i)
-                if (r.bin(xs[i]) == bp && k_cut.keeps(bp, xs[i], index(i))) add_candidate(xs[i], index(i));
+                if (r.bin(X(i)) == bp && k_cut.keeps(bp, X(i), index(i))) add_candidate(X(i), index(i));
             const int m = gather(true);
             for (int i = tid; i < m; i += kThreads) {
                 const uint64_t mine = order_pair(sh.all_x[i], sh.all_i[i]);
@@ -513,7 +582,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
     uint64_t s[2] = {0, 0}, sum[2];
     const double floor_w = double(mp) * unit;
     auto kept_weight = [&](int i, uint64_t* w) -> bool {
-        const float x = xs[i];
+        const float x = X(i);
         const int b = r.bin(x);
         if (b > cut.bin || b == kBins || (b == cut.bin && !cut.keeps(b, x, index(i)))) return false;
         *w = r.weight(x, b);
@@ -549,8 +618,8 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
                 before += by ? 1 : w;
                 if (double(before) > goal) {
                     ids[row] = int(index(i));
-                    const bool dead = (r.max_x - xs[i]) * r.bin_scale > 32000.0f;      // 2^-1000 of the maximum
-                    if (prob) prob[row] = dead ? 0.0f : float(r.scaled_weight(xs[i], 0) * unit / double(sum[0]));
+                    const bool dead = (r.max_x - X(i)) * r.bin_scale > 32000.0f;      // 2^-1000 of the maximum
+                    if (prob) prob[row] = dead ? 0.0f : float(r.scaled_weight(X(i), 0) * unit / double(sum[0]));
                     if (kept) kept[row] = int(sum[1]);
                     break;
                 }
