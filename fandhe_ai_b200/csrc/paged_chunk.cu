@@ -70,42 +70,69 @@ __device__ __forceinline__ void store_f32(T* p, const float (&x)[N]) {
     }
 }
 
-// One block per token row (grid.y blocks share the heads of a row when there are few rows).  A thread's unit of work is a pair of
-// N-element groups that rotate into each other (ADJ: one group holding N / 2 pairs) or a group that is copied; N elements are 16
-// bytes of the activation type, or N = 1 (ADJ: 2) where an alignment or a size does not allow that.
+constexpr int kAppendRows = 8;      // at most, token rows of a block
+struct AppendRow {
+    int64_t slot, angle;            // first element of the token's pool row, row of the cos / sin tables; slot < 0: nothing to do
+};
+
+// A block takes `rows_per_block` consecutive token rows (with few rows one, whose heads grid.y blocks share).  Warp r finds out where
+// the r-th of them goes, then all threads go through the rows' units of work together.  A unit is a pair of N-element groups that
+// rotate into each other (ADJ: one group holding N / 2 pairs) or a group that is copied; N elements are 16 bytes of the activation
+// type, or N = 1 (ADJ: 2) where an alignment or a size does not allow that.
 template <typename T, typename KvT, int N, bool ADJ>
 __global__ void __launch_bounds__(256)
-rope_append_kernel(RaggedShape sh, RopeShape rope, const T* __restrict__ qkv, const float* __restrict__ cos_t,
+rope_append_kernel(RaggedShape sh, RopeShape rope, int rows_per_block, const T* __restrict__ qkv, const float* __restrict__ cos_t,
                    const float* __restrict__ sin_t, const uint32_t* __restrict__ positions, const uint32_t* __restrict__ tables,
                    const uint32_t* __restrict__ q_starts, const uint32_t* __restrict__ seq_lens, T* __restrict__ q_out,
                    KvT* __restrict__ k_pool, KvT* __restrict__ v_pool, uint32_t* err) {
-    const int64_t row = blockIdx.x;
-    const int seq = sequence_of_row(q_starts, sh.batch, row);
-    if (seq >= sh.batch) return;                                        // behind the last sequence
-    const int64_t end = q_starts[seq + 1], len = seq_lens[seq];
-    const int64_t slot_pos = len - (end - row);                         // position in the cache
-    const int64_t angle_pos = positions ? int64_t(positions[row]) : slot_pos;
-    if (slot_pos < 0 || slot_pos >= int64_t(sh.max_blocks_per_seq) * sh.block_size || angle_pos < 0 || angle_pos >= rope.n_positions) {
-        if (threadIdx.x == 0) atomicCAS(err, 0u, static_cast<uint32_t>(kErrRaggedBatch));
-        return;
+    __shared__ AppendRow place[kAppendRows];
+    const int64_t row0 = int64_t(blockIdx.x) * rows_per_block;
+    const int count = int(min(int64_t(rows_per_block), sh.rows - row0));
+    const int64_t ekv = int64_t(sh.num_kv_heads) * sh.head_dim;
+    for (int i = threadIdx.x >> 5; i < count; i += blockDim.x >> 5) {
+        const int64_t row = row0 + i;
+        const int lane = threadIdx.x & 31;
+        int seq = 0;                       // the number of starts[1 .. batch] that are <= row: one load latency, no search
+        for (int b0 = 0; b0 < sh.batch; b0 += 128) {
+            int before = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int b = b0 + k * 32 + lane;
+                before += b < sh.batch && int64_t(q_starts[b + 1]) <= row;
+            }
+            seq += int(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(before)));
+        }
+        if (lane == 0) {
+            AppendRow to = {-1, 0};
+            if (seq < sh.batch) {          // else behind the last sequence
+                const int64_t pos = int64_t(seq_lens[seq]) - (int64_t(q_starts[seq + 1]) - row);      // position in the cache
+                to.angle = positions ? int64_t(positions[row]) : pos;
+                if (pos < 0 || pos >= int64_t(sh.max_blocks_per_seq) * sh.block_size || to.angle < 0 || to.angle >= rope.n_positions) {
+                    atomicCAS(err, 0u, static_cast<uint32_t>(kErrRaggedBatch));
+                } else {
+                    const uint32_t blk = tables[int64_t(seq) * sh.max_blocks_per_seq + pos / sh.block_size];
+                    if (blk >= uint32_t(sh.num_blocks)) atomicCAS(err, 0u, static_cast<uint32_t>(kErrAppendSlot));
+                    else to.slot = (int64_t(blk) * sh.block_size + pos % sh.block_size) * ekv;
+                }
+            }
+            place[i] = to;
+        }
     }
-    const uint32_t blk = tables[int64_t(seq) * sh.max_blocks_per_seq + slot_pos / sh.block_size];
-    if (blk >= uint32_t(sh.num_blocks)) {
-        if (threadIdx.x == 0) atomicCAS(err, 0u, static_cast<uint32_t>(kErrAppendSlot));
-        return;
-    }
+    __syncthreads();
     const int d = sh.head_dim, half = rope.rotary_dim / 2;
-    const int64_t ekv = int64_t(sh.num_kv_heads) * d;
-    const int64_t slot = (int64_t(blk) * sh.block_size + slot_pos % sh.block_size) * ekv;
-    const T* src = qkv + row * sh.row_stride;
-    T* q_row = q_out + row * (int64_t(sh.num_q_heads) * d);
-    const float* c_row = cos_t + angle_pos * half;
-    const float* s_row = sin_t + angle_pos * half;
     const int turned = ADJ ? rope.rotary_dim / N : half / N;            // units of a head that rotate
     const int units = turned + (d - rope.rotary_dim) / N;
     const int turning_heads = sh.num_q_heads + sh.num_kv_heads;
     const int total = turning_heads * units + sh.num_kv_heads * (d / N);
-    for (int w = blockIdx.y * blockDim.x + threadIdx.x; w < total; w += gridDim.y * blockDim.x) {
+#pragma unroll 2
+    for (int w0 = blockIdx.y * blockDim.x + threadIdx.x; w0 < total * count; w0 += gridDim.y * blockDim.x) {
+        const int i = w0 / total, w = w0 - i * total;
+        const int64_t slot = place[i].slot, row = row0 + i;
+        if (slot < 0) continue;
+        const T* src = qkv + row * sh.row_stride;
+        T* q_row = q_out + row * (int64_t(sh.num_q_heads) * d);
+        const float* c_row = cos_t + place[i].angle * half;
+        const float* s_row = sin_t + place[i].angle * half;
         if (w >= turning_heads * units) {                               // v: a copy
             const int e = (w - turning_heads * units) * N;
             float x[N];
@@ -165,14 +192,16 @@ cudaError_t launch_append(const RaggedShape& sh, const RopeShape& rope, const vo
     const bool wide = aligned(qkv) && aligned(q_out) && aligned(k_pool) && aligned(v_pool) && aligned(cos_t) && aligned(sin_t) &&
                       sh.row_stride % N == 0 && sh.head_dim % 8 == 0 && rope.rotary_dim % (2 * N) == 0;
     const int per_row = (sh.num_q_heads + 2 * sh.num_kv_heads) * sh.head_dim / (wide ? 2 * N : 2);
-    // blocks per row: as many as keep every SM busy, each with 64 units of work at least
+    // Many rows: eight to a block, so that a thread has several loads in flight and the look-ups are shared (one row to a block moves
+    // 14k rows of 4.6 KB at 2.3 TB/s).  Few rows: one, shared out over as many blocks as keep every SM busy with 64 units of work each.
+    const int per_block = sh.rows >= int64_t(4) * kAppendRows * sm_count ? kAppendRows : 1;
     int split = 1;
     while (split < 16 && sh.rows * split < 2 * sm_count && per_row / (2 * split) >= 64) split *= 2;
     int threads = 256;
-    while (threads > 64 && per_row / split <= threads / 2) threads /= 2;
-    const dim3 grid(static_cast<unsigned>(sh.rows), split);
+    while (per_block == 1 && threads > 64 && per_row / split <= threads / 2) threads /= 2;
+    const dim3 grid(static_cast<unsigned>((sh.rows + per_block - 1) / per_block), split);
 #define B200_APPEND(NN, ADJ)                                                                                                             \
-    rope_append_kernel<T, KvT, NN, ADJ><<<grid, threads, 0, s>>>(sh, rope, static_cast<const T*>(qkv), cos_t, sin_t, positions, tables,     \
+    rope_append_kernel<T, KvT, NN, ADJ><<<grid, threads, 0, s>>>(sh, rope, per_block, static_cast<const T*>(qkv), cos_t, sin_t, positions, tables,     \
                                                                  q_starts, seq_lens, static_cast<T*>(q_out), static_cast<KvT*>(k_pool), \
                                                                  static_cast<KvT*>(v_pool), err)
     if (wide) {

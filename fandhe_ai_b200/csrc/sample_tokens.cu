@@ -60,11 +60,9 @@ struct Shared {
     uint64_t warp_sum[kWarps][4];
     uint32_t hist[kBins];
     uint32_t total[kBins];                    // the bins of the whole row
-    float cand_x[kCandidates];
-    uint32_t cand_i[kCandidates];
-    float all_x[kCandidates];
-    uint32_t all_i[kCandidates];
+    uint64_t all_pair[kCandidates];           // the candidates of the whole row, written by the peers
     uint64_t all_w[kCandidates];
+    uint32_t counts[kMaxCluster];
     uint32_t scan_count[kWarps];
     float scan_mass[kWarps];
     float list_x[kSurvivors];
@@ -270,33 +268,30 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
     auto X = [&](int i) { return listed ? sh.list_x[i] : xs[i]; };
     auto index = [&](int i) { return uint32_t(first) + (listed ? uint32_t(sh.list_i[i]) : uint32_t(i)); };
 
-    // gathers the candidates of all blocks; returns their number (known not to exceed kCandidates)
-    auto gather = [&](bool weights) -> int {
-        __syncthreads();                     // every thread has added its candidates
-        const uint64_t mine[1] = {tid == 0 ? uint64_t(sh.n_cand) : 0};
-        uint64_t sum[1];
-        const int ph = phase;
-        cluster_reduce<1, false>(sh, phase, rank, nranks, mine, sum);
-        int at = 0;
-        for (uint32_t q = 0; q < nranks; ++q) {
-            const int m = int(sh.exchange[ph][q][0]);
-            for (int i = tid; i < m; i += kThreads) {
-                sh.all_x[at + i] = __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&sh.cand_x[i]), q)));
-                sh.all_i[at + i] = ld_cluster_u32(mapa_shared(smem_u32(&sh.cand_i[i]), q));
-            }
-            at += m;
-        }
-        __syncthreads();
-        if (weights)
-            for (int i = tid; i < at; i += kThreads) sh.all_w[i] = r.weight(sh.all_x[i], r.bin(sh.all_x[i]));
-        cluster_sync_all();                  // the peers have read this block's list: it may be refilled
+    // Every block hands the tokens of bin `b` to all blocks, as ordered pairs (0: not among `under`); returns how many places that
+    // takes, which is known not to exceed kCandidates.
+    auto gather = [&](int b, const Cut& under) -> int {
+        if (uint32_t(tid) < nranks) sh.counts[tid] = nranks > 1 ? ld_cluster_u32(mapa_shared(smem_u32(&sh.hist[b]), tid)) : sh.hist[b];
         if (tid == 0) { sh.n_cand = 0; sh.best = ~0ull; }
         __syncthreads();
-        return at;
+        int total = 0, at = 0;
+        for (uint32_t q = 0; q < nranks; ++q) {
+            if (q < rank) at += int(sh.counts[q]);
+            total += int(sh.counts[q]);
+        }
+        for (int i = lo; i < hi; ++i) {
+            const float x = X(i);
+            if (r.bin(x) != b) continue;
+            const uint64_t pair = under.keeps(b, x, index(i)) ? order_pair(x, index(i)) : 0;
+            const int to = at + int(atomicAdd(&sh.n_cand, 1u));
+            for (uint32_t q = 0; q < nranks; ++q) st_cluster_u64(mapa_shared(smem_u32(&sh.all_pair[to]), q), pair);
+        }
+        cluster_sync_all();
+        return total;
     };
-    auto add_candidate = [&](float x, uint32_t i) {
-        const uint32_t at = atomicAdd(&sh.n_cand, 1u);
-        if (at < kCandidates) { sh.cand_x[at] = x; sh.cand_i[at] = i; }
+    auto logit_of = [&](uint64_t pair) {
+        const uint32_t key = static_cast<uint32_t>(pair >> 32);
+        return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
     };
     // The last pair of bin `b` (under `under`) that belongs to the prefix in which `enough` is not reached before it, by
     // bisection over the 64-bit order: `measure` gives a token's contribution, `base` what lies above the bin.
@@ -434,13 +429,14 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
     else if (tp < 1.0f) last_bin = limited ? kBins - 1 : min(bp + 2, kBins - 1);      // (fewer tokens than top_k: their sum is still to come)
     else if (mp > 0.0f) last_bin = min(static_cast<int>(-32.0f * log2f(fminf(mp, 1.0f))) + 2, kBins - 1);
     if (last_bin < kBins - 1 && run <= 64) {
+        // a logit below this is in a later bin for certain (the bins themselves are asked for again below)
+        const float least = r.max_x - (float(last_bin + 1) / r.bin_scale * 1.00001f + fabsf(r.max_x) * 1e-6f);
         uint64_t mine = 0;
-        for (int i0 = lo; i0 < lo + run; i0 += 4) {
+        for (int i0 = lo; i0 < lo + run; i0 += 8) {
+            uint32_t some = 0;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float x = i0 + q < hi ? xs[i0 + q] : -INFINITY;
-                if (r.bin(x) <= last_bin) mine |= 1ull << (i0 + q - lo);
-            }
+            for (int q = 0; q < 8; ++q) some |= (i0 + q < hi && xs[i0 + q] >= least ? 1u : 0u) << q;
+            mine |= uint64_t(some) << (i0 - lo);
         }
         const int count = __popcll(mine);
         int upto = count;
@@ -482,13 +478,12 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         const uint32_t want = sh.found[1];
         cut.bin = bk;
         if (sh.total[bk] <= kCandidates) {
-            for (int i = lo; i < hi; ++i)
-                if (r.bin(X(i)) == bk) add_candidate(X(i), index(i));
-            const int m = gather(false);
+            const int m = gather(bk, Cut{kBins, 0});
             for (int i = tid; i < m; i += kThreads) {
-                const uint64_t mine = order_pair(sh.all_x[i], sh.all_i[i]);
+                const uint64_t mine = sh.all_pair[i];
                 uint32_t ahead = 0;
-                for (int j = 0; j < m; ++j) ahead += order_pair(sh.all_x[j], sh.all_i[j]) > mine;
+#pragma unroll 4
+                for (int j = 0; j < m; ++j) ahead += sh.all_pair[j] > mine;
                 if (ahead == want - 1) sh.best = mine;
             }
             __syncthreads();
@@ -561,15 +556,15 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         }
         cut.bin = bp;
         if (sh.total[bp] <= kCandidates) {
-            for (int i = lo; i < hi; ++i)
-                if (r.bin(X(i)) == bp && k_cut.keeps(bp, X(i), index(i))) add_candidate(X(i), index(i));
-            const int m = gather(true);
+            const int m = gather(bp, k_cut);
+            for (int i = tid; i < m; i += kThreads) sh.all_w[i] = sh.all_pair[i] ? r.weight(logit_of(sh.all_pair[i]), bp) : 0;
+            __syncthreads();
             for (int i = tid; i < m; i += kThreads) {
-                const uint64_t mine = order_pair(sh.all_x[i], sh.all_i[i]);
+                const uint64_t mine = sh.all_pair[i];
                 uint64_t ahead = above;
-                for (int j = 0; j < m; ++j)
-                    if (order_pair(sh.all_x[j], sh.all_i[j]) > mine) ahead += sh.all_w[j];
-                if (double(ahead) < target) atomicMin(&sh.best, static_cast<unsigned long long>(mine));   // the last kept one
+#pragma unroll 4
+                for (int j = 0; j < m; ++j) ahead += sh.all_pair[j] > mine ? sh.all_w[j] : 0;
+                if (mine && double(ahead) < target) atomicMin(&sh.best, static_cast<unsigned long long>(mine));   // the last kept one
             }
             __syncthreads();
             cut.pair = sh.best;
