@@ -52,6 +52,18 @@ __device__ __forceinline__ void load_f32(const T* p, float (&x)[N]) {
         for (int k = 0; k < W; ++k) x[g + k] = as_f32(raw.v[k]);
     }
 }
+// ... of what nobody reads again
+template <typename T, int N>
+__device__ __forceinline__ void load_once(const T* p, float (&x)[N]) {
+    if constexpr (sizeof(T) * N == 16) {
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+        const Pack<T, N> raw = *reinterpret_cast<const Pack<T, N>*>(&u);
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = as_f32(raw.v[k]);
+    } else {
+        load_f32<T, N>(p, x);
+    }
+}
 template <typename T, int N>
 __device__ __forceinline__ void store_f32(T* p, const float (&x)[N]) {
     constexpr int W = sizeof(T) * N > 16 ? 16 / sizeof(T) : N;
@@ -124,7 +136,7 @@ rope_append_kernel(RaggedShape sh, RopeShape rope, int rows_per_block, const T* 
     const int units = turned + (d - rope.rotary_dim) / N;
     const int turning_heads = sh.num_q_heads + sh.num_kv_heads;
     const int total = turning_heads * units + sh.num_kv_heads * (d / N);
-#pragma unroll 2
+#pragma unroll 1
     for (int w0 = blockIdx.y * blockDim.x + threadIdx.x; w0 < total * count; w0 += gridDim.y * blockDim.x) {
         const int i = w0 / total, w = w0 - i * total;
         const int64_t slot = place[i].slot, row = row0 + i;
@@ -136,7 +148,7 @@ rope_append_kernel(RaggedShape sh, RopeShape rope, int rows_per_block, const T* 
         if (w >= turning_heads * units) {                               // v: a copy
             const int e = (w - turning_heads * units) * N;
             float x[N];
-            load_f32<T, N>(src + int64_t(turning_heads) * d + e, x);
+            load_once<T, N>(src + int64_t(turning_heads) * d + e, x);
             store_f32<KvT, N>(v_pool + slot + e, x);
             continue;
         }
@@ -150,12 +162,12 @@ rope_append_kernel(RaggedShape sh, RopeShape rope, int rows_per_block, const T* 
         if (unit >= turned) {
             const int e = rope.rotary_dim + (unit - turned) * N;
             float x[N];
-            load_f32<T, N>(h + e, x);
+            load_once<T, N>(h + e, x);
             put(e, x);
         } else if constexpr (ADJ) {
             const int e = unit * N;
             float x[N], c[N / 2], s[N / 2], y[N];
-            load_f32<T, N>(h + e, x);
+            load_once<T, N>(h + e, x);
             load_f32<float, N / 2>(c_row + e / 2, c);
             load_f32<float, N / 2>(s_row + e / 2, s);
 #pragma unroll
@@ -167,8 +179,8 @@ rope_append_kernel(RaggedShape sh, RopeShape rope, int rows_per_block, const T* 
         } else {
             const int e = unit * N;
             float a[N], b[N], c[N], s[N], ya[N], yb[N];
-            load_f32<T, N>(h + e, a);
-            load_f32<T, N>(h + e + half, b);
+            load_once<T, N>(h + e, a);
+            load_once<T, N>(h + e + half, b);
             load_f32<float, N>(c_row + e, c);
             load_f32<float, N>(s_row + e, s);
 #pragma unroll
@@ -192,9 +204,11 @@ cudaError_t launch_append(const RaggedShape& sh, const RopeShape& rope, const vo
     const bool wide = aligned(qkv) && aligned(q_out) && aligned(k_pool) && aligned(v_pool) && aligned(cos_t) && aligned(sin_t) &&
                       sh.row_stride % N == 0 && sh.head_dim % 8 == 0 && rope.rotary_dim % (2 * N) == 0;
     const int per_row = (sh.num_q_heads + 2 * sh.num_kv_heads) * sh.head_dim / (wide ? 2 * N : 2);
-    // Many rows: eight to a block, so that a thread has several loads in flight and the look-ups are shared (one row to a block moves
-    // 14k rows of 4.6 KB at 2.3 TB/s).  Few rows: one, shared out over as many blocks as keep every SM busy with 64 units of work each.
-    const int per_block = sh.rows >= int64_t(4) * kAppendRows * sm_count ? kAppendRows : 1;
+    // Many rows: as many to a block as make about 2048 units of work, at most eight (8192 f32 rows of 24 KB: 65.6 us with two rows to a
+    // block, 71.3 with eight; 14k bf16 rows of 4.6 KB: 65.5 us with one, 40 with eight).  Few rows: one, shared out over as many
+    // blocks as keep every SM busy with 64 units of work each.
+    const int wanted = 2048 / (per_row > 0 ? per_row : 1);
+    const int per_block = sh.rows < int64_t(4) * kAppendRows * sm_count ? 1 : (wanted < 1 ? 1 : (wanted < kAppendRows ? wanted : kAppendRows));
     int split = 1;
     while (split < 16 && sh.rows * split < 2 * sm_count && per_row / (2 * split) >= 64) split *= 2;
     int threads = 256;
@@ -367,7 +381,7 @@ cudaError_t launch_tc5(const ChunkPlan& plan, const RaggedShape& sh, const void*
     p.scale_log2 = sh.scale == 0.0f ? 1.0f : fabsf(sh.scale) * 1.44269504088896341f;
     float* part_o = static_cast<float*>(workspace);
     float2* part_ml = reinterpret_cast<float2*>(part_o + (plan.max_chunks > 1 ? sh.rows * sh.num_q_heads * plan.max_chunks * D : 0));
-    const dim3 grid(static_cast<unsigned>(plan.items < sm_count ? plan.items : sm_count));
+    const dim3 grid(static_cast<unsigned>(plan.items));
     cudaError_t e = launch_ex(paged_chunk_tc5_kernel<D, F32, T>, grid, dim3(kTcThreads), Cfg::kSmem, s, 1, true, map_k, map_v, p,
                               static_cast<const T*>(q), static_cast<const uint16_t*>(v_pool), tables, q_starts, seq_lens,
                               static_cast<T*>(out), part_o, part_ml, err);

@@ -82,6 +82,8 @@ struct TcWalk {
 
     __device__ bool next_group(uint32_t* err) {
         base += total;
+        total = 0;
+        if (first >= p.sh.batch) return false;
         first += 32;
         if (first >= p.sh.batch) return false;
         const int b = first + lane;
@@ -106,8 +108,12 @@ struct TcWalk {
         total = __shfl_sync(0xffffffffu, incl, 31);
         return true;
     }
-    // the item `index` (not below the last one asked for); false when there are no more.  nt = 0: nothing to do.
+    // the item `index` (quickest when not below the last one asked for); false when there are no more.  nt = 0: nothing to do.
     __device__ bool get(int64_t index, TcItem& it, uint32_t* err) {
+        if (index < base) {
+            first = -32;
+            base = total = 0;
+        }
         while (index >= base + total)
             if (!next_group(err)) return false;
         const int local = int(index - base);
@@ -241,6 +247,27 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Asks the launch unit for a block of this grid that has not started: that block is cancelled and its work is the caller's.  The
+// answer (16 bytes) arrives on the barrier.  Not to be asked again once the answer was "none".
+__device__ __forceinline__ void steal_block(uint32_t answer, uint32_t bar) {
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int stolen_block(uint32_t answer) {      // -1: none
+    uint32_t ok, x;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t.reg .b128 A;\n\t"
+        "ld.shared.b128 A, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 P, A;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@P clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, A;\n\t}\n"
+        : "=r"(ok), "=r"(x)
+        : "r"(answer)
+        : "memory");
+    return ok ? static_cast<int>(x) : -1;
+}
+
 // First column, counted from a slot's scores, of the bf16 weights of half `h` and term `term` (one term: columns 0 to 63).  Three terms of 64 keys take 96 of the
 // 128 columns; the second half's last two terms go to columns that a 64-wide accumulator leaves free, or with D = 128 over the first
 // half's once that has been multiplied (p_free).
@@ -262,6 +289,8 @@ struct TcShared {
     uint64_t meet_all, meet[2];                // the softmax warps meet: all of them, one group
     uint32_t tmem;
     uint64_t item_full[kTcItemSlots], item_empty[kTcItemSlots];
+    uint64_t stolen_bar;
+    alignas(16) uint4 stolen;                  // answer of the launch unit: the block that will not be launched
     TcItem items[kTcItemSlots];                // nt < 0: no more
     float xm[2][128], xl[2][128];
 };
@@ -300,6 +329,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             mbar_init(smem_u32(&sh.meet[s]), 4);
         }
         mbar_init(smem_u32(&sh.meet_all), kTcSoftmaxWarps);
+        mbar_init(smem_u32(&sh.stolen_bar), 1);
         for (int i = 0; i < 4; ++i) sh.turn[i] = 0;
         for (int i = 0; i < kTcItemSlots; ++i) {
             mbar_init(smem_u32(&sh.item_full[i]), 1);
@@ -354,8 +384,21 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             ++k_item;
             return true;
         };
-        for (int64_t index = blockIdx.x; ok && walk.get(index, it, err); index += gridDim.x) {
-            if (it.nt == 0) continue;
+        // One block per item in the grid; a block that is through with its own takes over one that has not started, so the items
+        // spread evenly whatever their lengths.
+        int64_t index = blockIdx.x;
+        uint32_t asked = 0;
+        for (; ok; ++asked) {
+            if (asked > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.stolen_bar), (asked - 1) & 1, err, kErrProducerWait));
+                if (!ok) break;
+                index = stolen_block(smem_u32(&sh.stolen));
+                if (index < 0) break;
+                fence_proxy_async();
+                __syncwarp();
+            }
+            if (lane == 0) steal_block(smem_u32(&sh.stolen), smem_u32(&sh.stolen_bar));
+            if (!walk.get(index, it, err) || it.nt == 0) continue;
             ok = deal();
             if (!ok) break;
             const TcOrder order(pos, it);
@@ -398,6 +441,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             it.nt = -1;
             deal();
         }
+        if (!ok) mbar_wait(smem_u32(&sh.stolen_bar), asked & 1, err, kErrProducerWait);
         if (!ok)      // the consumer is gone: let this warp's own copies land before the memory is given back
             for (uint32_t at = issued > kNst ? issued - kNst : 0; at < issued; ++at) {
                 const uint32_t stage = at % kNst;
