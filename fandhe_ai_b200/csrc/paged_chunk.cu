@@ -360,13 +360,13 @@ ChunkPlan plan_chunk(const RaggedShape& sh, int io_bf16, int kv_bf16, int sm_cou
     return plan;
 }
 
-template <int D, bool F32, typename T>
-cudaError_t launch_tc5(const ChunkPlan& plan, const RaggedShape& sh, const void* q, const void* k_pool, const void* v_pool,
+template <int D, bool F32, bool TINY, typename T>
+cudaError_t launch_tc5_kind(const ChunkPlan& plan, const RaggedShape& sh, const void* q, const void* k_pool, const void* v_pool,
                        const uint32_t* tables, const uint32_t* q_starts, const uint32_t* seq_lens, void* workspace, void* out, int sm_count,
                        uint32_t* err, cudaStream_t s) {
     using Cfg = TcCfg<D, F32>;
     static int configured[64] = {};
-    if (cudaError_t e = ensure_dynamic_smem(paged_chunk_tc5_kernel<D, F32, T>, Cfg::kSmem, configured)) return e;
+    if (cudaError_t e = ensure_dynamic_smem(paged_chunk_tc5_kernel<D, F32, TINY, T>, Cfg::kSmem, configured)) return e;
     CUtensorMap map_k, map_v;
     const int64_t pool_rows = int64_t(sh.num_blocks) * sh.block_size, ekv = int64_t(sh.num_kv_heads) * D;
     const int box = sh.block_size < kTcKeys ? sh.block_size : kTcKeys;
@@ -382,13 +382,19 @@ cudaError_t launch_tc5(const ChunkPlan& plan, const RaggedShape& sh, const void*
     float* part_o = static_cast<float*>(workspace);
     float2* part_ml = reinterpret_cast<float2*>(part_o + (plan.max_chunks > 1 ? sh.rows * sh.num_q_heads * plan.max_chunks * D : 0));
     const dim3 grid(static_cast<unsigned>(plan.items));
-    cudaError_t e = launch_ex(paged_chunk_tc5_kernel<D, F32, T>, grid, dim3(kTcThreads), Cfg::kSmem, s, 1, true, map_k, map_v, p,
+    cudaError_t e = launch_ex(paged_chunk_tc5_kernel<D, F32, TINY, T>, grid, dim3(kTcThreads), Cfg::kSmem, s, 1, true, map_k, map_v, p,
                               static_cast<const T*>(q), static_cast<const uint16_t*>(v_pool), tables, q_starts, seq_lens,
                               static_cast<T*>(out), part_o, part_ml, err);
     if (e != cudaSuccess || plan.max_chunks == 1) return e;
     const dim3 join(static_cast<unsigned>(sh.rows), (sh.num_q_heads + 7) / 8);
     return launch_ex(paged_chunk_join_kernel<D, T>, join, dim3(256), 0, s, 1, true, p, Cfg::kRows, q_starts, seq_lens, part_o, part_ml,
                      static_cast<T*>(out));
+}
+
+template <int D, bool F32, typename T, typename... Args>
+cudaError_t launch_tc5(const ChunkPlan& plan, const RaggedShape& sh, Args... args) {
+    if (int64_t(sh.max_q_len) * (sh.num_q_heads / sh.num_kv_heads) <= TcCfg<D, F32>::kTinyRows) return launch_tc5_kind<D, F32, true, T>(plan, sh, args...);
+    return launch_tc5_kind<D, F32, false, T>(plan, sh, args...);
 }
 
 }  // namespace

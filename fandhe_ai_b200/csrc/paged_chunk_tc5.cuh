@@ -21,6 +21,13 @@
 // three times in the tile of accumulator rows, so that three warps of a group hold the same scores, and each contributes one term
 // of the weights: one product gives the three partial results, which are added at the end.
 //
+// Items of very few rows ("tiny": at most 32, with three terms 10 - single tokens and short drafts) have them in each quarter of the
+// tile, term by term: warp w of a group exponentiates the keys [32 w, 32 w + 32) only and leaves its weights of the others at zero, so
+// a tile takes a quarter of the time; with three terms a score is put together by shuffles from the partial scores that lanes
+// r, r + 10 and r + 20 hold, which takes one product instead of three.  Each warp has its own maximum and sum.  A batch of nothing
+// but such items runs in a kernel of its own (TINY): what the other items need would only crowd its instruction cache, and the
+// other way round (in one kernel with it, fresh prompts took 270 us instead of 239).
+//
 // The softmax weights go to the MMA warp in two parts, so that the second product starts while the rest is still in the
 // exponential: 96 and 32 keys (little is left to multiply after the last weight), or with three terms 64 and 64.
 //
@@ -48,6 +55,7 @@ struct TcCfg {
     static constexpr int kStages = D == 128 ? (F32 ? 4 : 5) : 8;
     static constexpr int kSmem = kQBytes + kStages * kTileBytes + 3072;
     static constexpr int kRows = F32 ? 128 : 256;                            // rows of an item
+    static constexpr int kTinyRows = F32 ? 10 : 32;
 };
 
 struct TcShape {
@@ -296,7 +304,7 @@ struct TcShared {
 };
 static_assert(sizeof(TcShared) <= 3072, "");
 
-template <int D, bool F32, typename T>
+template <int D, bool F32, bool TINY, typename T>
 __global__ void __launch_bounds__(kTcThreads, 1)
 paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcShape p,
                        const T* __restrict__ q, const uint16_t* __restrict__ v_pool, const uint32_t* __restrict__ tables,
@@ -460,7 +468,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         for (TcItem* item; ok && (item = next_item(k_item)) != nullptr; ++k_item) {
             const TcOrder order(pos, *item);
             const int n = item->nt;
-            const bool split = item->split, stack = F32 && item->stack;
+            const bool split = TINY || item->split, stack = F32 && (TINY || item->stack);
             release_item(k_item);
             pos += 2 * n;
             // (the other group's part last: it is at most one item behind once this group has stored its part)
@@ -480,18 +488,21 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     if (!ok) break;
                     tc5_fence_after();
                     const uint64_t k_desc = umma_desc_k128(ring_addr + stage * Cfg::kTileBytes);
-                    if (elect_one()) {
+                    auto multiply = [&](auto terms) {
+                        if (elect_one()) {
 #pragma unroll
-                        for (int term = 0; term < Cfg::kQTerms; ++term)
+                            for (int term = 0; term < decltype(terms)::value; ++term)
 #pragma unroll
-                            for (int kk = 0; kk < D / 16; ++kk) {
-                                const uint32_t off = ((kk / 4) * kHalfBytes + (kk % 4) * 32) >> 4;
-                                umma_bf16_ss(d_s, q_desc + off + ((term * Cfg::kQTileBytes) >> 4), k_desc + off, kIdescS, term + kk > 0);
-                            }
-                        tc5_commit(smem_u32(&sh.s_full[s]));
-                        release(stage);
-                    }
-                    __syncwarp();
+                                for (int kk = 0; kk < D / 16; ++kk) {
+                                    const uint32_t off = ((kk / 4) * kHalfBytes + (kk % 4) * 32) >> 4;
+                                    umma_bf16_ss(d_s, q_desc + off + ((term * Cfg::kQTileBytes) >> 4), k_desc + off, kIdescS, term + kk > 0);
+                                }
+                            tc5_commit(smem_u32(&sh.s_full[s]));
+                            release(stage);
+                        }
+                        __syncwarp();
+                    };
+                    multiply(std::integral_constant<int, TINY ? 1 : Cfg::kQTerms>());
                 }
                 const uint32_t at = order.v(t), stage = at % kNst;
                 ok = wait(&sh.full[stage], (at / kNst) & 1);
@@ -524,12 +535,14 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 ok = ok && wait(&sh.p_full[s][0], p_phase & 1);
                 if (!ok) break;
                 tc5_fence_after();
-                if (F32 && stack) multiply(Zero(), One());
+                if constexpr (TINY) multiply(Zero(), One());
+                else if (F32 && stack) multiply(Zero(), One());
                 else multiply(Zero(), All());
                 ok = wait(&sh.p_full[s][1], p_phase & 1);
                 if (!ok) break;
                 tc5_fence_after();
-                if (F32 && stack) multiply(One(), One());
+                if constexpr (TINY) multiply(One(), One());
+                else if (F32 && stack) multiply(One(), One());
                 else multiply(One(), All());
                 ++p_phase;
             }
@@ -619,9 +632,10 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         };
         for (TcItem* item; ok && (item = next_item(k_item)) != nullptr; release_item(k_item++)) {
             const TcItem& it = *item;
-            const bool stack = F32 && it.stack;
-            const int r = stack ? row & 31 : (it.split ? 0 : wg * 128) + row;      // row of the item
-            const bool live = r < it.rows;
+            const bool stack = F32 && !TINY && it.stack, split = TINY || it.split;
+            constexpr int kTiny = Cfg::kTinyRows;
+            const int r = TINY ? lane % kTiny : (stack ? row & 31 : (split ? 0 : wg * 128) + row);      // row of the item
+            const bool live = r < it.rows && (!TINY || lane < Cfg::kQTerms * kTiny);
             // a warp without rows only keeps the barriers going: its accumulator rows hold garbage that nobody reads
             const bool busy = __any_sync(0xffffffffu, live) && !(stack && (warp & 3) == 3);
             const int list = it.row0 + r, token = list / p.group, head = it.kvh * p.group + list % p.group;
@@ -630,22 +644,22 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
             // The query tiles are free: a group that has its slot to itself waits for its own warps only, and so works through its
             // items independently of the other group.
-            if (!it.split) meet_group();
+            if (!split) meet_group();
             else if (!was_split) meet_all();
-            was_split = it.split;
+            was_split = split;
             if (!ok) break;
 
             // Queries into shared memory, 128-byte swizzled.  A warp reads whole rows (a lane 8 elements of one), several before it
             // uses the first; a tile that both slots use is shared out over all eight warps.
             {
                 constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces, kBatch = F32 ? 2 : 8;
-                const int per = stack ? 4 : (it.split ? 16 : 32), base = (it.split ? warp : warp & 3) * per;
-                const int first = (it.split ? 0 : wg * 128) + base, count = min(per, it.rows - first);      // rows of this warp (<= 0: none)
+                const int per = stack || TINY ? 4 : (split ? 16 : 32), base = (split ? warp : warp & 3) * per;
+                const int first = (split ? 0 : wg * 128) + base, count = min(per, it.rows - first);      // rows of this warp (<= 0: none)
                 // place of the row base + lane; rows that the item does not have read its first row and are set to zero
                 const int at = it.row0 + (lane < count ? first + lane : 0), tok = at / p.group;
                 const int64_t from = (int64_t(it.start) + tok) * p.sh.row_stride + int64_t(it.kvh * p.group + at - tok * p.group) * D;
                 const int piece = lane % kPieces;
-                unsigned char* dst = q_smem + (it.split ? 0 : wg) * Cfg::kQTileBytes + (piece / 8) * kHalfBytes;
+                unsigned char* dst = q_smem + (split ? 0 : wg) * Cfg::kQTileBytes + (piece / 8) * kHalfBytes;
                 for (int j0 = lane / kPieces; j0 < per; j0 += kBatch * kAtOnce) {
                     using Raw = Pack<T, 8>;
                     Raw raw[kBatch];
@@ -673,8 +687,17 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                                 x[2 * k + 1] -= bf16_hi(w[k]);
                             }
                             unsigned char* tile = dst + term * Cfg::kQTileBytes;
-                            if (j < per) *reinterpret_cast<uint4*>(tile + to * 128 + sw) = make_uint4(w[0], w[1], w[2], w[3]);
-                            if (stack && j < per) {
+                            if constexpr (TINY) {
+                                if (j < per && to < kTiny) {
+#pragma unroll
+                                    for (int quarter = 0; quarter < 4; ++quarter) {
+                                        const int tr = quarter * 32 + term * kTiny + to;
+                                        *reinterpret_cast<uint4*>(dst + tr * 128 + (((piece % 8) ^ (tr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                                    }
+                                }
+                            }
+                            if (!TINY && j < per) *reinterpret_cast<uint4*>(tile + to * 128 + sw) = make_uint4(w[0], w[1], w[2], w[3]);
+                            if (!TINY && stack && j < per) {
                                 *reinterpret_cast<uint4*>(tile + (32 + to) * 128 + sw) = make_uint4(w[0], w[1], w[2], w[3]);
                                 *reinterpret_cast<uint4*>(tile + (64 + to) * 128 + sw) = make_uint4(w[0], w[1], w[2], w[3]);
                             }
@@ -688,9 +711,9 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
 
             float m = -INFINITY, l = 0.0f;
-            const int masked_from = it.min_limit / kTcKeys - it.t0, step = it.split ? 2 : 1, nt = it.nt, k0 = it.t0 * kTcKeys;
+            const int masked_from = it.min_limit / kTcKeys - it.t0, step = split ? 2 : 1, nt = it.nt, k0 = it.t0 * kTcKeys;
             int done = 0;
-            for (int t = it.split ? wg : 0; t < nt; t += step, ++done) {
+            for (int t = split ? wg : 0; t < nt; t += step, ++done) {
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.s_full[wg]), s_phase & 1, err, kErrEpilogueWait));
                 if (!ok) break;
                 if (!busy) {
@@ -727,7 +750,66 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     }
                 };
                 F2 sum[2] = {F2(0.0f, 0.0f), F2(0.0f, 0.0f)};
-                if constexpr (!F32) {
+                if constexpr (TINY) {
+                    const int key0 = (warp & 3) * 32;
+                    uint32_t raw[32];
+                    tmem_ld_32x32(t_s + key0, raw);
+                    tmem_ld_wait();
+                    if constexpr (F32) {      // the three partial scores, added in the same order by all three lanes
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            const float v = __uint_as_float(raw[k]);
+                            const float a = __shfl_sync(0xffffffffu, v, r), b = __shfl_sync(0xffffffffu, v, r + 10), d = __shfl_sync(0xffffffffu, v, r + 20);
+                            raw[k] = __float_as_uint((d + b) + a);
+                        }
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (key0 + k >= visible) raw[k] = 0xFF800000u;
+                    }
+                    float mx[4];
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        mx[g] = max_nan(__uint_as_float(raw[g]), __uint_as_float(raw[g + 4]));
+#pragma unroll
+                        for (int k = 8; k < 32; k += 8) mx[g] = max_nan(mx[g], __uint_as_float(raw[k + g]), __uint_as_float(raw[k + g + 4]));
+                    }
+                    raise(max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])));
+                    const float mc = m == -INFINITY ? 0.0f : (m == INFINITY ? __int_as_float(0x7FC00000) : m * c);
+                    const F2 c2(c, c), mc2(-mc, -mc);
+                    const int term = F32 ? lane / kTiny : 0;
+                    uint32_t w[16];
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        float a, b;
+                        fma2(F2(__uint_as_float(raw[k]), __uint_as_float(raw[k + 1])), c2, mc2).get(a, b);
+                        a = ex2(a);
+                        b = ex2(b);
+                        sum[(k / 2) & 1] = add2(sum[(k / 2) & 1], F2(a, b));
+                        if constexpr (F32) {
+                            uint32_t w0 = cut_bf16(a, b);
+                            cut_rest(a, b).get(a, b);
+                            const uint32_t w1 = cut_bf16(a, b);
+                            cut_rest(a, b).get(a, b);
+                            w[k / 2] = term == 0 ? w0 : (term == 1 ? w1 : cut_bf16(a, b));
+                        } else {
+                            w[k / 2] = pack_bf16(a, b);
+                        }
+                    }
+                    tmem_st_32x16(t_s + (warp & 3) * 16, w);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) w[k] = 0;
+#pragma unroll
+                    for (int g = 1; g < 4; ++g) tmem_st_32x16(t_s + ((warp + g) & 3) * 16, w);
+                    tmem_st_wait();
+                    tc5_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_u32(&sh.p_full[wg][0]));
+                        mbar_arrive(smem_u32(&sh.p_full[wg][1]));
+                    }
+                } else if constexpr (!F32) {
                     float s[128];      // the whole row stays in registers
                     {
                         uint32_t raw[4][32];
@@ -917,8 +999,8 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             auto staged = [&](unsigned char* area, int width, int rr, int col) -> float4* {
                 return reinterpret_cast<float4*>(area + (size_t(rr) * width + (((col >> 2) ^ (rr & 7)) << 2)) * 4);
             };
-            if (!it.split) {
-                if constexpr (!F32) {
+            if (!TINY && !split) {
+                if constexpr (!F32 && !TINY) {
                     patch = *reinterpret_cast<volatile uint32_t*>(&item->nonfinite) != 0;      // set before the products that o_full stands for
                     const float inv = direct ? 1.0f / l : 1.0f;
                     // 32 rows of 64 columns at a time in this warp's part of its group's query tile (D = 64: of 32 columns)
@@ -952,13 +1034,81 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 tc5_fence_before();
             } else {
                 const int lane_row = stack ? lane : row;
-                if (!stack || (warp & 3) == 0) {
-                    sh.xm[wg][row] = m;
-                    sh.xl[wg][row] = l;
-                }
+                sh.xm[wg][row] = m;
+                sh.xl[wg][row] = l;
                 meet_all();      // every product that reads the query tile is complete: it may be overwritten
                 if (!ok) break;
                 patch = *reinterpret_cast<volatile uint32_t*>(&item->nonfinite) != 0;
+                if constexpr (TINY) {
+                    // Row rr: the sum over slots, warps and terms.  One slot's accumulator rows at a time fit the query tiles.
+                    constexpr int kMost = (kTiny + 7) / 8;
+                    float o[kMost][4], top[kMost], total[kMost];
+                    const int col = lane * 4;
+#pragma unroll
+                    for (int j = 0; j < kMost; ++j) {
+                        const int rr = min(warp + j * 8, kTiny - 1);
+                        top[j] = -INFINITY;
+                        total[j] = 0.0f;
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) top[j] = max_nan(top[j], sh.xm[x >> 2][(x & 3) * 32 + rr]);
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const float mx = sh.xm[x >> 2][(x & 3) * 32 + rr];
+                            if (mx != -INFINITY) total[j] = fmaf(sh.xl[x >> 2][(x & 3) * 32 + rr], ex2((mx - top[j]) * c), total[j]);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[j][k] = 0.0f;
+                    }
+#pragma unroll 1
+                    for (int from = 0; from < 2; ++from) {
+                        if (wg == from && done > 0) {
+#pragma unroll
+                            for (int g = 0; g < D / 32; ++g) {
+                                uint32_t raw[32];
+                                tmem_ld_32x32(t_o + g * 32, raw);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int k = 0; k < 32; k += 4)
+                                    *staged(q_smem, D, row, g * 32 + k) = make_float4(__uint_as_float(raw[k]), __uint_as_float(raw[k + 1]),
+                                                                                      __uint_as_float(raw[k + 2]), __uint_as_float(raw[k + 3]));
+                            }
+                        }
+                        meet_all();
+#pragma unroll
+                        for (int j = 0; j < kMost; ++j) {
+                            const int rr = warp + j * 8;
+                            if (rr >= it.rows || col >= D) continue;
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const float mx = sh.xm[from][x * 32 + rr];
+                                if (mx == -INFINITY) continue;      // no key there
+                                const float f = ex2((mx - top[j]) * c);
+                                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                                for (int term = Cfg::kQTerms - 1; term >= 0; --term) {
+                                    const float4 y = *staged(q_smem, D, x * 32 + term * kTiny + rr, col);
+                                    v[0] += y.x; v[1] += y.y; v[2] += y.z; v[3] += y.w;
+                                }
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) o[j][k] = fmaf(v[k], f, o[j][k]);
+                            }
+                        }
+                        meet_all();      // read: the other slot's rows, or the next item's queries, may come
+                        if (!ok) break;
+                    }
+                    if (!ok) break;
+#pragma unroll
+                    for (int j = 0; j < kMost; ++j) {
+                        const int rr = warp + j * 8, reach = reach_of(min(rr, kTiny - 1));
+                        const int64_t to_row = row_of(min(rr, kTiny - 1));
+                        if (rr >= it.rows) continue;
+                        if (lane == 0 && !direct) part_ml[to_row * p.max_chunks + it.chunk] = make_float2(top[j] * c, total[j]);
+                        const float inv = direct ? 1.0f / total[j] : 1.0f;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[j][k] *= inv;
+                        if (col < D) finish(to_row, reach, col, o[j]);
+                    }
+                } else {
                 const float m0 = sh.xm[0][lane_row], m1 = sh.xm[1][lane_row], mt = fmaxf(m0, m1);
                 const float f0 = m0 == -INFINITY ? 0.0f : ex2((m0 - mt) * c), f1 = m1 == -INFINITY ? 0.0f : ex2((m1 - mt) * c);
                 const float lt = fmaf(sh.xl[0][lane_row], f0, sh.xl[1][lane_row] * f1);
@@ -1046,6 +1196,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         });
                 }
                 meet_all();      // the exchanged halves have been read
+                }
             }
         }
     }
