@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
                                                                  float* __restrict__ prob, int* __restrict__ kept) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
-    float* xs = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
+    T* xs = reinterpret_cast<T*>(smem_raw + (sizeof(Shared) + 15) / 16 * 16);      // in their own type
     const uint32_t nranks = p.cluster, rank = nranks > 1 ? cluster_ctarank() : 0;
     const int64_t row = blockIdx.x / nranks;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -208,7 +208,6 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
     // ---- the row into shared memory; its first maximum; is there a NaN or +inf?
     uint64_t best = 0, bad = 0;
     auto take = [&](int i, float x) {
-        xs[i] = x;
         if (!(x < INFINITY)) bad = 1;
         const uint64_t pr = order_pair(x, uint32_t(first) + i);
         if (x != -INFINITY && pr > best) best = pr;
@@ -222,11 +221,15 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         for (int g = tid; g < n / kVec; g += kThreads) {
             const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(src) + g);
             const T* v = reinterpret_cast<const T*>(&raw);
+            reinterpret_cast<uint4*>(xs)[g] = raw;
 #pragma unroll
             for (int k = 0; k < kVec; ++k) take(g * kVec + k, logit_f32<T>(v[k]));
         }
     }
-    for (int i = done + tid; i < n; i += kThreads) take(i, logit_f32<T>(src[i]));
+    for (int i = done + tid; i < n; i += kThreads) {
+        xs[i] = src[i];
+        take(i, logit_f32<T>(src[i]));
+    }
     for (int b = tid; b < kBins; b += kThreads) sh.hist[b] = 0;
     if (tid < 64) sh.roots[tid] = kRoots[tid];
     if (tid == 0) sh.n_cand = 0;
@@ -265,7 +268,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
     const int run = p.run;
     int lo = tid * run, hi = min(n, lo + run);      // this thread's elements: of the block's share, or of the list
     bool listed = false;
-    auto X = [&](int i) { return listed ? sh.list_x[i] : xs[i]; };
+    auto X = [&](int i) { return listed ? sh.list_x[i] : logit_f32<T>(xs[i]); };
     auto index = [&](int i) { return uint32_t(first) + (listed ? uint32_t(sh.list_i[i]) : uint32_t(i)); };
 
     // Every block hands the tokens of bin `b` to all blocks, as ordered pairs (0: not among `under`); returns how many places that
@@ -320,7 +323,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
             int b[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                x[q] = i0 + q < hi ? xs[i0 + q] : -INFINITY;
+                x[q] = i0 + q < hi ? logit_f32<T>(xs[i0 + q]) : -INFINITY;
                 b[q] = r.bin(x[q]);
             }
 #pragma unroll
@@ -435,7 +438,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         for (int i0 = lo; i0 < lo + run; i0 += 8) {
             uint32_t some = 0;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) some |= (i0 + q < hi && xs[i0 + q] >= least ? 1u : 0u) << q;
+            for (int q = 0; q < 8; ++q) some |= (i0 + q < hi && logit_f32<T>(xs[i0 + q]) >= least ? 1u : 0u) << q;
             mine |= uint64_t(some) << (i0 - lo);
         }
         const int count = __popcll(mine);
@@ -457,7 +460,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
             while (mine) {
                 const int j = __ffsll(static_cast<long long>(mine)) - 1;
                 mine &= mine - 1;
-                sh.list_x[at] = xs[lo + j];
+                sh.list_x[at] = logit_f32<T>(xs[lo + j]);
                 sh.list_i[at++] = uint16_t(lo + j);
             }
             __syncthreads();
@@ -641,7 +644,7 @@ cudaError_t sample_tokens(const SampleShape& want, const void* logits, int bf16,
     int bits = 12;                                              // weights below 2^52, see Row::weight
     while ((int64_t(1) << bits) < p.vocab) ++bits;
     p.shift = 62 - bits;
-    const int smem = int(sizeof(Shared)) + p.per_cta * 4;
+    const int smem = int((sizeof(Shared) + 15) / 16 * 16) + p.per_cta * (bf16 ? 2 : 4);
     static int configured[2][64] = {};
     const dim3 grid(static_cast<unsigned>(p.rows * c));
     if (bf16) {
