@@ -296,6 +296,10 @@ struct b200_decoder {
     cudaEvent_t ids_copied = nullptr;           // the staged ids of the previous step have reached the device
     bool ids_copy_pending = false;
     int* next_pinned = nullptr;
+    float* sample_dev = nullptr;                // per-row sampling parameters: temperature, top_k, top_p, min_p, uniform, M of each
+    float* sample_pinned = nullptr;
+    cudaEvent_t sample_copied = nullptr;        // the staged parameters of the previous draw have reached the device
+    bool sample_copy_pending = false;
     // graph
     cudaGraphExec_t graph = nullptr;
     int eager_steps_done = 0;
@@ -875,6 +879,9 @@ int32_t b200_decoder_create(b200_ctx* ctx, const b200_decoder_config* cfg, b200_
     A(dmalloc(&d->logits, M * size_t(c.vocab)));
     A(cudaMallocHost(reinterpret_cast<void**>(&d->ids_pinned), M * sizeof(int)));
     A(cudaEventCreateWithFlags(&d->ids_copied, cudaEventDisableTiming));
+    A(dmalloc(&d->sample_dev, M * 5));
+    A(cudaMallocHost(reinterpret_cast<void**>(&d->sample_pinned), M * 5 * sizeof(float)));
+    A(cudaEventCreateWithFlags(&d->sample_copied, cudaEventDisableTiming));
     A(cudaMallocHost(reinterpret_cast<void**>(&d->next_pinned), M * sizeof(int)));
     if (e == cudaSuccess) e = cudaMemsetAsync(d->vectors, 0, vec * sizeof(float), ctx->stream);
     if (e != cudaSuccess) {
@@ -931,11 +938,13 @@ int32_t b200_decoder_destroy(b200_decoder* d) {
     for (void* p : pf_ptrs) cudaFree(p);
     void* ptrs[] = {d->payload, d->scales, d->vectors, d->embed, d->cos_t, d->sin_t, d->tables_dev, d->seq_lens_dev, d->pos_dev,
                     d->ids_dev, d->next_ids_dev, d->h, d->xq, d->sx, d->raw, d->q, d->attn_out, d->part, d->logits,
-                    d->attn_scratch, d->tp_block, d->tp_epoch, d->tp_peers_dev, d->active_dev, d->tp_amax, d->tp_rows_f32, d->tp_acc};
+                    d->attn_scratch, d->tp_block, d->tp_epoch, d->tp_peers_dev, d->active_dev, d->tp_amax, d->tp_rows_f32, d->tp_acc, d->sample_dev};
     for (void* p : ptrs) cudaFree(p);
     if (d->ids_pinned) cudaFreeHost(d->ids_pinned);
     if (d->active_pinned) cudaFreeHost(d->active_pinned);
     if (d->ids_copied) cudaEventDestroy(d->ids_copied);
+    if (d->sample_pinned) cudaFreeHost(d->sample_pinned);
+    if (d->sample_copied) cudaEventDestroy(d->sample_copied);
     if (d->next_pinned) cudaFreeHost(d->next_pinned);
     b200_block_table_destroy(d->table);
     cudaGetLastError();
@@ -1764,6 +1773,48 @@ int32_t b200_decoder_row_restart(b200_decoder* d, int32_t row, int32_t max_total
                            cudaMemcpyHostToDevice, s));
     CU_TRY(cudaMemcpyAsync(d->seq_lens_dev + row, &zero, 4, cudaMemcpyHostToDevice, s));
     CU_TRY(cudaStreamSynchronize(s));      // the host vectors above go out of scope
+    return B200_OK;
+}
+
+// Draws the next ids from the logits of the last step on the device, in place of the greedy ones.
+int32_t b200_decoder_sample(b200_decoder* d, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                            const float* uniform, int32_t* next_ids_host) {
+    if (int32_t st = dec_check(d)) return st;
+    if (!d->planned || d->steps == 0) return fail(B200_INVALID_ARGUMENT, "decoder_sample: no step has run");
+    if (!uniform) return fail(B200_INVALID_ARGUMENT, "decoder_sample: uniform is null");
+    if (d->cfg.vocab > sample_tokens_max_vocab()) return fail(B200_UNSUPPORTED, "decoder_sample: vocabulary too large for the sampling kernel");
+    const int M = d->batch;
+    for (int b = 0; b < M; ++b) {
+        const std::string row = "decoder_sample: row " + std::to_string(b) + ": ";
+        if (temperature && !(temperature[b] >= 0.0f && std::isfinite(temperature[b]))) return fail(B200_INVALID_ARGUMENT, row + "temperature must be finite and not negative");
+        if (!(uniform[b] >= 0.0f && uniform[b] < 1.0f)) return fail(B200_INVALID_ARGUMENT, row + "uniform must be in [0, 1)");
+        if ((top_p && std::isnan(top_p[b])) || (min_p && std::isnan(min_p[b]))) return fail(B200_INVALID_ARGUMENT, row + "top_p and min_p must not be NaN");
+    }
+    cudaStream_t s = d->ctx->stream;
+    if (d->sample_copy_pending) CU_TRY(cudaEventSynchronize(d->sample_copied));      // read when the copy executes, as the ids are
+    const void* host[5] = {temperature, top_k, top_p, min_p, uniform};
+    for (int i = 0; i < 5; ++i)
+        if (host[i]) std::memcpy(d->sample_pinned + size_t(i) * M, host[i], size_t(M) * 4);
+        else std::memset(d->sample_pinned + size_t(i) * M, 0, size_t(M) * 4);
+    CU_TRY(cudaMemcpyAsync(d->sample_dev, d->sample_pinned, size_t(M) * 5 * 4, cudaMemcpyHostToDevice, s));
+    CU_TRY(cudaEventRecord(d->sample_copied, s));
+    d->sample_copy_pending = true;
+    auto param = [&](int i) -> const float* { return host[i] ? d->sample_dev + size_t(i) * M : nullptr; };
+    SampleShape sh = {};
+    sh.rows = M;
+    sh.row_stride = sh.vocab = d->cfg.vocab;
+    CU_TRY(sample_tokens(sh, d->logits, 0, param(0), reinterpret_cast<const int*>(param(1)), param(2), param(3), param(4), d->next_ids_dev, nullptr,
+                         nullptr, d->ctx->sm_count, s));
+    if (next_ids_host) {
+        CU_TRY(cudaMemcpyAsync(d->next_pinned, d->next_ids_dev, size_t(M) * sizeof(int), cudaMemcpyDeviceToHost, s));
+        if (int32_t st = b200_synchronize(d->ctx)) {
+            d->store_poisoned = true;
+            return st;
+        }
+        std::memcpy(next_ids_host, d->next_pinned, size_t(M) * sizeof(int));
+        for (int b = 0; b < M; ++b)
+            if (next_ids_host[b] < 0) return fail(B200_INVALID_ARGUMENT, "decoder_sample: row " + std::to_string(b) + " holds a NaN or infinite logit");
+    }
     return B200_OK;
 }
 

@@ -243,6 +243,16 @@ class Decoder:
         check(lib().b200_decoder_logits(self._h, out.ctypes.data_as(C.c_void_p), out.size))
         return out
 
+    def sample(self, uniform, temperature=None, top_k=None, top_p=None, min_p=None, want_ids: bool = True):
+        """Draws the next ids from the last step's logits on the device (scalars or one value per row; None: off) from the
+        given uniform numbers; `step()` without ids feeds them.  Returns them, or None with want_ids False."""
+        def rows(v, dtype):
+            return None if v is None else np.ascontiguousarray(np.broadcast_to(np.asarray(v, dtype), (self._batch,)))
+        a = [rows(v, t) for v, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32), (uniform, np.float32))]
+        ids = np.empty(self._batch, np.int32) if want_ids else None
+        check(lib().b200_decoder_sample(self._h, *[x.ctypes.data_as(C.c_void_p) if x is not None else None for x in [*a, ids]]))
+        return ids
+
     def sampling_weights(self, strategy: int, k: int = 0, temperature: float = 1.0) -> np.ndarray:
         """[batch, vocab] f32 weights of the last step's logits, as the reference's sample_step builds them before
         it draws (crates/autodiff/src/generate/mod.rs:382-455); the draw stays with the caller's generator."""

@@ -613,6 +613,14 @@ int32_t b200_sampling_weights(const float* logits, int64_t rows, int64_t vocab, 
 /* The same for the logits of the decoder's last step: weights_out[batch][vocab] (host, capacity in elements). */
 int32_t b200_decoder_sampling_weights(b200_decoder* dec, int32_t strategy, int32_t k, float temperature, float* weights_out,
                                       uint64_t capacity_elems);
+/* The draw itself on the device, from given random numbers: b200_sample_tokens on the logits of the last step, whose ids replace
+ * the greedy ones (a following b200_decoder_step with ids NULL feeds them).  Host arrays of one value per row of the running
+ * generation; all but `uniform` may be NULL (off).  next_ids_host != NULL: the drawn ids are copied back (this synchronises; a
+ * row whose logits are not finite is InvalidArgument, as in sample_step).  Without it nothing leaves the device; such a row
+ * then fails the next step's check of its ids.  No logits and no weights cross to the host, unlike
+ * b200_decoder_sampling_weights, which serves the reference's own generator. */
+int32_t b200_decoder_sample(b200_decoder* dec, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                            const float* uniform, int32_t* next_ids_host);
 /* Between steps: empties row `row` (its blocks return to the free stack) and reserves blocks for a new sequence
  * of up to max_total_len tokens (at most the largest length given to b200_decoder_begin). */
 int32_t b200_decoder_row_restart(b200_decoder* dec, int32_t row, int32_t max_total_len);

@@ -519,3 +519,53 @@ def test_a_captured_step_replays_with_other_inputs(be):
     st.bt = bt
     st.check(qkv)
     del graph
+
+
+def make_small_decoder(be, batch):
+    from fandhe_ai_b200.decoder import Decoder, DecoderConfig
+
+    cfg = dict(n_layers=2, d_model=256, n_heads=4, n_kv_heads=2, head_dim=64, d_ff=512, vocab=512)
+    dec = Decoder(be, DecoderConfig(**cfg, max_batch=batch, max_seq_len=32))
+    dec.init_random(3, 0.05)
+    return dec
+
+
+def test_decoder_draws_on_the_device_and_feeds_what_it_drew(be):
+    """Two decoders with the same weights: one draws on the device and feeds its ids without the host, the other gets the plain form's
+    draws from its own logits as host ids.  They must stay together."""
+    rng = np.random.default_rng(30)
+    batch, steps = 3, 10
+    a, b = make_small_decoder(be, batch), make_small_decoder(be, batch)
+    try:
+        for dec in (a, b):
+            dec.begin(batch, [steps + 2] * batch)
+        ids = np.array([3, 77, 400], np.int32)
+        a.step(ids, want_next=False)
+        b.step(ids)
+        t, k, p, m = np.array([0.7, 1.5, 0.0]), np.array([0, 40, 0]), np.array([0.9, 1.0, 1.0]), 0.02
+        for s in range(steps):
+            u = rng.random(batch).astype(np.float32)
+            logits = b.logits()
+            assert np.array_equal(logits, a.logits())
+            want = [sample_ref(logits[r], float(np.float32(t[r])), int(k[r]), float(np.float32(p[r])), float(np.float32(m)), float(u[r]))[0] for r in range(batch)]
+            got = a.sample(u, t, k, p, m, want_ids=s % 2 == 0)
+            if got is not None:
+                assert got.tolist() == want
+            a.step(None, want_next=False)
+            b.step(np.array(want, np.int32))
+        for bad in (dict(uniform=[0.1, 1.0, 0.2]), dict(uniform=0.1, temperature=-1.0), dict(uniform=0.1, top_p=np.nan)):
+            with pytest.raises(BackendError):
+                a.sample(**bad)
+    finally:
+        a.close()
+        b.close()
+
+
+def test_decoder_sample_needs_a_step(be):
+    dec = make_small_decoder(be, 2)
+    try:
+        dec.begin(2, [4, 4])
+        with pytest.raises(BackendError):
+            dec.sample(0.5)
+    finally:
+        dec.close()
