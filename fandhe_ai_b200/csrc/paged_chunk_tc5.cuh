@@ -652,7 +652,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             // Queries into shared memory, 128-byte swizzled.  A warp reads whole rows (a lane 8 elements of one), several before it
             // uses the first; a tile that both slots use is shared out over all eight warps.
             {
-                constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces, kBatch = F32 ? 2 : 8;
+                constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces, kBatch = F32 ? 2 : 4;
                 const int per = stack || TINY ? 4 : (split ? 16 : 32), base = (split ? warp : warp & 3) * per;
                 const int first = (split ? 0 : wg * 128) + base, count = min(per, it.rows - first);      // rows of this warp (<= 0: none)
                 // place of the row base + lane; rows that the item does not have read its first row and are set to zero
@@ -660,6 +660,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 const int64_t from = (int64_t(it.start) + tok) * p.sh.row_stride + int64_t(it.kvh * p.group + at - tok * p.group) * D;
                 const int piece = lane % kPieces;
                 unsigned char* dst = q_smem + (split ? 0 : wg) * Cfg::kQTileBytes + (piece / 8) * kHalfBytes;
+#pragma unroll 1
                 for (int j0 = lane / kPieces; j0 < per; j0 += kBatch * kAtOnce) {
                     using Raw = Pack<T, 8>;
                     Raw raw[kBatch];
@@ -738,7 +739,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         const float f = m_new == m ? 1.0f : ex2((m - m_new) * c);
                         m = m_new;
                         l *= f;
-#pragma unroll
+#pragma unroll 1
                         for (int g = 0; g < D / 16; ++g) {
                             uint32_t o[16];
                             tmem_ld_32x16(t_o + g * 16, o);
@@ -862,7 +863,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 } else {
                     // The scores are read twice, 32 at a time: a row of them and its three terms do not fit the registers together.
                     float top = -INFINITY;
-#pragma unroll
+#pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
                         uint32_t raw[2][32];
                         tmem_ld_32x32(t_s + h * 64, raw[0]);
@@ -981,7 +982,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             // reads the staged columns of a row.
             auto write_rows = [&](auto lanes, auto columns, int col0, auto get) {
                 constexpr int kLanes = decltype(lanes)::value, N = decltype(columns)::value, kAtOnce = 32 / kLanes, kSteps = 32 / kAtOnce;
-                constexpr int kBatch = kSteps < 8 ? kSteps : 8;
+                constexpr int kBatch = kSteps < 2 ? kSteps : 2;
                 const int col = lane % kLanes * N;
 #pragma unroll 1
                 for (int j0 = 0; j0 < 32; j0 += kBatch * kAtOnce) {
@@ -1006,10 +1007,10 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     // 32 rows of 64 columns at a time in this warp's part of its group's query tile (D = 64: of 32 columns)
                     constexpr int kCols = D / 2;
                     unsigned char* area = q_smem + wg * Cfg::kQTileBytes + (warp & 3) * (Cfg::kQTileBytes / 4);
-#pragma unroll
+#pragma unroll 1
                     for (int part = 0; part < 2; ++part) {
                         if (busy) {
-#pragma unroll
+#pragma unroll 1
                             for (int g = 0; g < kCols / 32; ++g) {
                                 uint32_t raw[32];
                                 tmem_ld_32x32(t_o + part * kCols + g * 32, raw);
@@ -1117,7 +1118,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 if (!direct && live && warp == (stack ? 0 : warp & 3)) part_ml[out_row * p.max_chunks + it.chunk] = make_float2(mt * c, lt);
                 if (stack) {
                     if (busy) {
-#pragma unroll
+#pragma unroll 1
                         for (int g = 0; g < D / 32; ++g) {
                             uint32_t raw[32];
                             if (done > 0) {
@@ -1152,7 +1153,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     constexpr int kCols = D / 2;
                     const int other = wg ^ 1;
                     if (busy) {
-#pragma unroll
+#pragma unroll 1
                         for (int g = 0; g < kCols / 32; ++g) {
                             uint32_t raw[32];
                             if (done > 0) {
@@ -1170,7 +1171,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     meet_all();
                     unsigned char* area = q_smem + wg * 128 * kCols * 4;
                     if (busy && done > 0) {
-#pragma unroll
+#pragma unroll 1
                         for (int g = 0; g < kCols / 32; ++g) {
                             uint32_t raw[32];
                             tmem_ld_32x32(t_o + wg * kCols + g * 32, raw);
