@@ -454,6 +454,12 @@ int32_t b200_release(b200_ctx* ctx, b200_buf* buf) {
     if (!ctx || buf->owner != ctx) return fail(B200_DEVICE_MISMATCH, "release: buffer belongs to another context");
     if (buf->ptr) {
         cudaSetDevice(ctx->ordinal);
+        // (a handle of the caller's memory may go while its stream is being captured, which a wait would end)
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        if (buf->imported && cudaStreamIsCapturing(ctx->stream, &capturing) == cudaSuccess && capturing != cudaStreamCaptureStatusNone) {
+            delete buf;
+            return B200_OK;
+        }
         cudaStreamSynchronize(ctx->stream);
         if (!buf->imported) cudaFree(buf->ptr);
         cudaGetLastError();

@@ -116,10 +116,10 @@ rope_append_kernel(RaggedShape sh, RopeShape rope, int rows_per_block, const T* 
         }
         if (lane == 0) {
             AppendRow to = {-1, 0};
-            if (seq < sh.batch) {          // else behind the last sequence
+            if (seq < sh.batch && row >= int64_t(q_starts[seq])) {          // else behind the last sequence
                 const int64_t pos = int64_t(seq_lens[seq]) - (int64_t(q_starts[seq + 1]) - row);      // position in the cache
                 to.angle = positions ? int64_t(positions[row]) : pos;
-                if (pos < 0 || pos >= int64_t(sh.max_blocks_per_seq) * sh.block_size || to.angle < 0 || to.angle >= rope.n_positions) {
+                if (pos < 0 || pos >= int64_t(sh.max_blocks_per_seq) * sh.block_size || (rope.rotary_dim > 0 && (to.angle < 0 || to.angle >= rope.n_positions))) {
                     atomicCAS(err, 0u, static_cast<uint32_t>(kErrRaggedBatch));
                 } else {
                     const uint32_t blk = tables[int64_t(seq) * sh.max_blocks_per_seq + pos / sh.block_size];
@@ -247,7 +247,7 @@ paged_chunk_generic_kernel(RaggedShape sh, const T* __restrict__ q, const KvT* _
     const int64_t row = blockIdx.x;
     const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int seq = sequence_of_row(q_starts, sh.batch, row);
-    if (seq >= sh.batch) return;
+    if (seq >= sh.batch || row < int64_t(q_starts[seq])) return;
     const int dh = sh.head_dim;
     const int64_t len = seq_lens[seq], new_rows = int64_t(q_starts[seq + 1]) - int64_t(q_starts[seq]);
     const int64_t cap = int64_t(sh.max_blocks_per_seq) * sh.block_size;

@@ -491,11 +491,13 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     auto multiply = [&](auto terms) {
                         if (elect_one()) {
 #pragma unroll
-                            for (int term = 0; term < decltype(terms)::value; ++term)
+                            for (int left = decltype(terms)::value - 1; left >= 0; --left)      // the small terms first: every step cuts to the sum's precision
 #pragma unroll
                                 for (int kk = 0; kk < D / 16; ++kk) {
+                                    constexpr int kTerms = decltype(terms)::value;
+                                    const int term = left;
                                     const uint32_t off = ((kk / 4) * kHalfBytes + (kk % 4) * 32) >> 4;
-                                    umma_bf16_ss(d_s, q_desc + off + ((term * Cfg::kQTileBytes) >> 4), k_desc + off, kIdescS, term + kk > 0);
+                                    umma_bf16_ss(d_s, q_desc + off + ((term * Cfg::kQTileBytes) >> 4), k_desc + off, kIdescS, term < kTerms - 1 || kk > 0);
                                 }
                             tc5_commit(smem_u32(&sh.s_full[s]));
                             release(stage);
@@ -1218,7 +1220,7 @@ paged_chunk_join_kernel(const __grid_constant__ TcShape p, int tile_rows, const 
     const int seq = sequence_of_row(q_starts, p.sh.batch, row);
     if (seq >= p.sh.batch) return;
     const int64_t s = q_starts[seq], e = q_starts[seq + 1], len = seq_lens[seq];
-    if (e > p.sh.rows || e - s > len || e - s > p.sh.max_q_len || len > p.sh.max_seq_len) return;      // reported by the first kernel
+    if (row < s || e > p.sh.rows || e - s > len || e - s > p.sh.max_q_len || len > p.sh.max_seq_len) return;      // reported by the first kernel
     const int n = int(e - s), token = int(row - s);
     const int chunks = ((int(len) + kTcKeys - 1) / kTcKeys + p.chunk_tiles - 1) / p.chunk_tiles;
     if (chunks == 1) return;                                                                            // written already

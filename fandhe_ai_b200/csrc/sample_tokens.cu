@@ -31,9 +31,9 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kCandidates = 512;
-constexpr int kSurvivors = 2048;
+constexpr int kSurvivors = 3584;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxPerCta = 49152;      // 192 KB of f32 logits per thread block
+constexpr int kMaxPerCta = 45056;      // f32 logits of a thread block: 176 KB, which leaves room for what else it keeps
 
 // 2^(j / 64)
 __constant__ double kRoots[64] = {
@@ -104,6 +104,8 @@ template <>
 __device__ __forceinline__ float logit_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ float logit_f32<uint16_t>(uint16_t v) { return bf16_bits_to_f32(v); }
+
+static_assert(sizeof(Shared) + 16 + kMaxPerCta * 4 <= 232448, "a thread block's shared memory");
 
 struct Row {
     float max_x, bin_scale;

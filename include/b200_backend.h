@@ -131,7 +131,7 @@ void* b200_buf_device_ptr(const b200_buf* buf);
 /* A handle for device memory that belongs to the caller (another library's allocation on the same ordinal); the one
  * exception to "buffers are created only by the backend", with no counterpart in the reference.  Both ends of the range
  * are checked to be device memory of the context's ordinal (InvalidArgument / DeviceMismatch); the memory must stay
- * allocated until b200_release, which waits for the context's stream and frees the handle only.  The context works on its
+ * allocated until b200_release, which waits for the context's stream (unless that is being captured) and frees the handle only.  The context works on its
  * own stream: memory that another stream has written or will read is ordered by the two calls below. */
 int32_t b200_buf_import(b200_ctx* ctx, void* device_ptr, size_t bytes, b200_buf** out);
 /* Later work of the context starts after everything enqueued on `cuda_stream` (a cudaStream_t of the same device, NULL:
@@ -416,7 +416,7 @@ int32_t b200_paged_chunk_attention(b200_ctx* ctx, const b200_buf* q, size_t q_of
 
 typedef struct b200_sample_args {
     uint64_t rows;
-    uint64_t vocab;                /* 1 .. 393216 */
+    uint64_t vocab;                /* 1 .. 360448 */
     uint64_t row_stride;           /* elements from one row of logits to the next; 0: rows are dense */
     int32_t dtype;                 /* B200_F32 or B200_BF16 */
 } b200_sample_args;

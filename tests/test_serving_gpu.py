@@ -80,6 +80,40 @@ def test_append_matches_the_plain_form(be, case, adjacent, io_bf16):
         assert np.array_equal(down(vp, bt.v.shape, bt.pool_bf16), want_v.reshape(bt.v.shape))
 
 
+def test_append_without_rotation_needs_no_table(be):
+    bt = Batch([3, 2], [20, 2], heads=4, kv_heads=1, dh=64, seed=5)
+    qkv = np.random.default_rng(6).standard_normal((5, 6 * 64)).astype(np.float32)
+    tables, starts, lens = index_buffers(be, bt)
+    kp, vp = be.upload(bt.pool_array(bt.k)), be.upload(bt.pool_array(bt.v))
+    q, none = be.alloc_zeroed((5, 256)), be.alloc_zeroed((0,))
+    args = P.RopeAppendArgs(layout_of(bt), 2, 5, 4, 1, bt.width, 0, 0)
+    P.rope_paged_kv_append(be, be.upload(qkv), none, none, tables, starts, lens, kp, vp, args, q)
+    assert np.array_equal(q.numpy(), qkv[:, :256])
+
+
+def test_rows_before_the_first_sequence_are_left_alone(be):
+    """q_starts that begin above zero are outside the contract; the rows before them still are not touched."""
+    bt = Batch([3, 2], [20, 2], heads=4, kv_heads=1, dh=64, seed=5, pad_rows=4)
+    bt.q_starts = (bt.q_starts + 4).astype(np.uint32)
+    tables, starts, lens = index_buffers(be, bt)
+    kp, vp = be.upload(bt.pool_array(bt.k)), be.upload(bt.pool_array(bt.v))
+    qkv = be.upload(np.ones((9, 6 * 64), np.float32))
+    cos, sin = P.rope_table(10000.0, 64, 32)
+    q = be.upload(np.full((9, 256), 7.0, np.float32))
+    args = P.RopeAppendArgs(layout_of(bt), 2, 9, 4, 1, bt.width, 64, 32)
+    P.rope_paged_kv_append(be, qkv, be.upload(cos), be.upload(sin), tables, starts, lens, kp, vp, args, q)
+    assert (q.numpy()[:4] == 7.0).all() and (q.numpy()[4:] != 7.0).any()
+    for seqs in (1, 2):                    # one launch, and with the keys shared out and joined
+        long = Batch([3], [4000], heads=4, kv_heads=1, dh=64 * seqs, seed=5, pad_rows=4)
+        long.q_starts = (long.q_starts + 4).astype(np.uint32)
+        t2, s2, l2 = index_buffers(be, long)
+        out = be.upload(np.full((7, 4 * long.dh), 7.0, np.float32))
+        ca = P.PagedChunkArgs(layout_of(long), 1, 7, 3, 4000, 4, 1, long.width, 0.1)
+        ws = be.alloc_zeroed((max(16, P.paged_chunk_workspace(be, ca)),), np.uint8)
+        P.paged_chunk_attention(be, be.upload(long.q), be.upload(long.pool_array(long.k)), be.upload(long.pool_array(long.v)), t2, s2, l2, ca, ws, out)
+        assert (out.numpy()[:4] == 7.0).all() and (out.numpy()[4:] != 7.0).any()
+
+
 def test_append_with_positions_of_its_own(be):
     bt = Batch([3, 2], [20, 2], heads=4, kv_heads=1, dh=64, seed=5)
     qkv = np.random.default_rng(6).standard_normal((5, 6 * 64)).astype(np.float32)
@@ -385,6 +419,13 @@ def test_sampling_masked_rows_and_bad_parameters(be):
     x2[1, 69999] = 0.0
     check_draw(be, x2, k=35001, u=np.float32(0.9999))
     assert draw(be, x2, u=[0.5, 0.5], with_extras=False)[0].tolist()[1] == 69999
+
+
+def test_sampling_the_largest_vocabulary(be):
+    x = (np.random.default_rng(5).standard_normal((2, 360448)) * 2).astype(np.float32)
+    check_draw(be, x, 0.9, [0, 300], [0.9, 0.8], 0.0, seed=6)
+    with pytest.raises(BackendError):
+        draw(be, np.zeros((1, 360449), np.float32), u=[0.5])
 
 
 def test_sampling_does_not_depend_on_the_batch(be):
