@@ -18,7 +18,7 @@
 // usually a few hundred) move to a list in index order, and what follows works on that.  A bin that holds more than kCandidates tokens (flat or heavily tied rows) is
 // resolved by bisection over the ordered pair (logit, index) instead.
 //
-// Measured on a B200: one row of 128256 f32 logits 25 us, 128 such rows with every filter 106 us, 512 rows of 32000 bf16 logits 89 us.
+// Measured on a B200: one row of 128256 f32 logits 25 us, 128 such rows with every filter 106 us, 512 rows of 32000 bf16 logits 60 us.
 // Bound by latency, not by HBM (whose share is 10 us of the 106): a row takes about 37 thousand clocks, of which 5 load it, 9 go
 // into the bins and the f64 sum, 9 into cluster barriers and 4 each into leaving tokens behind and ranking the border's bin.
 #include <cfloat>
@@ -639,10 +639,10 @@ cudaError_t sample_tokens(const SampleShape& want, const void* logits, int bf16,
                           cudaStream_t s) {
     SampleShape p = want;
     if (p.rows == 0) return cudaSuccess;
-    // Blocks per row: enough that 16384 logits fit one block's share (so that two blocks share an SM), and for few rows as
-    // many as there are idle SMs as long as each keeps 4096 logits.
+    // Blocks per row: enough that 64 KB of logits are one block's share (so that two blocks share an SM; 512 rows of 32000 bf16 logits
+    // take 89 us with two blocks to a row), and for few rows as many as there are idle SMs as long as each keeps 4096 logits.
     int c = 1;
-    while (c < kMaxCluster && (p.vocab > int64_t(c) * 16384 || (p.rows * c * 2 <= sm_count && p.vocab >= c * 2 * 4096))) c *= 2;
+    while (c < kMaxCluster && (p.vocab > int64_t(c) * (bf16 ? 32768 : 16384) || (p.rows * c * 2 <= sm_count && p.vocab >= c * 2 * 4096))) c *= 2;
     p.cluster = c;
     p.per_cta = (((p.vocab + c - 1) / c) + 7) / 8 * 8;
     if (p.per_cta > kMaxPerCta) return cudaErrorInvalidValue;

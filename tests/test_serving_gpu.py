@@ -610,3 +610,13 @@ def test_decoder_sample_needs_a_step(be):
             dec.sample(0.5)
     finally:
         dec.close()
+
+
+@pytest.mark.parametrize("io_bf16", [False, True])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_attention_long_chunks_among_single_tokens(be, dh, io_bf16):
+    """Chunks, single tokens and sequences without new ones in one batch: items of every kind in one launch."""
+    check_attention(be, Batch([1, 200, 1, 0, 3, 1, 1, 1, 2, 1], [40, 330, 600, 5, 3, 1, 129, 300, 2, 17], heads=8, kv_heads=2, dh=dh, seed=17, pad_rows=2), io_bf16)
+    # and with the keys of a row shared out
+    check_attention(be, Batch([1, 40, 1, 1, 1, 1], [3000, 2100, 60, 900, 1, 5000], heads=4, kv_heads=1, dh=dh, seed=18), io_bf16)
+    check_attention(be, Batch([1] * 20 + [90], [33] * 20 + [90], heads=4, kv_heads=4, dh=dh, seed=19), io_bf16)
