@@ -378,8 +378,9 @@ cudaError_t launch_tc5_kind(const ChunkPlan& plan, const RaggedShape& sh, const 
     p.group = sh.num_q_heads / sh.num_kv_heads;
     p.chunk_tiles = plan.chunk_tiles;
     p.max_chunks = plan.max_chunks;
-    p.q_sign = sh.scale > 0.0f ? 1.0f : (sh.scale < 0.0f ? -1.0f : 0.0f);
-    p.scale_log2 = sh.scale == 0.0f ? 1.0f : fabsf(sh.scale) * 1.44269504088896341f;
+    p.q_sign = sh.scale < 0.0f ? -1.0f : 1.0f;
+    // scale 0: a factor so small that every finite score gives a weight of one, and a masked one (-inf) still none
+    p.scale_log2 = fmaxf(fabsf(sh.scale) * 1.44269504088896341f, 1.2e-38f);
     float* part_o = static_cast<float*>(workspace);
     float2* part_ml = reinterpret_cast<float2*>(part_o + (plan.max_chunks > 1 ? sh.rows * sh.num_q_heads * plan.max_chunks * D : 0));
     const dim3 grid(static_cast<unsigned>(plan.items));

@@ -70,7 +70,7 @@ struct TcShape {
     RaggedShape sh;
     int group, chunk_tiles, max_chunks;
     float scale_log2;          // > 0
-    float q_sign;              // queries are multiplied by this: -1 for a negative scale, 0 for scale 0
+    float q_sign;              // -1 for a negative scale: the queries are negated (f32: as they are split; bf16: by the MMA)
 };
 
 struct TcItem {
@@ -261,6 +261,11 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+// 16 bytes from global to shared memory without a register in between; zeros where `real` is false
+__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Asks the launch unit for a block of this grid that has not started: that block is cancelled and its work is the caller's.  The
@@ -468,6 +473,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         // ------------------------------------------------------------ MMA issue for slot `s` (one elected thread)
         constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((kTcKeys >> 3) << 17) | ((128 >> 4) << 24);
         constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((D >> 3) << 17) | ((128 >> 4) << 24);
+        const uint32_t idesc_s = kIdescS | (!F32 && p.q_sign < 0.0f ? 1u << 13 : 0u);      // bit 13: the A operand negated
         const int s = warp - 9;
         const uint32_t d_s = tmem + s * 128, d_o = tmem + 256 + s * 128;
         uint32_t pos = 0, p_phase = 0, k_item = 0;
@@ -505,7 +511,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                                     constexpr int kTerms = decltype(terms)::value;
                                     const int term = left;
                                     const uint32_t off = ((kk / 4) * kHalfBytes + (kk % 4) * 32) >> 4;
-                                    umma_bf16_ss(d_s, q_desc + off + ((term * Cfg::kQTileBytes) >> 4), k_desc + off, kIdescS, term < kTerms - 1 || kk > 0);
+                                    umma_bf16_ss(d_s, q_desc + off + ((term * Cfg::kQTileBytes) >> 4), k_desc + off, idesc_s, term < kTerms - 1 || kk > 0);
                                 }
                             tc5_commit(smem_u32(&sh.s_full[s]));
                             release(stage);
@@ -671,6 +677,19 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 const int piece = lane % kPieces;
                 unsigned char* dst = q_smem + (split ? 0 : wg) * Cfg::kQTileBytes + (piece / 8) * kHalfBytes;
 #pragma unroll 1
+                if constexpr (!F32) {      // straight into shared memory, all of it in flight at once
+#pragma unroll 1
+                    for (int j = lane / kPieces; j < per; j += kAtOnce) {
+                        const int64_t f = __shfl_sync(0xffffffffu, static_cast<long long>(from), j & 31);
+                        const int to = base + j;
+#pragma unroll
+                        for (int quarter = 0; quarter < (TINY ? 4 : 1); ++quarter) {
+                            const int tr = quarter * 32 + to;
+                            copy_async_16(smem_u32(dst + tr * 128 + (((piece % 8) ^ (tr & 7)) << 4)), q + f + piece * 8, j < count);
+                        }
+                    }
+                    copy_async_wait();
+                } else {
                 for (int j0 = lane / kPieces; j0 < per; j0 += kBatch * kAtOnce) {
                     using Raw = Pack<T, 8>;
                     Raw raw[kBatch];
@@ -714,6 +733,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                             }
                         }
                     }
+                }
                 }
                 fence_proxy_async();
                 tc5_fence_before();
