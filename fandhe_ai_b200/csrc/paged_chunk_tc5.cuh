@@ -1034,11 +1034,38 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 if constexpr (!F32 && !TINY) {
                     patch = *reinterpret_cast<volatile uint32_t*>(&item->nonfinite) != 0;      // set before the products that o_full stands for
                     const float inv = direct ? 1.0f / l : 1.0f;
-                    // 32 rows of 64 columns at a time in this warp's part of its group's query tile (D = 64: of 32 columns)
-                    constexpr int kCols = D / 2;
                     unsigned char* area = q_smem + wg * Cfg::kQTileBytes + (warp & 3) * (Cfg::kQTileBytes / 4);
+                    const bool plain = direct && !patch;
+                    if (plain && busy) {      // 32 finished bf16 rows fit this warp's part of its group's query tile
 #pragma unroll 1
-                    for (int part = 0; part < 2; ++part) {
+                        for (int g = 0; g < D / 32; ++g) {
+                            uint32_t raw[32];
+                            tmem_ld_32x32(t_o + g * 32, raw);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 32; k += 8) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    w[e] = pack_bf16(__uint_as_float(raw[k + 2 * e]) * inv, __uint_as_float(raw[k + 2 * e + 1]) * inv);
+                                *reinterpret_cast<uint4*>(area + lane * (D * 2) + (((g * 4 + k / 8) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                        __syncwarp();
+                        constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces;
+                        const int piece = lane % kPieces;
+#pragma unroll 4
+                        for (int j = lane / kPieces; j < 32; j += kAtOnce) {
+                            const int64_t to_row = row_of(j);
+                            const bool there = reach_of(j) > 0;
+                            const uint4 v = *reinterpret_cast<const uint4*>(area + j * (D * 2) + ((piece ^ (j & 7)) << 4));
+                            if (there) *reinterpret_cast<uint4*>(out + to_row * D + piece * 8) = v;
+                        }
+                    }
+                    // key ranges and patched rows: 32 rows of 64 f32 columns at a time (D = 64: of 32 columns)
+                    constexpr int kCols = D / 2;
+#pragma unroll 1
+                    for (int part = plain ? 2 : 0; part < 2; ++part) {
                         if (busy) {
 #pragma unroll 1
                             for (int g = 0; g < kCols / 32; ++g) {
