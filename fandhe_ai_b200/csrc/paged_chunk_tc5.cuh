@@ -38,12 +38,14 @@
 // masked keys (only the last ones of a sequence; such a tile is announced to warp 11, and by it to the MMA warps) rows beyond the item's last visible key are zeroed, non-finite elements
 // of rows that some query must not see are replaced by zero, and if there were any the epilogue adds them back to the rows that do see them.
 //
-// Measured on a B200 (us; 32 / 8 heads of 128 unless said otherwise): 2039 bf16 tokens over 30011 cached ones 1219, which is 850
-// TFLOP/s; four prompts of 2048 213 (645 TFLOP/s); one f32 token of each of 128 sequences over 256 to 2048 184 (3.2 TB/s); four chunks
-// of about 400 f32 tokens among 60 single ones 236; sixteen f32 prompts of 300 to 1024, 12 heads of 64, 158; four drafted bf16
-// tokens of eight sequences 21.  Bound by the chain of a slot (about 3800 clocks a tile where the products alone take 1024, two slots
-// side by side) and, for short items, by their start and finish; not by HBM and not by the tensor cores' rate.  Code that runs
-// once per item is not unrolled: the instruction cache shows (prompts 239 -> 213).
+// Measured on a B200 (us; 32 / 8 heads of 128 unless said otherwise): 2039 bf16 tokens over 30011 cached ones 1180 to 1225 (the
+// power cap decides), which is 846 to 878 TFLOP/s; four prompts of 2048 188 (731 TFLOP/s); one f32 token of each of 128 sequences
+// over 256 to 2048 184 (3.2 TB/s); four chunks of about 400 f32 tokens among 60 single ones 236; sixteen f32 prompts of 300 to
+// 1024, 12 heads of 64, 158; four drafted bf16 tokens of eight sequences 21.  Bound by the chain of a slot (about 3800 clocks a
+// tile where the products alone take 1024, two slots side by side) and, for short items, by their start and finish; not by HBM
+// and not by the tensor cores' rate.  What an item does once is kept short for that reason (prompts, step by step): code that runs once is not
+// unrolled, since the instruction cache shows (239 -> 213); bf16 queries go to shared memory by asynchronous copies (213 -> 196);
+// finished bf16 rows leave in one pass, staged as bf16 (196 -> 188).
 
 constexpr int kTcSoftmaxWarps = 8;
 constexpr int kTcThreads = 32 * (kTcSoftmaxWarps + 4);
@@ -668,7 +670,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             // Queries into shared memory, 128-byte swizzled.  A warp reads whole rows (a lane 8 elements of one), several before it
             // uses the first; a tile that both slots use is shared out over all eight warps.
             {
-                constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces, kBatch = F32 ? 2 : 4;
+                constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces, kBatch = 2;
                 const int per = stack || TINY ? 4 : (split ? 16 : 32), base = (split ? warp : warp & 3) * per;
                 const int first = (split ? 0 : wg * 128) + base, count = min(per, it.rows - first);      // rows of this warp (<= 0: none)
                 // place of the row base + lane; rows that the item does not have read its first row and are set to zero
@@ -676,7 +678,6 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 const int64_t from = (int64_t(it.start) + tok) * p.sh.row_stride + int64_t(it.kvh * p.group + at - tok * p.group) * D;
                 const int piece = lane % kPieces;
                 unsigned char* dst = q_smem + (split ? 0 : wg) * Cfg::kQTileBytes + (piece / 8) * kHalfBytes;
-#pragma unroll 1
                 if constexpr (!F32) {      // straight into shared memory, all of it in flight at once
 #pragma unroll 1
                     for (int j = lane / kPieces; j < per; j += kAtOnce) {
@@ -690,6 +691,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     }
                     copy_async_wait();
                 } else {
+#pragma unroll 1
                 for (int j0 = lane / kPieces; j0 < per; j0 += kBatch * kAtOnce) {
                     using Raw = Pack<T, 8>;
                     Raw raw[kBatch];
