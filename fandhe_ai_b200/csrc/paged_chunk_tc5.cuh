@@ -492,6 +492,10 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             tc5_fence_after();
             const uint64_t q_desc = umma_desc_k128(q_addr + (F32 || split ? 0 : s) * Cfg::kQTileBytes);
             const int step = split ? 2 : 1;
+            // No tile of this item for this slot: its group waits for o_full all the same, since a group that went on to the next item
+            // could complete its q_full again before this warp has seen the last one, and the parity wait above would never end.
+            if (ok && split && s >= n && elect_one()) mbar_arrive(smem_u32(&sh.o_full[s]));
+            __syncwarp();
             // a stage is free when both slots are done with it; a slot that has it for itself says so twice
             auto release = [&](uint32_t stage) {
                 tc5_commit(smem_u32(&sh.empty[stage]));
@@ -980,7 +984,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 l += a + b;
                 if (!ok) break;
             }
-            if (ok && done > 0) {
+            if (ok) {      // done == 0 too: its slot has then seen the queries' barriers, see there
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.o_full[wg]), o_phase & 1, err, kErrEpilogueWait));
                 ++o_phase;
                 tc5_fence_after();
