@@ -306,7 +306,9 @@ __device__ __forceinline__ F2 cut_rest(float lo, float hi) {
 }
 
 struct TcShared {
-    uint64_t full[8], empty[8], raw[8];        // raw: a V tile with masked keys has landed and is to be cleaned
+    // Two `full` barriers a stage, taken in turn: a slot that shares the key tiles waits for its own only, so it may ask for a stage
+    // while the other slot's tile before it has not landed - with one barrier, whose phase before that is complete, the wait would pass.
+    uint64_t full[2][8], empty[8], raw[8];     // raw: a V tile with masked keys has landed and is to be cleaned
     uint64_t s_full[2], p_full[2][2], p_free[2], o_full[2], q_full[2];
     uint32_t turn[4];                          // taken by one of the two softmax warps of a scheduler
     uint64_t meet_all, meet[2];                // the softmax warps meet: all of them, one group
@@ -338,7 +340,8 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kNst; ++i) {
-            mbar_init(smem_u32(&sh.full[i]), 1);
+            mbar_init(smem_u32(&sh.full[0][i]), 1);
+            mbar_init(smem_u32(&sh.full[1][i]), 1);
             mbar_init(smem_u32(&sh.empty[i]), 2);      // both slots, or one slot twice
             mbar_init(smem_u32(&sh.raw[i]), 1);
         }
@@ -377,6 +380,9 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     pdl_launch_dependents();
 
     const int block = p.sh.block_size;
+    // the barrier of the tile at place `at` of the ring, and the parity of its phase
+    auto full_bar = [&](uint32_t at) { return &sh.full[(at / kNst) & 1][at % kNst]; };
+    auto full_parity = [](uint32_t at) { return (at / (2 * kNst)) & 1; };
     // the k-th item, for every warp but the one that deals them out; null: no more (or the wait ran out)
     auto next_item = [&](uint32_t k) -> TcItem* {
         const uint32_t slot = k % kTcItemSlots;
@@ -434,7 +440,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 issued = at + 1;
                 const int boxes = (min(kTcKeys, end - k0) + box - 1) / box;
                 const bool masked = values && it.t0 + t >= masked_from;
-                const uint32_t bar = smem_u32(masked ? &sh.raw[stage] : &sh.full[stage]);
+                const uint32_t bar = smem_u32(masked ? &sh.raw[stage] : full_bar(at));
                 if (masked) { raw_last |= 1u << stage; raw_phase ^= 1u << stage; }
                 else raw_last &= ~(1u << stage);
                 if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box * D * 2);
@@ -469,7 +475,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             for (uint32_t at = issued > kNst ? issued - kNst : 0; at < issued; ++at) {
                 const uint32_t stage = at % kNst;
                 if ((raw_last >> stage) & 1) mbar_wait(smem_u32(&sh.raw[stage]), ((raw_phase >> stage) & 1) ^ 1, err, kErrProducerWait);
-                else mbar_wait(smem_u32(&sh.full[stage]), (at / kNst) & 1, err, kErrProducerWait);
+                else mbar_wait(smem_u32(full_bar(at)), full_parity(at), err, kErrProducerWait);
             }
     } else if (warp <= 10) {
         // ------------------------------------------------------------ MMA issue for slot `s` (one elected thread)
@@ -504,7 +510,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             for (int t = split ? s : 0; ok && t < n; t += step) {
                 {
                     const uint32_t at = order.k(t), stage = at % kNst;
-                    ok = wait(&sh.full[stage], (at / kNst) & 1);
+                    ok = wait(full_bar(at), full_parity(at));
                     if (!ok) break;
                     tc5_fence_after();
                     const uint64_t k_desc = umma_desc_k128(ring_addr + stage * Cfg::kTileBytes);
@@ -527,7 +533,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     multiply(std::integral_constant<int, TINY ? 1 : Cfg::kQTerms>());
                 }
                 const uint32_t at = order.v(t), stage = at % kNst;
-                ok = wait(&sh.full[stage], (at / kNst) & 1);
+                ok = wait(full_bar(at), full_parity(at));
                 const uint64_t v_desc = umma_desc_mn128(ring_addr + stage * Cfg::kTileBytes, kHalfBytes);
                 const uint32_t keep = t >= step;            // not the first product of this item
                 const bool last = t + step >= n;
@@ -613,7 +619,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 if (found) item->nonfinite = 1;
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.full[stage]));
+                if (lane == 0) mbar_arrive(smem_u32(full_bar(at)));
             }
         }
     }

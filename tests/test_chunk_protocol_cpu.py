@@ -49,7 +49,7 @@ class Order:
 
 
 class Model:
-    def __init__(self, items, stages, seed, full_barriers=1, idle_slot_answers=True, item_slots=4):
+    def __init__(self, items, stages, seed, full_barriers=2, idle_slot_answers=True, item_slots=4):
         self.items, self.stages, self.rng = items, stages, random.Random(seed)
         self.full_barriers, self.idle_slot_answers, self.slots = full_barriers, idle_slot_answers, item_slots
         self.full = [[Bar(f"full[{r}][{i}]") for i in range(stages)] for r in range(full_barriers)]
@@ -193,3 +193,16 @@ def test_the_model_sees_a_slot_that_nobody_waits_for(stages):
 @pytest.mark.parametrize("stages", [4, 5, 8])
 def test_a_slot_without_tiles_is_waited_for(stages):
     assert not [f for f in faults(stages) if "q_full" in f]
+
+
+# ring stages: heads of 128 with f32 / bf16 activations, heads of 64; f32 activations share every item between the slots
+@pytest.mark.parametrize("stages,split_only", [(4, True), (5, False), (5, True), (8, False), (8, True)])
+def test_no_wait_is_early_or_overtaken(stages, split_only):
+    for seed in range(200):
+        Model(batches(seed, split_only), stages, seed).run()
+
+
+def test_the_model_sees_a_stage_asked_for_before_the_tile_ahead_has_landed():
+    """With one `full` barrier a stage, a slot's wait passes while the other slot's tile before it is still on its way."""
+    found = faults(4, full_barriers=1) + faults(5, full_barriers=1)
+    assert found and all("full[0]" in f and "passes" in f for f in found)
