@@ -416,17 +416,19 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         // One block per item in the grid; a block that is through with its own takes over one that has not started, so the items
         // spread evenly whatever their lengths.
         int64_t index = blockIdx.x;
-        uint32_t asked = 0;
-        for (; ok; ++asked) {
-            if (asked > 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.stolen_bar), (asked - 1) & 1, err, kErrProducerWait));
+        uint32_t asked = 0, answered = 0;      // requests to the launch unit, and answers taken: at most one is on its way
+        while (ok) {
+            if (asked > answered) {
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.stolen_bar), answered & 1, err, kErrProducerWait));
                 if (!ok) break;
+                ++answered;
                 index = stolen_block(smem_u32(&sh.stolen));
                 if (index < 0) break;
                 fence_proxy_async();
                 __syncwarp();
             }
             if (lane == 0) steal_block(smem_u32(&sh.stolen), smem_u32(&sh.stolen_bar));
+            ++asked;
             if (!walk.get(index, it, err) || it.nt == 0) continue;
             ok = deal();
             if (!ok) break;
@@ -470,7 +472,8 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             it.nt = -1;
             deal();
         }
-        if (!ok) mbar_wait(smem_u32(&sh.stolen_bar), asked & 1, err, kErrProducerWait);
+        // given up: the answer on its way still lands in this block's shared memory
+        if (asked > answered) mbar_wait(smem_u32(&sh.stolen_bar), answered & 1, err, kErrProducerWait);
         if (!ok)      // the consumer is gone: let this warp's own copies land before the memory is given back
             for (uint32_t at = issued > kNst ? issued - kNst : 0; at < issued; ++at) {
                 const uint32_t stage = at % kNst;

@@ -206,3 +206,37 @@ def test_the_model_sees_a_stage_asked_for_before_the_tile_ahead_has_landed():
     """With one `full` barrier a stage, a slot's wait passes while the other slot's tile before it is still on its way."""
     found = faults(4, full_barriers=1) + faults(5, full_barriers=1)
     assert found and all("full[0]" in f and "passes" in f for f in found)
+
+
+def unwinding(fail_at, fail_where, items):
+    """The producer's requests for blocks that have not started, up to a wait that runs out (`fail_where` of round `fail_at`) or the
+    answer "none" after `items` blocks.  Returns (requests made, phases waited for in full, phase of the last wait or None)."""
+    asked = answered = 0
+    waited, ok, index = [], True, 0
+    while ok:
+        if asked > answered:
+            if (fail_at, fail_where) == (asked, "answer"):
+                ok = False
+                break
+            waited.append(answered)
+            answered += 1
+            index += 1
+            if index >= items:
+                break
+        asked += 1
+        if asked - 1 == fail_at and fail_where == "deal":
+            ok = False
+            break
+        if asked - 1 == fail_at and fail_where == "fetch":
+            ok = False
+    last = answered if asked > answered else None
+    return asked, waited, last
+
+
+@pytest.mark.parametrize("where", ["answer", "deal", "fetch", None])
+def test_a_block_that_gives_up_waits_for_the_answer_on_its_way(where):
+    """However the producer ends, every request's phase is waited for once and in order; only the answer "none" leaves nothing open."""
+    for fail_at in range(6):
+        asked, waited, last = unwinding(fail_at, where, 5)
+        assert waited + ([last] if last is not None else []) == list(range(asked))
+        assert (last is None) == (where is None or asked == 5 and len(waited) == 5)
