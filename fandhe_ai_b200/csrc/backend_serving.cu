@@ -111,6 +111,7 @@ int32_t append_args(const b200_rope_append_args* a, Ragged* r, uint64_t* row_wid
         return bad(op, "a row of q, k and v exceeds i32::MAX elements");
     if (int32_t st = check_ragged(op, &a->layout, a->batch, a->rows, a->qkv_stride, *row_width, a->num_heads, a->num_kv_heads, a->max_blocks_per_seq, a->io_dtype, r))
         return st;
+    r->sh.max_q_len = r->sh.max_seq_len = r->sh.max_blocks_per_seq * r->sh.block_size;
     if (a->rotary_dim % 2 != 0 || a->rotary_dim > dh) return bad(op, "rotary_dim must be even and at most head_dim");
     if (a->adjacent_pairs && (dh % 2 != 0 || r->sh.row_stride % 2 != 0)) return bad(op, "adjacent pairs need an even head_dim and an even row stride");
     if (a->n_positions > kI32Max) return bad(op, "n_positions exceeds i32::MAX");

@@ -68,7 +68,7 @@ struct RaggedShape {
     int64_t rows;            // token rows of the activations
     int64_t row_stride;      // elements from one activation row to the next
     int batch, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq;
-    int max_q_len, max_seq_len;      // attention: bounds of the new and the cached tokens of a sequence
+    int max_q_len, max_seq_len;      // bounds of the new and the cached tokens of a sequence (append: what a table row can hold)
     float scale;
 };
 struct RopeShape {

@@ -13,8 +13,20 @@
 namespace b200 {
 namespace {
 
+// What a sequence's entries [s, e) of q_starts and its length must satisfy; nothing is read or written for one that does not.
+__device__ __forceinline__ bool sequence_ok(const RaggedShape& sh, int64_t s, int64_t e, int64_t len) {
+    return e >= s && e <= sh.rows && e - s <= len && e - s <= sh.max_q_len && len <= sh.max_seq_len;
+}
+// The same for all sequences, by one warp of a launch: the kernels whose blocks look at single rows do not meet every entry.
+__device__ __forceinline__ void check_sequences(const RaggedShape& sh, const uint32_t* __restrict__ q_starts,
+                                                const uint32_t* __restrict__ seq_lens, uint32_t* err) {
+    for (int b = threadIdx.x & 31; b < sh.batch; b += 32)
+        if (!sequence_ok(sh, q_starts[b], q_starts[b + 1], seq_lens[b])) atomicCAS(err, 0u, static_cast<uint32_t>(kErrRaggedBatch));
+}
+
 // Index of the sequence that row `row` belongs to, by one pass of the whole block over q_starts (one load latency instead of the
 // log2(batch) dependent ones of a binary search): the number of starts[1..batch] that are <= row.  `batch` when it belongs to none.
+// Only a guess where the starts decrease: the caller asks whether the row stands in [starts[seq], starts[seq + 1]).
 __device__ __forceinline__ int sequence_of_row(const uint32_t* __restrict__ q_starts, int batch, int64_t row) {
     int seq = 0;
     for (int b0 = 0; b0 < batch; b0 += blockDim.x) {
@@ -99,6 +111,8 @@ rope_append_kernel(RaggedShape sh, RopeShape rope, int rows_per_block, const T* 
                    const uint32_t* __restrict__ q_starts, const uint32_t* __restrict__ seq_lens, T* __restrict__ q_out,
                    KvT* __restrict__ k_pool, KvT* __restrict__ v_pool, uint32_t* err) {
     __shared__ AppendRow place[kAppendRows];
+    // (the last warp: with one row to a block it has nothing else to do here)
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x + 32 >= blockDim.x) check_sequences(sh, q_starts, seq_lens, err);
     const int64_t row0 = int64_t(blockIdx.x) * rows_per_block;
     const int count = int(min(int64_t(rows_per_block), sh.rows - row0));
     const int64_t ekv = int64_t(sh.num_kv_heads) * sh.head_dim;
@@ -117,10 +131,11 @@ rope_append_kernel(RaggedShape sh, RopeShape rope, int rows_per_block, const T* 
         }
         if (lane == 0) {
             AppendRow to = {-1, 0};
-            if (seq < sh.batch && row >= int64_t(q_starts[seq])) {          // else behind the last sequence
-                const int64_t pos = int64_t(seq_lens[seq]) - (int64_t(q_starts[seq + 1]) - row);      // position in the cache
+            const int64_t from = seq < sh.batch ? int64_t(q_starts[seq]) : 0, upto = seq < sh.batch ? int64_t(q_starts[seq + 1]) : 0;
+            if (row >= from && row < upto) {                                // else behind the last sequence
+                const int64_t len = seq_lens[seq], pos = len - (upto - row);      // position in the cache
                 to.angle = positions ? int64_t(positions[row]) : pos;
-                if (pos < 0 || pos >= int64_t(sh.max_blocks_per_seq) * sh.block_size || (rope.rotary_dim > 0 && (to.angle < 0 || to.angle >= rope.n_positions))) {
+                if (!sequence_ok(sh, from, upto, len) || (rope.rotary_dim > 0 && (to.angle < 0 || to.angle >= rope.n_positions))) {
                     atomicCAS(err, 0u, static_cast<uint32_t>(kErrRaggedBatch));
                 } else {
                     const uint32_t blk = tables[int64_t(seq) * sh.max_blocks_per_seq + pos / sh.block_size];
@@ -248,15 +263,12 @@ paged_chunk_generic_kernel(RaggedShape sh, const T* __restrict__ q, const KvT* _
     const int64_t row = blockIdx.x;
     const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int seq = sequence_of_row(q_starts, sh.batch, row);
-    if (seq >= sh.batch || row < int64_t(q_starts[seq])) return;
+    if (row == 0 && h == 0 && warp == 0) check_sequences(sh, q_starts, seq_lens, err);
+    if (seq >= sh.batch) return;
+    const int64_t from = q_starts[seq], upto = q_starts[seq + 1], len = seq_lens[seq];
+    if (row < from || row >= upto) return;
     const int dh = sh.head_dim;
-    const int64_t len = seq_lens[seq], new_rows = int64_t(q_starts[seq + 1]) - int64_t(q_starts[seq]);
-    const int64_t cap = int64_t(sh.max_blocks_per_seq) * sh.block_size;
-    int64_t limit = len - (int64_t(q_starts[seq + 1]) - row) + 1;       // visible keys
-    if (len > cap || len > sh.max_seq_len || new_rows > len || new_rows > sh.max_q_len) {
-        if (threadIdx.x == 0) atomicCAS(err, 0u, static_cast<uint32_t>(kErrRaggedBatch));
-        limit = 0;
-    }
+    const int64_t limit = sequence_ok(sh, from, upto, len) ? len - (upto - row) + 1 : 0;       // visible keys
     const int kvh = h / (sh.num_q_heads / sh.num_kv_heads);
     const int64_t ekv = int64_t(sh.num_kv_heads) * dh;
     const T* q_row = q + row * sh.row_stride + int64_t(h) * dh;
@@ -357,7 +369,9 @@ ChunkPlan plan_chunk(const RaggedShape& sh, int io_bf16, int kv_bf16, int sm_cou
     plan.chunk_tiles = (tiles + best - 1) / best;
     plan.max_chunks = (tiles + plan.chunk_tiles - 1) / plan.chunk_tiles;
     plan.items = units * plan.max_chunks;
-    plan.tc5 = plan.items < 0x7FFFFFFF && int64_t(sh.max_q_len) * group < 0x7FFFFFFF;
+    // (32 sequences of any length within the bounds, whatever q_starts holds: a warp adds their items up in 32 bits)
+    const int64_t of_32 = 32 * ((int64_t(sh.max_q_len) * group + rows - 1) / rows) * sh.num_kv_heads * plan.max_chunks;
+    plan.tc5 = plan.items < 0x7FFFFFFF && of_32 < 0x7FFFFFFF && int64_t(sh.max_q_len) * group < 0x7FFFFFFF;
     return plan;
 }
 

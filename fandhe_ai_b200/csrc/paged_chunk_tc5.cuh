@@ -108,7 +108,7 @@ struct TcWalk {
         items = n = len = 0;
         if (b < p.sh.batch) {
             const int64_t s = q_starts[b], e = q_starts[b + 1], l = seq_lens[b];
-            if (e < s || e > p.sh.rows || e - s > l || e - s > p.sh.max_q_len || l > p.sh.max_seq_len) {
+            if (!sequence_ok(p.sh, s, e, l)) {
                 if (err) atomicCAS(err, 0u, static_cast<uint32_t>(kErrRaggedBatch));
             } else if (e > s) {
                 n = int(e - s);
@@ -1290,7 +1290,7 @@ paged_chunk_join_kernel(const __grid_constant__ TcShape p, int tile_rows, const 
     const int seq = sequence_of_row(q_starts, p.sh.batch, row);
     if (seq >= p.sh.batch) return;
     const int64_t s = q_starts[seq], e = q_starts[seq + 1], len = seq_lens[seq];
-    if (row < s || e > p.sh.rows || e - s > len || e - s > p.sh.max_q_len || len > p.sh.max_seq_len) return;      // reported by the first kernel
+    if (row < s || row >= e || !sequence_ok(p.sh, s, e, len)) return;      // reported by the first kernel
     const int n = int(e - s), token = int(row - s);
     const int chunks = ((int(len) + kTcKeys - 1) / kTcKeys + p.chunk_tiles - 1) / p.chunk_tiles;
     if (chunks == 1) return;                                                                            // written already

@@ -21,3 +21,80 @@ def test_attention_many_items_of_one_tile(be, dh, io_bf16):
     # one tile and several tiles in turn, more rows than the variant for few rows takes
     new = [12, 60, 12, 33] * 30
     check_attention(be, Batch(new, [n + [0, 200, 90, 600][i % 4] for i, n in enumerate(new)], heads=2, kv_heads=1, dh=dh, seed=33), io_bf16)
+
+
+# ------------------------------------------------------------------------------------------ device arrays that make no sense
+
+def reported(be):
+    with pytest.raises(BackendError) as e:
+        be.synchronize_device()
+    return e.value.message
+
+
+BAD_STARTS = [
+    dict(starts=[0, 100, 2, 3], lens=[100, 60, 40], rows=110, dh=64),        # the second sequence ends before it starts
+    dict(starts=[0, 100, 2, 3], lens=[100, 60, 40], rows=110, dh=80),
+    dict(starts=[0, 3, 1, 2], lens=[4000, 4000, 4000], rows=6, dh=128),      # the same with the keys of a row shared out and joined
+    dict(starts=[0, 3, 1, 2], lens=[4000, 4000, 4000], rows=6, dh=40),
+    dict(starts=[0, 4, 9], lens=[40, 40], rows=8, dh=64),                    # ends behind the last row
+    dict(starts=[0, 4, 9], lens=[40, 40], rows=8, dh=80),
+    dict(starts=[0, 4, 4, 8], lens=[40, 70, 40], rows=8, dh=64, max_len=64),  # too long, and without a new token
+    dict(starts=[0, 4, 4, 8], lens=[40, 70, 40], rows=8, dh=80, max_len=64),
+]
+
+
+@pytest.mark.parametrize("case", BAD_STARTS)
+def test_starts_that_make_no_sense_are_reported(case):
+    be = Backend(0)
+    try:
+        starts, lens, rows, dh = case["starts"], case["lens"], case["rows"], case["dh"]
+        bt = Batch([1] * len(lens), lens, heads=4, kv_heads=2, dh=dh, seed=40)
+        q = be.upload(np.random.default_rng(1).standard_normal((rows, 4 * dh)).astype(np.float32))
+        tables, st, sl = be.upload(bt.tables), be.upload(np.array(starts, np.uint32)), be.upload(bt.seq_lens)
+        kp, vp = be.upload(bt.pool_array(bt.k)), be.upload(bt.pool_array(bt.v))
+        layout = P.PagedKvLayout(bt.blocks, bt.block, 2 * dh, BF16)
+        most = case.get("max_len", max(lens))
+        args = P.PagedChunkArgs(layout, len(lens), rows, min(100, most), most, 4, 2, bt.width, 0.1)
+        need = P.paged_chunk_workspace(be, args)
+        ws = be.upload(np.zeros(max(16, need), np.uint8))
+        out = be.upload(np.full((rows, 4 * dh), 7.0, np.float32))
+        P.paged_chunk_attention(be, q, kp, vp, tables, st, sl, args, ws, out)
+        assert "0x205" in reported(be)
+    finally:
+        be.close()
+    be = Backend(0)
+    try:
+        qkv = be.upload(np.random.default_rng(2).standard_normal((rows, 8 * dh)).astype(np.float32))
+        tables, st, sl = be.upload(bt.tables), be.upload(np.array(starts, np.uint32)), be.upload(bt.seq_lens)
+        kp, vp = be.upload(bt.pool_array(bt.k)), be.upload(bt.pool_array(bt.v))
+        cos, sin = (be.upload(x) for x in P.rope_table(10000.0, dh, max(lens) + 1))
+        width = case["max_len"] // bt.block if "max_len" in case else bt.width
+        t2 = be.upload(np.ascontiguousarray(bt.tables[:, :width]))
+        args = P.RopeAppendArgs(layout, len(lens), rows, 4, 2, width, dh, max(lens) + 1)
+        P.rope_paged_kv_append(be, qkv, cos, sin, t2, st, sl, kp, vp, args, be.upload(np.zeros((rows, 4 * dh), np.float32)))
+        assert "0x205" in reported(be)
+    finally:
+        be.close()
+
+
+@pytest.mark.parametrize("dh", [64, 80, 128])
+def test_starts_that_make_no_sense_leave_the_rest_alone(dh):
+    """Memory of torch, which can be read after the error: rows of no sequence, guard rows and the workspace's guard keep what they held."""
+    torch = pytest.importorskip("torch")
+    be = Backend(0)
+    try:
+        lens, rows = [4000, 4000, 4000], 6
+        bt = Batch([1] * 3, lens, heads=4, kv_heads=2, dh=dh, seed=41)
+        layout = P.PagedKvLayout(bt.blocks, bt.block, 2 * dh, BF16)
+        args = P.PagedChunkArgs(layout, 3, rows, 100, 4000, 4, 2, bt.width, 0.1)
+        need = P.paged_chunk_workspace(be, args)
+        ws = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+        out = torch.full((rows + 8, 4 * dh), 7.0, device="cuda")
+        torch.cuda.synchronize()
+        up = lambda x: be.upload(np.ascontiguousarray(x))
+        P.paged_chunk_attention(be, up(bt.q[:1].repeat(rows, 0)), up(bt.pool_array(bt.k)), up(bt.pool_array(bt.v)), up(bt.tables),
+                                up(np.array([0, 3, 1, 2], np.uint32)), up(bt.seq_lens), args, be.import_tensor(ws), be.import_tensor(out))
+        assert "0x205" in reported(be)
+        assert bool((out[3:] == 7.0).all()) and bool((ws[need:] == 0x5A).all())
+    finally:
+        be.close()
