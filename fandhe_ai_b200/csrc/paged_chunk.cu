@@ -14,8 +14,9 @@ namespace b200 {
 namespace {
 
 // What a sequence's entries [s, e) of q_starts and its length must satisfy; nothing is read or written for one that does not.
-__device__ __forceinline__ bool sequence_ok(const RaggedShape& sh, int64_t s, int64_t e, int64_t len) {
-    return e >= s && e <= sh.rows && e - s <= len && e - s <= sh.max_q_len && len <= sh.max_seq_len;
+__device__ __forceinline__ bool sequence_ok(const RaggedShape& sh, uint32_t s, uint32_t e, uint32_t len) {
+    return e >= s && e <= static_cast<uint32_t>(sh.rows) && e - s <= len && e - s <= static_cast<uint32_t>(sh.max_q_len) &&
+           len <= static_cast<uint32_t>(sh.max_seq_len);
 }
 // The same for all sequences, by one warp of a launch: the kernels whose blocks look at single rows do not meet every entry.
 __device__ __forceinline__ void check_sequences(const RaggedShape& sh, const uint32_t* __restrict__ q_starts,
@@ -104,15 +105,14 @@ struct AppendRow {
 // rotate into each other (ADJ: one group holding N / 2 pairs) or a group that is copied; N elements are 16 bytes of the activation
 // type, or N = 1 (ADJ: 2) where an alignment or a size does not allow that.  Bound by HBM where rows are long: 8192 f32 rows of 24 KB in
 // 65.5 us (5.7 TB/s); 14k bf16 rows of 4.6 KB in 41 us (3.6 TB/s); 128 rows in 5.8 us, the launch.
+// Eight blocks fit an SM with 32 registers, which the adjacent form has to be told (it chose 31 and took 42.9 us instead of 41.0).
 template <typename T, typename KvT, int N, bool ADJ>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, ADJ ? 8 : 0)
 rope_append_kernel(RaggedShape sh, RopeShape rope, int rows_per_block, const T* __restrict__ qkv, const float* __restrict__ cos_t,
                    const float* __restrict__ sin_t, const uint32_t* __restrict__ positions, const uint32_t* __restrict__ tables,
                    const uint32_t* __restrict__ q_starts, const uint32_t* __restrict__ seq_lens, T* __restrict__ q_out,
                    KvT* __restrict__ k_pool, KvT* __restrict__ v_pool, uint32_t* err) {
     __shared__ AppendRow place[kAppendRows];
-    // (the last warp: with one row to a block it has nothing else to do here)
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x + 32 >= blockDim.x) check_sequences(sh, q_starts, seq_lens, err);
     const int64_t row0 = int64_t(blockIdx.x) * rows_per_block;
     const int count = int(min(int64_t(rows_per_block), sh.rows - row0));
     const int64_t ekv = int64_t(sh.num_kv_heads) * sh.head_dim;
@@ -131,21 +131,25 @@ rope_append_kernel(RaggedShape sh, RopeShape rope, int rows_per_block, const T* 
         }
         if (lane == 0) {
             AppendRow to = {-1, 0};
-            const int64_t from = seq < sh.batch ? int64_t(q_starts[seq]) : 0, upto = seq < sh.batch ? int64_t(q_starts[seq + 1]) : 0;
-            if (row >= from && row < upto) {                                // else behind the last sequence
-                const int64_t len = seq_lens[seq], pos = len - (upto - row);      // position in the cache
-                to.angle = positions ? int64_t(positions[row]) : pos;
-                if (!sequence_ok(sh, from, upto, len) || (rope.rotary_dim > 0 && (to.angle < 0 || to.angle >= rope.n_positions))) {
+            seq = min(seq, sh.batch - 1);
+            const uint32_t from = q_starts[seq], upto = q_starts[seq + 1], len = seq_lens[seq], r = static_cast<uint32_t>(row);
+            if (r >= from && r < upto) {                                    // else behind the last sequence
+                const uint32_t pos = len - (upto - r);                      // position in the cache
+                const uint32_t angle = positions ? positions[row] : pos;
+                to.angle = angle;
+                if (!sequence_ok(sh, from, upto, len) || (rope.rotary_dim > 0 && angle >= static_cast<uint32_t>(rope.n_positions))) {
                     atomicCAS(err, 0u, static_cast<uint32_t>(kErrRaggedBatch));
                 } else {
-                    const uint32_t blk = tables[int64_t(seq) * sh.max_blocks_per_seq + pos / sh.block_size];
+                    const uint32_t blk = tables[int64_t(seq) * sh.max_blocks_per_seq + pos / static_cast<uint32_t>(sh.block_size)];
                     if (blk >= uint32_t(sh.num_blocks)) atomicCAS(err, 0u, static_cast<uint32_t>(kErrAppendSlot));
-                    else to.slot = (int64_t(blk) * sh.block_size + pos % sh.block_size) * ekv;
+                    else to.slot = (int64_t(blk) * sh.block_size + pos % static_cast<uint32_t>(sh.block_size)) * ekv;
                 }
             }
             place[i] = to;
         }
     }
+    // (the last warp: with one row to a block it has nothing else to do here)
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x + 32 >= blockDim.x) check_sequences(sh, q_starts, seq_lens, err);
     __syncthreads();
     const int d = sh.head_dim, half = rope.rotary_dim / 2;
     const int turned = ADJ ? rope.rotary_dim / N : half / N;            // units of a head that rotate
