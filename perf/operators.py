@@ -294,7 +294,12 @@ def _plain_sample(st):
 
 def run(state):
     if own:
-        return _own(state)
+        # the framework works on its context's stream, the tensors belong to torch's: in order on the device, without the host waiting
+        stream = torch.cuda.current_stream().cuda_stream
+        _backend.wait_stream(stream)
+        out = _own(state)
+        _backend.stream_wait(stream)
+        return out
     return {"append": _plain_append, "attention": _plain_attention, "sample": _plain_sample}[state["case"]["op"]](state)
 
 
