@@ -5,6 +5,8 @@ import pytest
 from fandhe_ai_b200 import BF16, F32, Backend, BackendError
 from fandhe_ai_b200 import paged_kv as P
 
+from fandhe_ai_b200.decoder import SampleArgs, sample_tokens
+
 from serving_ref import Batch, bf16
 from test_serving_gpu import check_attention
 
@@ -98,3 +100,96 @@ def test_starts_that_make_no_sense_leave_the_rest_alone(dh):
         assert bool((out[3:] == 7.0).all()) and bool((ws[need:] == 0x5A).all())
     finally:
         be.close()
+
+
+# ------------------------------------------------------------------------------------------ streams
+
+def test_stream_order_both_ways_again_and_again(be):
+    """Two streams of another library in turn, each ordered against the context's: every call sees the values that its own stream wrote
+    last, although all calls share the context's event."""
+    torch = pytest.importorskip("torch")
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    x, ids, u = [torch.zeros(4, 5000, device="cuda") for _ in streams], [torch.zeros(4, dtype=torch.int32, device="cuda") for _ in streams], torch.zeros(4, device="cuda")
+    big = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    hx, hid, hu = [be.import_tensor(t) for t in x], [be.import_tensor(t) for t in ids], be.import_tensor(u)
+    got = []
+    for i in range(40):
+        j = i % 2
+        with torch.cuda.stream(streams[j]):
+            if i % 8 == j:
+                _ = big @ big
+            x[j].fill_(-1.0)
+            x[j][:, 37 * i + j] = 5.0
+            be.wait_stream(streams[j].cuda_stream)
+            sample_tokens(be, hx[j], SampleArgs(4, 5000), hu, hid[j], top_k=None, temperature=hu)       # temperature 0: the maximum
+            be.stream_wait(streams[j].cuda_stream)
+            got.append(ids[j].clone())
+            x[j].zero_()
+    torch.cuda.synchronize()
+    assert [g.tolist() for g in got] == [[37 * i + i % 2] * 4 for i in range(40)]
+
+
+def test_stream_order_inside_a_captured_graph(be):
+    """A stream of another library is captured; the context joins the capture for one call and hands over again."""
+    torch = pytest.importorskip("torch")
+    x, ids, u = torch.zeros(4, 5000, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(4, device="cuda")
+    at = torch.zeros(4, 1, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    hx, hid, hu = be.import_tensor(x), be.import_tensor(ids), be.import_tensor(u)
+    side = torch.cuda.Stream()
+
+    def step():
+        x.fill_(-1.0)
+        x.scatter_(1, at, 5.0)
+        be.wait_stream(torch.cuda.current_stream().cuda_stream)
+        sample_tokens(be, hx, SampleArgs(4, 5000), hu, hid, temperature=hu)
+        be.stream_wait(torch.cuda.current_stream().cuda_stream)
+        return ids * 2
+
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="relaxed"):
+        twice = step()
+    for i in (3, 4999, 0, 77):
+        at.fill_(i)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert twice.tolist() == [2 * i] * 4
+    be.wait_stream(side.cuda_stream)             # and outside a capture again
+    sample_tokens(be, hx, SampleArgs(4, 5000), hu, hid, temperature=hu)
+    assert hid.numpy().tolist() == [77] * 4
+    del graph
+def test_measured_calls_are_ordered_with_the_callers_stream(be):
+    """perf/operators.py hands out tensors of torch: its calls wait for what the current stream has still to write, and work that
+    the caller puts behind them sees finished results - without a wait of the host in between."""
+    torch = pytest.importorskip("torch")
+    import importlib.util
+    from pathlib import Path
+
+    spec = importlib.util.spec_from_file_location("measured_cases", Path(__file__).resolve().parents[1] / "perf" / "operators.py")
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    m.own = True
+    case = dict(op="attention", dtype="bf16", seqs=2, chunked=2, chunk_lo=900, chunk_hi=1000, step=1, prefix_lo=0, prefix_hi=0, lens=1,
+                heads=8, kv_heads=8, head_dim=128, block=16)
+    st = m.prepare(case, 5)
+    torch.cuda.synchronize()
+    want = m.run(st)["out"].clone()
+    torch.cuda.synchronize()
+    big, q = torch.randn(8192, 8192, device="cuda"), st["q"].clone()
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        st["q"].zero_()
+        st["out"].zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for _ in range(4):
+                big = big @ big * 1e-4                       # some milliseconds before the queries are there
+            st["q"].copy_(q)
+            got = m.run(st)["out"].clone()
+            st["q"].zero_()                                  # and gone again as soon as the call's place in the stream is past
+        stream.synchronize()
+        assert torch.equal(got, want)
