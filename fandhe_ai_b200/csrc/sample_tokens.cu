@@ -10,6 +10,7 @@
 // Arithmetic.  A token stands next to a border of these sums in every row (neighbours in a flat row of 128k tokens are 1e-5 of
 // the sum apart), so weights are computed in f64 and held as integers, w * 2^shift rounded (vocab * 2^shift <= 2^62, so
 // no sum of a row overflows): integer sums do not depend on their order, whatever the cluster size or the scheduling.
+// A weight below 2^-(shift + 1) is zero in the sums; min_p is compared with the f64 weight.
 //
 // One cluster of C thread blocks owns a row and keeps it in its shared memory, so that the logits are read from HBM once
 // however many passes the filters take.  Selection needs no sort: tokens fall into 2048 bins of (max - x) / T (a monotone
@@ -142,6 +143,10 @@ struct Row {
     __device__ __forceinline__ uint64_t weight(float x, int b) const {
         const double w = scaled_weight(b >= dead_bin ? max_x : x, shift) + 4503599627370496.0;      // 2^52: rounds, and the mantissa is the integer
         return b >= dead_bin ? 0 : static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
+    }
+    // min_p asks for the weight itself: rounded, it would be zero or a small whole number there.  Beyond 2^-150 no f32 reaches.
+    __device__ __forceinline__ bool reaches(float x, double least) const {
+        return (max_x - x) * bin_scale < 4800.0f && scaled_weight(x, 0) >= least;
     }
 };
 
@@ -584,13 +589,12 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
 
     // ---- the draw: sums of the kept weights in index order
     uint64_t s[2] = {0, 0}, sum[2];
-    const double floor_w = double(mp) * unit;
     auto kept_weight = [&](int i, uint64_t* w) -> bool {
         const float x = X(i);
         const int b = r.bin(x);
         if (b > cut.bin || b == kBins || (b == cut.bin && !cut.keeps(b, x, index(i)))) return false;
         *w = r.weight(x, b);
-        return double(*w) >= floor_w || index(i) == best_i;
+        return !(mp > 0.0f) || index(i) == best_i || r.reaches(x, double(mp));
     };
     for (int i = lo; i < hi; ++i) {
         uint64_t w;

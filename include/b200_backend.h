@@ -429,7 +429,9 @@ int32_t b200_validate_sample(const b200_sample_args* args);
  * logit and equal logits by rising index (the order of top_k_indices, crates/autodiff/src/generate/mod.rs:359-369): the
  * first top_k of them are kept; of those the shortest prefix whose weight reaches top_p of theirs; of those the ones
  * with w_i >= min_p; the first token always.  Drawn is the smallest kept index at which the running sum of the kept weights,
- * in index order, exceeds uniform * their sum.  Weights are computed in f64 and summed exactly.  A logit of -inf is a masked token and
+ * in index order, exceeds uniform * their sum.  Weights are computed in f64, which min_p is compared with; top_p and the draw add
+ * them up as multiples of 2^-s of the largest, s = 62 - max(12, ceil(log2(vocab))) (50 for 4096 tokens, 45 for 128256), so that a sum
+ * does not depend on its order.  A logit of -inf is a masked token and
  * never kept.  ids i32 [rows]; prob f32 [rows] (may be NULL): the drawn token's share of the kept weight; kept i32 [rows]
  * (may be NULL): how many tokens were kept.  A row that offers nothing to draw from answers id -1, prob 0, kept 0: all
  * logits -inf, a NaN or +inf among them, a temperature that is negative or not finite, a NaN parameter, or uniform outside

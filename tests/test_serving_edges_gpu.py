@@ -7,8 +7,8 @@ from fandhe_ai_b200 import paged_kv as P
 
 from fandhe_ai_b200.decoder import SampleArgs, sample_tokens
 
-from serving_ref import Batch, bf16
-from test_serving_gpu import check_attention
+from serving_ref import Batch, bf16, sample_ref
+from test_serving_gpu import check_attention, draw
 
 pytestmark = pytest.mark.gpu
 
@@ -193,3 +193,30 @@ def test_measured_calls_are_ordered_with_the_callers_stream(be):
             st["q"].zero_()                                  # and gone again as soon as the call's place in the stream is past
         stream.synchronize()
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------ sampling
+
+@pytest.mark.parametrize("min_p", [1e-3, 1e-6, 1e-10, 1e-14, 1e-18, 1e-30])
+@pytest.mark.parametrize("vocab", [50, 5000, 128256])
+def test_sampling_min_p_is_compared_with_the_weight_itself(be, vocab, min_p):
+    """Tokens one step of f32 apart around the border, far below the resolution of the sums."""
+    m = np.float32(min_p)
+    rows = 3
+    x = np.full((rows, vocab), -np.inf, np.float32)
+    border = np.float32(np.log(float(m)))
+    near = [border]
+    for _ in range(4):
+        near = [np.nextafter(near[0], np.float32(-np.inf)), *near, np.nextafter(near[-1], np.float32(0))]
+    at = np.random.default_rng(vocab).permutation(vocab)[:len(near) + 2]
+    for r in range(rows):
+        x[r, at[:-2]] = near
+        x[r, at[-2]] = 0.0
+        x[r, at[-1]] = border * 2                                   # far below the border
+    # f64 exponentials differ by 2^-50; a step of f32 at the border is at least 2^-23 of the logit, and the weight moves as much
+    assert np.abs(np.exp(np.float64(near)) / float(m) - 1).min() > 1e-9
+    want = sample_ref(x[0], 1.0, 0, 1.0, float(m), 0.0)
+    for kw in (dict(), dict(k=vocab), dict(k=len(at) + 1)):
+        ids, prob, kept = draw(be, x, m=m, u=[0.0, 0.3, 0.9999999], **kw)
+        assert kept.tolist() == [want[2]] * 3 and want[2] not in (1, len(at))
+        assert ids[0] == want[0] and ids[1:].tolist() == [sample_ref(x[0], 1.0, 0, 1.0, float(m), u)[0] for u in (float(np.float32(0.3)), float(np.float32(0.9999999)))]
