@@ -111,6 +111,7 @@ template <>
 __device__ __forceinline__ float logit_f32<uint16_t>(uint16_t v) { return bf16_bits_to_f32(v); }
 
 static_assert(sizeof(Shared) + 16 + kMaxPerCta * 4 <= 232448, "a thread block's shared memory");
+static_assert((kMaxPerCta + kThreads - 1) / kThreads < 128, "a thread's run, in two words of bits");
 
 struct Row {
     float max_x, bin_scale;
@@ -442,17 +443,17 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
     if (cut_k) last_bin = bk;
     else if (tp < 1.0f) last_bin = limited ? kBins - 1 : min(bp + 2, kBins - 1);      // (fewer tokens than top_k: their sum is still to come)
     else if (mp > 0.0f) last_bin = min(static_cast<int>(-32.0f * log2f(fminf(mp, 1.0f))) + 2, kBins - 1);
-    if (last_bin < kBins - 1 && run <= 64) {
+    if (last_bin < kBins - 1) {
         // a logit below this is in a later bin for certain (the bins themselves are asked for again below)
         const float least = r.max_x - (float(last_bin + 1) / r.bin_scale * 1.00001f + fabsf(r.max_x) * 1e-6f);
-        uint64_t mine = 0;
+        uint64_t mine = 0, more = 0;      // of this thread's first 64 elements, and of the others
         for (int i0 = lo; i0 < lo + run; i0 += 8) {
             uint32_t some = 0;
 #pragma unroll
             for (int q = 0; q < 8; ++q) some |= (i0 + q < hi && logit_f32<T>(xs[i0 + q]) >= least ? 1u : 0u) << q;
-            mine |= uint64_t(some) << (i0 - lo);
+            (i0 - lo < 64 ? mine : more) |= uint64_t(some) << ((i0 - lo) & 63);
         }
-        const int count = __popcll(mine);
+        const int count = __popcll(mine) + __popcll(more);
         int upto = count;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -468,12 +469,16 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
         }
         __syncthreads();
         if (total <= kSurvivors) {
-            while (mine) {
-                const int j = __ffsll(static_cast<long long>(mine)) - 1;
-                mine &= mine - 1;
-                sh.list_x[at] = logit_f32<T>(xs[lo + j]);
-                sh.list_i[at++] = uint16_t(lo + j);
-            }
+            auto put = [&](uint64_t bits, int from) {
+                while (bits) {
+                    const int j = from + __ffsll(static_cast<long long>(bits)) - 1;
+                    bits &= bits - 1;
+                    sh.list_x[at] = logit_f32<T>(xs[j]);
+                    sh.list_i[at++] = uint16_t(j);
+                }
+            };
+            put(mine, lo);
+            put(more, lo + 64);
             __syncthreads();
             listed = true;
             const int per = (total + kThreads - 1) / kThreads;

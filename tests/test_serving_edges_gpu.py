@@ -8,7 +8,7 @@ from fandhe_ai_b200 import paged_kv as P
 from fandhe_ai_b200.decoder import SampleArgs, sample_tokens
 
 from serving_ref import Batch, bf16, sample_ref
-from test_serving_gpu import check_attention, draw
+from test_serving_gpu import check_attention, check_draw, draw
 
 pytestmark = pytest.mark.gpu
 
@@ -220,3 +220,17 @@ def test_sampling_min_p_is_compared_with_the_weight_itself(be, vocab, min_p):
         ids, prob, kept = draw(be, x, m=m, u=[0.0, 0.3, 0.9999999], **kw)
         assert kept.tolist() == [want[2]] * 3 and want[2] not in (1, len(at))
         assert ids[0] == want[0] and ids[1:].tolist() == [sample_ref(x[0], 1.0, 0, 1.0, float(m), u)[0] for u in (float(np.float32(0.3)), float(np.float32(0.9999999)))]
+
+
+@pytest.mark.parametrize("vocab,as_bf16", [(32767, True), (32768, True), (65536, True), (131072, True), (262144, True), (262144, False)])
+def test_sampling_vocabularies_that_are_powers_of_two(be, vocab, as_bf16):
+    """The longest runs of logits a thread has to go through, 65 of them, and the borders of the survivors among them."""
+    rng = np.random.default_rng(vocab)
+    rows = 6
+    x = (rng.standard_normal((rows, vocab)) * 2.5).astype(np.float32)
+    x[0, [0, 63, 64, 65, vocab // 2, vocab - 1]] = 12.0               # first, last and the borders of a run
+    x[1, 64::65] += 4.0                                               # the last element of every run
+    x[2] = -np.inf
+    x[2, vocab - 70:] = np.linspace(-3, 3, 70)
+    check_draw(be, x, [1.0, 0.8, 1.0, 0.7, 1.0, 1.1], [0, 200, 0, 50, 1000, 0], [0.9, 0.95, 0.9, 1.0, 0.7, 0.99],
+               [0.0, 0.0, 0.05, 0.0, 0.02, 0.01], seed=vocab + 3, as_bf16=as_bf16)
