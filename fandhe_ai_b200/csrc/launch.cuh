@@ -4,6 +4,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <mutex>
+
 namespace b200 {
 
 // Process-wide switch for programmatic dependent launch (set from the environment variable
@@ -15,16 +17,20 @@ int current_sm_count();
 
 // Raises a kernel's dynamic shared-memory limit to `bytes` on the current device.  Function attributes belong to
 // the device, so the largest value already set is remembered per device ordinal in `cache` (64 entries, zero
-// initialised, one array per kernel instantiation).
+// initialised, one array per kernel instantiation).  Only ever raised, by one thread at a time: of two threads that set different
+// sizes at once the later could otherwise lower what the other remembers.
 template <typename K>
 cudaError_t ensure_dynamic_smem(K kernel, int bytes, int* cache) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (__atomic_load_n(&cache[dev], __ATOMIC_ACQUIRE) >= bytes) return cudaSuccess;
+    static std::mutex lock;
+    std::lock_guard<std::mutex> guard(lock);
     if (cache[dev] >= bytes) return cudaSuccess;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) cache[dev] = bytes;
+    if (e == cudaSuccess) __atomic_store_n(&cache[dev], bytes, __ATOMIC_RELEASE);
     return e;
 }
 

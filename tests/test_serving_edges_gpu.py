@@ -234,3 +234,41 @@ def test_sampling_vocabularies_that_are_powers_of_two(be, vocab, as_bf16):
     x[2, vocab - 70:] = np.linspace(-3, 3, 70)
     check_draw(be, x, [1.0, 0.8, 1.0, 0.7, 1.0, 1.1], [0, 200, 0, 50, 1000, 0], [0.9, 0.95, 0.9, 1.0, 0.7, 0.99],
                [0.0, 0.0, 0.05, 0.0, 0.02, 0.01], seed=vocab + 3, as_bf16=as_bf16)
+
+
+def test_threads_that_use_kernels_for_the_first_time_at_once():
+    """Contexts of their own, vocabularies in a different order each: a smaller one must not take the shared memory of a larger one
+    away.  In a process of its own, whose kernels nobody has used yet."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import sys, threading
+import numpy as np
+from fandhe_ai_b200 import Backend
+from fandhe_ai_b200.decoder import SampleArgs, sample_tokens
+sizes = [360448, 20, 128256, 300000, 4097, 50000, 200000, 1000]
+start, failed = threading.Barrier(4), []
+def work(k):
+    be = Backend(0)
+    bufs = [(be.upload(np.eye(1, v, v // 2, dtype=np.float32) * 50), v) for v in sizes[2 * k:] + sizes[:2 * k]]
+    u, ids = be.upload(np.zeros(1, np.float32)), be.alloc_zeroed((1,), np.int32)
+    be.synchronize_device()
+    start.wait()
+    try:
+        for _ in range(30):
+            for x, v in bufs:
+                sample_tokens(be, x, SampleArgs(1, v), u, ids)
+        for x, v in bufs:
+            sample_tokens(be, x, SampleArgs(1, v), u, ids, temperature=u)
+            assert ids.numpy()[0] == v // 2
+    except Exception as e:
+        failed.append((k, v, e))
+    be.close()
+threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+[t.start() for t in threads]; [t.join() for t in threads]
+assert not failed, failed
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0, r.stderr[-2000:]
