@@ -299,7 +299,7 @@ paged_chunk_generic_kernel(RaggedShape sh, const T* __restrict__ q, const KvT* _
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         s *= sh.scale;
-        const float m_new = fmaxf(m, s);
+        const float m_new = m > s || m != m ? m : s;      // NaN stays
         const float base = m_new == -INFINITY ? 0.0f : m_new;
         const float corr = expf(m - base), p = expf(s - base);
         l = fmaf(l, corr, p);
@@ -322,8 +322,9 @@ paged_chunk_generic_kernel(RaggedShape sh, const T* __restrict__ q, const KvT* _
         for (int d = threadIdx.x; d < dh; d += kGenThreads) o_row[d] = from_f32<T>(__int_as_float(0x7FC00000));
         return;
     }
-    const float mm = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
-    float w[4], ll = 0.0f;
+    float w[4], ll = 0.0f, mm = red_m[0];
+#pragma unroll
+    for (int t = 1; t < 4; ++t) mm = mm > red_m[t] || mm != mm ? mm : red_m[t];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         w[t] = red_m[t] == -INFINITY ? 0.0f : expf(red_m[t] - mm);
@@ -333,6 +334,15 @@ paged_chunk_generic_kernel(RaggedShape sh, const T* __restrict__ q, const KvT* _
         float o = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) o = fmaf(red_o[t][d], w[t], o);
+        if (o != o && ll > 0.0f && ll < INFINITY) {      // infinities that met weights of zero, or NaN: the values themselves
+            float extra = 0.0f;
+            for (int64_t j = 0; j < limit; ++j) {
+                const int64_t blk = tables[int64_t(seq) * sh.max_blocks_per_seq + j / sh.block_size];
+                const float v = as_f32(v_pool[(blk * sh.block_size + j % sh.block_size) * ekv + int64_t(kvh) * dh + d]);
+                if (!(fabsf(v) < INFINITY)) extra += v;
+            }
+            if (extra != 0.0f) o = extra;
+        }
         o_row[d] = from_f32<T>(limit > 0 ? o / ll : 0.0f);
     }
 }

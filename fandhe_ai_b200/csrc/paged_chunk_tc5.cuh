@@ -36,7 +36,8 @@
 // chain scores -> softmax -> values of a slot free of the other slot's waits; 11 cleans V: an MMA multiplies what it must not
 // see by zero, which does not remove NaN and infinities.  In tiles with
 // masked keys (only the last ones of a sequence; such a tile is announced to warp 11, and by it to the MMA warps) rows beyond the item's last visible key are zeroed, non-finite elements
-// of rows that some query must not see are replaced by zero, and if there were any the epilogue adds them back to the rows that do see them.
+// of rows that some query must not see are replaced by zero, and if there were any the epilogue adds them back to the rows that do see them
+// (as it does where a visible infinity met a weight of zero in some term or quarter).
 //
 // Measured on a B200 (us; 32 / 8 heads of 128 unless said otherwise): 2039 bf16 tokens over 30011 cached ones 1180 to 1225 (the
 // power cap decides), which is 846 to 878 TFLOP/s; four prompts of 2048 188 (731 TFLOP/s); one f32 token of each of 128 sequences
@@ -194,6 +195,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {       // NaN if one
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
     float y;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+__device__ __forceinline__ uint32_t max_nan_bf16(uint32_t a, uint32_t b) {      // of two bf16 each; 0x7FFF where one is NaN
+    uint32_t y;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
     return y;
 }
 // Two f32 operations in one instruction
@@ -1004,25 +1010,41 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             // row r of a staging area of W-element rows keeps its 16-byte piece j at piece j ^ (r & 7).
             const bool direct = it.nchunks == 1;
             bool patch = false;
-            // finishes N columns of the row with this place and reach: non-finite values that the MMAs did not get, where the row sees them
-            auto finish = [&](int64_t to_row, int reach, int col, auto& o) {
+            // A row's reach (visible keys) as the warps hand it round: negative where the sum of its weights is no positive number, so that
+            // its results mean what they are.
+            int reach = limit;
+            auto weigh = [&](float sum) { reach = sum > 0.0f && sum < INFINITY ? limit : -limit; };
+            // Finishes N columns of the row with this place and reach.  Infinities and NaN of V that the row sees: the MMAs did not get
+            // those of cleaned tiles, and made NaN of the others where they met weights of zero (the terms of a weight, the keys of the
+            // other warps, a sum scaled down to nothing).  The definition has the values themselves, so such a column is put together again.
+            auto finish = [&](int64_t to_row, int seen, int col, auto& o) {
                 constexpr int N = sizeof(o) / sizeof(float);
-                if (patch) {
-                    const int from = max(it.min_limit, k0), to = min(reach, k0 + nt * kTcKeys);
-                    for (int j = from; j < to; ++j) {
+                bool look = patch;
+#pragma unroll
+                for (int k = 0; k < N; ++k) look |= o[k] != o[k];
+                if (look && seen > 0) {
+                    float extra[N];
+#pragma unroll
+                    for (int k = 0; k < N; ++k) extra[k] = 0.0f;
+                    const int to = min(seen, k0 + nt * kTcKeys);
+#pragma unroll 1
+                    for (int j = k0; j < to; ++j) {
                         const uint32_t blk = tables[int64_t(it.seq) * p.sh.max_blocks_per_seq + j / block];
                         if (blk >= uint32_t(p.sh.num_blocks)) continue;
                         const uint16_t* v = v_pool + (int64_t(blk) * block + j % block) * (int64_t(p.sh.num_kv_heads) * D) + it.kvh * D + col;
 #pragma unroll
                         for (int k = 0; k < N; ++k)
-                            if ((v[k] & 0x7F80u) == 0x7F80u) o[k] += bf16_bits_to_f32(v[k]);
+                            if ((v[k] & 0x7F80u) == 0x7F80u) extra[k] += bf16_bits_to_f32(v[k]);
                     }
+#pragma unroll
+                    for (int k = 0; k < N; ++k)
+                        if (extra[k] != 0.0f) o[k] = (o[k] != o[k] ? 0.0f : o[k]) + extra[k];
                 }
                 if (direct) store_f32<T, N>(out + to_row * D + col, o);
                 else store_f32<float, N>(part_o + (to_row * p.max_chunks + it.chunk) * D + col, o);
             };
             auto row_of = [&](int j) { return static_cast<int64_t>(__shfl_sync(0xffffffffu, static_cast<long long>(out_row), j)); };
-            auto reach_of = [&](int j) { return __shfl_sync(0xffffffffu, limit, j); };
+            auto reach_of = [&](int j) { return __shfl_sync(0xffffffffu, reach, j); };
             // The rows [j, j + 32 / kLanes, ...) of a warp's 32, kLanes lanes of N columns to a row: all in flight together.  `get`
             // reads the staged columns of a row.
             auto write_rows = [&](auto lanes, auto columns, int col0, auto get) {
@@ -1036,9 +1058,9 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     for (int b = 0; b < kBatch; ++b) get(j0 + b * kAtOnce + lane / kLanes, col, o[b]);
 #pragma unroll
                     for (int b = 0; b < kBatch; ++b) {
-                        const int j = j0 + b * kAtOnce + lane / kLanes, reach = reach_of(j);
+                        const int j = j0 + b * kAtOnce + lane / kLanes, seen = reach_of(j);
                         const int64_t to_row = row_of(j);
-                        if (reach > 0) finish(to_row, reach, col0 + col, o[b]);
+                        if (seen != 0) finish(to_row, seen, col0 + col, o[b]);
                     }
                 }
             };
@@ -1049,9 +1071,11 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 if constexpr (!F32 && !TINY) {
                     patch = *reinterpret_cast<volatile uint32_t*>(&item->nonfinite) != 0;      // set before the products that o_full stands for
                     const float inv = direct ? 1.0f / l : 1.0f;
+                    weigh(l);
                     unsigned char* area = q_smem + wg * Cfg::kQTileBytes + (warp & 3) * (Cfg::kQTileBytes / 4);
-                    const bool plain = direct && !patch;
+                    bool plain = direct && !patch;
                     if (plain && busy) {      // 32 finished bf16 rows fit this warp's part of its group's query tile
+                        uint32_t nan = 0;
 #pragma unroll 1
                         for (int g = 0; g < D / 32; ++g) {
                             uint32_t raw[32];
@@ -1061,22 +1085,27 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                             for (int k = 0; k < 32; k += 8) {
                                 uint32_t w[4];
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
+                                for (int e = 0; e < 4; ++e) {
                                     w[e] = pack_bf16(__uint_as_float(raw[k + 2 * e]) * inv, __uint_as_float(raw[k + 2 * e + 1]) * inv);
+                                    nan = max_nan_bf16(nan, w[e]);
+                                }
                                 *reinterpret_cast<uint4*>(area + lane * (D * 2) + (((g * 4 + k / 8) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                             }
                         }
                         __syncwarp();
+                        // a NaN that the weights did not make (the largest of the bf16 that came by): the rows go the other way
+                        plain = !__any_sync(0xffffffffu, reach > 0 && ((nan & 0xFFFFu) == 0x7FFFu || nan >> 16 == 0x7FFFu));
                         constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces;
                         const int piece = lane % kPieces;
 #pragma unroll 4
-                        for (int j = lane / kPieces; j < 32; j += kAtOnce) {
+                        for (int j = lane / kPieces; plain && j < 32; j += kAtOnce) {
                             const int64_t to_row = row_of(j);
-                            const bool there = reach_of(j) > 0;
+                            const bool there = reach_of(j) != 0;
                             const uint4 v = *reinterpret_cast<const uint4*>(area + j * (D * 2) + ((piece ^ (j & 7)) << 4));
                             if (there) *reinterpret_cast<uint4*>(out + to_row * D + piece * 8) = v;
                         }
                     }
+                    __syncwarp();
                     // key ranges and patched rows: 32 rows of 64 f32 columns at a time (D = 64: of 32 columns)
                     constexpr int kCols = D / 2;
 #pragma unroll 1
@@ -1172,20 +1201,21 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     if (!ok) break;
 #pragma unroll
                     for (int j = 0; j < kMost; ++j) {
-                        const int rr = warp + j * 8, reach = reach_of(min(rr, kTiny - 1));
+                        const int rr = warp + j * 8, seen = abs(reach_of(min(rr, kTiny - 1)));
                         const int64_t to_row = row_of(min(rr, kTiny - 1));
                         if (rr >= it.rows) continue;
                         if (lane == 0 && !direct) part_ml[to_row * p.max_chunks + it.chunk] = make_float2(top[j] * c, total[j]);
                         const float inv = direct ? 1.0f / total[j] : 1.0f;
 #pragma unroll
                         for (int k = 0; k < 4; ++k) o[j][k] *= inv;
-                        if (col < D) finish(to_row, reach, col, o[j]);
+                        if (col < D) finish(to_row, total[j] > 0.0f && total[j] < INFINITY ? seen : -seen, col, o[j]);
                     }
                 } else {
                 const float m0 = sh.xm[0][lane_row], m1 = sh.xm[1][lane_row], mt = fmaxf(m0, m1);
                 const float f0 = m0 == -INFINITY ? 0.0f : ex2((m0 - mt) * c), f1 = m1 == -INFINITY ? 0.0f : ex2((m1 - mt) * c);
                 const float lt = fmaf(sh.xl[0][lane_row], f0, sh.xl[1][lane_row] * f1);
                 const float inv = direct ? 1.0f / lt : 1.0f;
+                weigh(lt);
                 const float mine = (wg == 0 ? f0 : f1) * inv;
                 if (!direct && live && warp == (stack ? 0 : warp & 3)) part_ml[out_row * p.max_chunks + it.chunk] = make_float2(mt * c, lt);
                 if (stack) {
@@ -1209,16 +1239,16 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;
 #pragma unroll
                     for (int j = 0; j < 4; j += kAtOnce) {
-                        const int rr = warp * 4 + j + lane / kLanes, col = lane % kLanes * 4, reach = reach_of(rr);
+                        const int rr = warp * 4 + j + lane / kLanes, col = lane % kLanes * 4, seen = reach_of(rr);
                         const int64_t to_row = row_of(rr);
-                        if (reach == 0) continue;
+                        if (seen == 0) continue;
                         float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                         for (int x = 5; x >= 0; --x) {      // the small terms first
                             const float4 v = *staged(q_smem, D, (x & 1) * 96 + (x >> 1) * 32 + rr, col);
                             o[0] += v.x; o[1] += v.y; o[2] += v.z; o[3] += v.w;
                         }
-                        finish(to_row, reach, col, o);
+                        finish(to_row, seen, col, o);
                     }
                 } else {
                     // group g finishes the columns [g D/2, (g + 1) D/2): the other group's half through shared memory, scaled
@@ -1316,7 +1346,7 @@ paged_chunk_join_kernel(const __grid_constant__ TcShape p, int tile_rows, const 
             float o[V];
             load_f32<float, V>(part_o + (base + i) * D + lane * V, o);
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] = fmaf(o[k], w, acc[k]);
+            for (int k = 0; k < V; ++k) acc[k] = fmaf(o[k], fabsf(o[k]) == INFINITY ? 1.0f : w, acc[k]);      // (a weight of zero would make it NaN)
         }
         const float inv = 1.0f / l;
 #pragma unroll

@@ -7,8 +7,8 @@ from fandhe_ai_b200 import paged_kv as P
 
 from fandhe_ai_b200.decoder import SampleArgs, sample_tokens
 
-from serving_ref import Batch, bf16, sample_ref
-from test_serving_gpu import check_attention, check_draw, draw
+from serving_ref import Batch, attention_ref, bf16, sample_ref
+from test_serving_gpu import check_attention, check_draw, draw, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -272,3 +272,74 @@ assert not failed, failed
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# ------------------------------------------------------------------------------------------ infinities and NaN that a token sees
+
+# the forms of the attention: few rows, at most 32 rows, 128 rows, 256 rows, keys shared out and joined, the general kernel
+FORMS = [
+    dict(new=[1, 2], total=[300, 140]),
+    dict(new=[1, 1], total=[300, 40], dh=64),
+    dict(new=[8], total=[300]),
+    dict(new=[16], total=[300], dh=64, heads=4, kv_heads=2),
+    dict(new=[32], total=[500]),
+    dict(new=[60], total=[400], dh=64),
+    dict(new=[80, 70], total=[500, 310], heads=8, kv_heads=2),
+    dict(new=[3], total=[6000], heads=4, kv_heads=1),
+    dict(new=[40], total=[4000], heads=4, kv_heads=1),
+    dict(new=[90], total=[3000], heads=8, kv_heads=2, dh=64),
+    dict(new=[5, 1], total=[200, 3], dh=80),
+    dict(new=[5, 1], total=[200, 3], pool_bf16=False),
+]
+
+
+def check_non_finite(be, bt, io_bf16, scale, places):
+    """`places`: (key, element, value) of KV head 0 of sequence 0.  Where one token sees them, the element is their sum; the others do
+    not notice."""
+    blk, off = bt.places(0)
+    clean = bt.v.copy()
+    for key, e, value in places:
+        bt.v[blk[key], off[key], e] = value
+    q = bf16(bt.q) if io_bf16 else bt.q
+    got = run_attention(be, bt, q, io_bf16, scale)
+    bt.v, dirty = clean, bt.v
+    ref, bound = attention_ref(bt, q, scale, split_terms=not io_bf16)
+    g, first = bt.heads // bt.kv_heads, bt.total[0] - bt.new[0]
+    step = 2.0 ** -8 if io_bf16 else 2.0 ** -24
+    want = ref.copy()
+    for i in range(bt.new[0]):
+        for key, e, value in places:
+            if key <= first + i:
+                for h in range(g):
+                    at = h * bt.dh + e
+                    want[i, at] = value + (want[i, at] if not np.isfinite(want[i, at]) else 0.0)
+    touched = ~np.isfinite(want)
+    assert touched.any() and (np.abs(got - ref) <= bound + step * 1.001 * (np.abs(ref) + bound))[~touched].all()
+    assert np.array_equal(got[touched], want[touched].astype(np.float32), equal_nan=True)
+
+
+@pytest.mark.parametrize("io_bf16", [False, True])
+@pytest.mark.parametrize("case", FORMS)
+def test_attention_infinities_that_every_token_sees(be, case, io_bf16):
+    inf, dh = np.inf, case.get("dh", 128)
+    for key in (0, 2, 37, 130, 200):
+        if key < case["total"][0] - case["new"][0]:
+            check_non_finite(be, Batch(seed=50, **case), io_bf16, dh ** -0.5, [(key, 3, inf), (key, 40, -inf), (key, 41, np.nan), (0, dh - 1, inf)])
+    key = min(150, case["total"][0] - case["new"][0] - 1)
+    check_non_finite(be, Batch(seed=51, **case), io_bf16, dh ** -0.5, [(0, 7, inf), (key, 7, inf), (1, 8, inf), (key, 8, -inf)])
+    # weights that vanish next to the largest, and a key that a later maximum scales down
+    check_non_finite(be, Batch(seed=52, q_scale=30.0, **case), io_bf16, dh ** -0.5, [(0, 7, inf), (key, 9, -inf), (key // 2, 10, inf)])
+
+
+@pytest.mark.parametrize("io_bf16", [False, True])
+@pytest.mark.parametrize("case", FORMS)
+def test_attention_nan_of_a_key_reaches_every_token_that_sees_it(be, case, io_bf16):
+    for key in (0, case["total"][0] - 1):
+        bt = Batch(seed=53, **case)
+        blk, off = bt.places(0)
+        bt.k[blk[key], off[key], 5] = np.nan
+        got = run_attention(be, bt, bf16(bt.q) if io_bf16 else bt.q, io_bf16, 0.1)
+        first, g = bt.total[0] - bt.new[0], bt.heads // bt.kv_heads
+        sees = np.zeros(got.shape, bool)
+        sees[max(0, key - first):bt.new[0], :g * bt.dh] = True
+        assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all()
