@@ -413,7 +413,7 @@ cudaError_t launch_tc5_kind(const ChunkPlan& plan, const RaggedShape& sh, const 
     float2* part_ml = reinterpret_cast<float2*>(part_o + (plan.max_chunks > 1 ? sh.rows * sh.num_q_heads * plan.max_chunks * D : 0));
     const dim3 grid(static_cast<unsigned>(plan.items));
     cudaError_t e = launch_ex(paged_chunk_tc5_kernel<D, F32, TINY, T>, grid, dim3(kTcThreads), Cfg::kSmem, s, 1, true, map_k, map_v, p,
-                              static_cast<const T*>(q), static_cast<const uint16_t*>(v_pool), tables, q_starts, seq_lens,
+                              static_cast<const T*>(q), static_cast<const uint16_t*>(k_pool), static_cast<const uint16_t*>(v_pool), tables, q_starts, seq_lens,
                               static_cast<T*>(out), part_o, part_ml, err);
     if (e != cudaSuccess || plan.max_chunks == 1) return e;
     const dim3 join(static_cast<unsigned>(sh.rows), (sh.num_q_heads + 7) / 8);

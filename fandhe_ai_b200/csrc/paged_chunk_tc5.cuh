@@ -254,6 +254,14 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
         "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ uint32_t tmem_ld_32x1(uint32_t taddr) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
+    return r;
+}
+__device__ __forceinline__ void tmem_st_32x1(uint32_t taddr, uint32_t r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory");
+}
 __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -330,7 +338,7 @@ static_assert(sizeof(TcShared) <= kTcBookBytes, "");
 template <int D, bool F32, bool TINY, typename T>
 __global__ void __launch_bounds__(kTcThreads, 1)
 paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcShape p,
-                       const T* __restrict__ q, const uint16_t* __restrict__ v_pool, const uint32_t* __restrict__ tables,
+                       const T* __restrict__ q, const uint16_t* __restrict__ k_pool, const uint16_t* __restrict__ v_pool, const uint32_t* __restrict__ tables,
                        const uint32_t* __restrict__ q_starts, const uint32_t* __restrict__ seq_lens, T* __restrict__ out,
                        float* __restrict__ part_o, float2* __restrict__ part_ml, uint32_t* err) {
     using Cfg = TcCfg<D, F32>;
@@ -827,7 +835,25 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
                         for (int k = 8; k < 32; k += 8) mx[g] = max_nan(mx[g], __uint_as_float(raw[k + g]), __uint_as_float(raw[k + g + 4]));
                     }
-                    raise(max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])));
+                    float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
+                    if constexpr (F32) {
+                        // Infinities of K or q: the small terms of a query make NaN of them (0 inf, inf - inf), the first term alone does not
+                        if (__any_sync(0xffffffffu, live && top != top)) {
+                            tmem_ld_32x32(t_s + key0, raw);
+                            tmem_ld_wait();
+                            top = -INFINITY;
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) {
+                                const float v = __uint_as_float(raw[k]);
+                                const float a = __shfl_sync(0xffffffffu, v, r), b = __shfl_sync(0xffffffffu, v, r + 10), d = __shfl_sync(0xffffffffu, v, r + 20);
+                                float x = (d + b) + a;
+                                x = masked && key0 + k >= visible ? -INFINITY : (x != x ? a : x);
+                                top = max_nan(top, x);
+                                raw[k] = __float_as_uint(x);
+                            }
+                        }
+                    }
+                    raise(top);
                     const float mc = m == -INFINITY ? 0.0f : (m == INFINITY ? __int_as_float(0x7FC00000) : m * c);
                     const F2 c2(c, c), mc2(-mc, -mc);
                     const int term = F32 ? lane / kTiny : 0;
@@ -940,6 +966,27 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         top = max_nan(top, max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])));
                     }
                     tmem_st_wait();
+                    // The same for the other items, whose terms are added up by the MMA: such scores are computed again
+                    if (__any_sync(0xffffffffu, live && top != top)) {
+                        top = -INFINITY;
+#pragma unroll 1
+                        for (int k = 0; k < kTcKeys; ++k) {
+                            float x = __uint_as_float(tmem_ld_32x1(t_s + k));
+                            tmem_ld_wait();
+                            if (live && x != x) {
+                                const int key = k0 + t * kTcKeys + k;
+                                const uint32_t blk = min(tables[int64_t(it.seq) * p.sh.max_blocks_per_seq + key / block], uint32_t(p.sh.num_blocks - 1));
+                                const uint16_t* kr = k_pool + (int64_t(blk) * block + key % block) * (int64_t(p.sh.num_kv_heads) * D) + it.kvh * D;
+                                const T* qr = q + (int64_t(it.start) + token) * p.sh.row_stride + int64_t(head) * D;
+                                x = 0.0f;
+#pragma unroll 1
+                                for (int d = 0; d < D; ++d) x = fmaf(as_f32(qr[d]) * p.q_sign, bf16_bits_to_f32(kr[d]), x);
+                            }
+                            tmem_st_32x1(t_s + k, __float_as_uint(x));
+                            top = max_nan(top, x);
+                        }
+                        tmem_st_wait();
+                    }
                     raise(top);
                     const float mc = m == -INFINITY ? 0.0f : (m == INFINITY ? __int_as_float(0x7FC00000) : m * c);      // a score of +inf: NaN, as inf - inf is
                     const F2 c2(c, c), mc2(-mc, -mc);

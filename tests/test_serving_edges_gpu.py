@@ -343,3 +343,41 @@ def test_attention_nan_of_a_key_reaches_every_token_that_sees_it(be, case, io_bf
         sees = np.zeros(got.shape, bool)
         sees[max(0, key - first):bt.new[0], :g * bt.dh] = True
         assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all()
+
+
+@pytest.mark.parametrize("io_bf16", [False, True])
+@pytest.mark.parametrize("case", FORMS)
+def test_attention_infinities_of_a_key(be, case, io_bf16):
+    """A score of -inf has no weight; one of +inf leaves no number (inf - inf)."""
+    for key, value, scale in ((0, np.inf, 0.1), (2, -np.inf, 0.1), (min(150, case["total"][0] - case["new"][0] - 1), np.inf, -0.1)):
+        bt = Batch(seed=54, **case)
+        blk, off = bt.places(0)
+        q = bf16(bt.q) if io_bf16 else bt.q
+        n, t, dh, g = bt.new[0], bt.total[0], bt.dh, bt.heads // bt.kv_heads
+        ref, bound = attention_ref(bt, q, scale, split_terms=not io_bf16)
+        ks = bt.k[blk, off].astype(np.float64).reshape(t, bt.kv_heads, dh)[:, 0]
+        vs = bt.v[blk, off].astype(np.float64).reshape(t, bt.kv_heads, dh)[:, 0]
+        bt.k[blk[key], off[key], 6] = value
+        got = run_attention(be, bt, q, io_bf16, scale)
+        step = 2.0 ** -8 if io_bf16 else 2.0 ** -24
+        numbers = 0
+        for i in range(n):
+            keep = np.array([j for j in range(t - n + i + 1) if j != key])
+            for h in range(g):
+                sl = slice(h * dh, (h + 1) * dh)
+                if q[i, h * dh + 6] * value * scale > 0:
+                    assert np.isnan(got[i, sl]).all()
+                    continue
+                s = ks[keep] @ q[i, sl].astype(np.float64) * scale
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                ds = (dh + 8) * 2.0 ** -23 * abs(scale) * (np.abs(ks[keep]) @ np.abs(q[i, sl].astype(np.float64))).max()
+                rel = np.expm1(2 * ds + 2.0 ** -21) + (2.0 ** -8 if io_bf16 else 2.0 ** -16) + 2 * len(keep) * 2.0 ** -23
+                lim = 2 * rel * (p @ np.abs(vs[keep]))
+                want = p @ vs[keep]
+                assert (np.abs(got[i, sl] - want) <= lim + step * 1.001 * (np.abs(want) + lim)).all()
+                numbers += 1
+        rest = np.ones(got.shape, bool)
+        rest[:n, :g * dh] = False
+        assert (np.abs(got - ref) <= bound + step * 1.001 * (np.abs(ref) + bound))[rest].all()
+        assert numbers > 0 or n * g < 4
