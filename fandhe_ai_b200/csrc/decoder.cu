@@ -1785,6 +1785,7 @@ int32_t b200_decoder_sample(b200_decoder* d, const float* temperature, const int
     if (d->cfg.vocab > sample_tokens_max_vocab()) return fail(B200_UNSUPPORTED, "decoder_sample: vocabulary too large for the sampling kernel");
     const int M = d->batch;
     for (int b = 0; b < M; ++b) {
+        if (!d->active_host[b]) continue;      // sat the last step out
         const std::string row = "decoder_sample: row " + std::to_string(b) + ": ";
         if (temperature && !(temperature[b] >= 0.0f && std::isfinite(temperature[b]))) return fail(B200_INVALID_ARGUMENT, row + "temperature must be finite and not negative");
         if (!(uniform[b] >= 0.0f && uniform[b] < 1.0f)) return fail(B200_INVALID_ARGUMENT, row + "uniform must be in [0, 1)");
@@ -1803,6 +1804,7 @@ int32_t b200_decoder_sample(b200_decoder* d, const float* temperature, const int
     SampleShape sh = {};
     sh.rows = M;
     sh.row_stride = sh.vocab = d->cfg.vocab;
+    sh.active = d->active_dev;
     CU_TRY(sample_tokens(sh, d->logits, 0, param(0), reinterpret_cast<const int*>(param(1)), param(2), param(3), param(4), d->next_ids_dev, nullptr,
                          nullptr, d->ctx->sm_count, s));
     if (next_ids_host) {
@@ -1813,7 +1815,7 @@ int32_t b200_decoder_sample(b200_decoder* d, const float* temperature, const int
         }
         std::memcpy(next_ids_host, d->next_pinned, size_t(M) * sizeof(int));
         for (int b = 0; b < M; ++b)
-            if (next_ids_host[b] < 0) return fail(B200_INVALID_ARGUMENT, "decoder_sample: row " + std::to_string(b) + " holds a NaN or infinite logit");
+            if (d->active_host[b] && next_ids_host[b] < 0) return fail(B200_INVALID_ARGUMENT, "decoder_sample: row " + std::to_string(b) + " holds a NaN or infinite logit");
     }
     return B200_OK;
 }

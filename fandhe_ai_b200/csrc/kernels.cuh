@@ -90,6 +90,7 @@ cudaError_t paged_chunk_attention(const RaggedShape& sh, const void* q, int io_b
 struct SampleShape {
     int64_t rows, row_stride;
     int vocab;
+    const uint32_t* active;                // device [rows] or null; a row with 0 is left out: nothing of it is read or written
     int cluster, per_cta, run, shift;      // set by the launcher
 };
 cudaError_t sample_tokens(const SampleShape& shape, const void* logits, int bf16, const float* temperature, const int* top_k,

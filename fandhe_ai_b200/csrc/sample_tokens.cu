@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleShape p, 
     T* xs = reinterpret_cast<T*>(smem_raw + (sizeof(Shared) + 15) / 16 * 16);      // in their own type
     const uint32_t nranks = p.cluster, rank = nranks > 1 ? cluster_ctarank() : 0;
     const int64_t row = blockIdx.x / nranks;
+    if (p.active && p.active[row] == 0) return;      // the whole cluster, before its first barrier
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t first = int64_t(rank) * p.per_cta;
     const int64_t left = int64_t(p.vocab) - first;

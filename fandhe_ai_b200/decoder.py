@@ -245,7 +245,8 @@ class Decoder:
 
     def sample(self, uniform, temperature=None, top_k=None, top_p=None, min_p=None, want_ids: bool = True):
         """Draws the next ids from the last step's logits on the device (scalars or one value per row; None: off) from the
-        given uniform numbers; `step()` without ids feeds them.  Returns them, or None with want_ids False."""
+        given uniform numbers; `step()` without ids feeds them.  Rows that sat the last step out are left out.  Returns the
+        ids, or None with want_ids False."""
         def rows(v, dtype):
             return None if v is None else np.ascontiguousarray(np.broadcast_to(np.asarray(v, dtype), (self._batch,)))
         a = [rows(v, t) for v, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32), (uniform, np.float32))]

@@ -617,7 +617,8 @@ int32_t b200_decoder_sampling_weights(b200_decoder* dec, int32_t strategy, int32
                                       uint64_t capacity_elems);
 /* The draw itself on the device, from given random numbers: b200_sample_tokens on the logits of the last step, whose ids replace
  * the greedy ones (a following b200_decoder_step with ids NULL feeds them).  Host arrays of one value per row of the running
- * generation; all but `uniform` may be NULL (off).  next_ids_host != NULL: the drawn ids are copied back (this synchronises; a
+ * generation; all but `uniform` may be NULL (off).  Rows that sat the last step out (b200_decoder_step_rows) are left out: their
+ * values are not looked at and their ids stay what that step left, which means nothing.  next_ids_host != NULL: the drawn ids are copied back (this synchronises; a
  * row whose logits are not finite is InvalidArgument, as in sample_step).  Without it nothing leaves the device; such a row
  * then fails the next step's check of its ids.  No logits and no weights cross to the host, unlike
  * b200_decoder_sampling_weights, which serves the reference's own generator. */

@@ -8,7 +8,7 @@ from fandhe_ai_b200 import paged_kv as P
 from fandhe_ai_b200.decoder import SampleArgs, sample_tokens
 
 from serving_ref import Batch, attention_ref, bf16, sample_ref
-from test_serving_gpu import check_attention, check_draw, draw, run_attention
+from test_serving_gpu import check_attention, check_draw, draw, make_small_decoder, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -381,3 +381,39 @@ def test_attention_infinities_of_a_key(be, case, io_bf16):
         rest[:n, :g * dh] = False
         assert (np.abs(got - ref) <= bound + step * 1.001 * (np.abs(ref) + bound))[rest].all()
         assert numbers > 0 or n * g < 4
+
+
+# ------------------------------------------------------------------------------------------ the decoder's own draw
+
+def step_rows(dec, ids, active):
+    a, nxt = np.array(active, np.uint8), np.empty(len(active), np.int32)
+    c = np.ascontiguousarray(ids, np.int32) if ids is not None else None
+    P.check(P.lib().b200_decoder_step_rows(dec._h, c.ctypes.data if c is not None else None, a.ctypes.data, nxt.ctypes.data))
+    return nxt
+
+
+def test_decoder_draws_for_the_rows_that_took_part(be):
+    """A row that sat the step out needs no valid parameters and keeps its id; the others draw as ever."""
+    dec = make_small_decoder(be, 3)
+    try:
+        dec.begin(3, [12] * 3)
+        dec.step(np.array([3, 77, 400], np.int32))
+        nan = float("nan")
+        for active, uniform, temperature, top_p in (([1, 0, 1], [0.3, nan, 0.7], [1.0, -1.0, 1.3], [0.9, nan, 1.0]),
+                                                    ([0, 1, 0], [2.0, 0.9, -1.0], [nan, 0.8, nan], [nan, 0.5, nan])):
+            left = step_rows(dec, [5, 6, 7], active)
+            logits = dec.logits()
+            got = dec.sample(uniform, temperature, top_p=top_p)
+            for r in range(3):
+                want = left[r]
+                if active[r]:
+                    want = sample_ref(logits[r], float(np.float32(temperature[r])), 0, float(np.float32(top_p[r])), 0.0, float(np.float32(uniform[r])))[0]
+                assert got[r] == want
+        with pytest.raises(BackendError):
+            dec.sample([0.1, nan, 0.1])                       # the row that takes part
+        step_rows(dec, None, [1, 1, 1])
+        with pytest.raises(BackendError):
+            dec.sample([0.1, 0.1, nan])
+        assert (dec.sample([0.1, 0.1, 0.1]) >= 0).all()
+    finally:
+        dec.close()
