@@ -1786,10 +1786,11 @@ int32_t b200_decoder_sample(b200_decoder* d, const float* temperature, const int
     const int M = d->batch;
     for (int b = 0; b < M; ++b) {
         if (!d->active_host[b]) continue;      // sat the last step out
-        const std::string row = "decoder_sample: row " + std::to_string(b) + ": ";
-        if (temperature && !(temperature[b] >= 0.0f && std::isfinite(temperature[b]))) return fail(B200_INVALID_ARGUMENT, row + "temperature must be finite and not negative");
-        if (!(uniform[b] >= 0.0f && uniform[b] < 1.0f)) return fail(B200_INVALID_ARGUMENT, row + "uniform must be in [0, 1)");
-        if ((top_p && std::isnan(top_p[b])) || (min_p && std::isnan(min_p[b]))) return fail(B200_INVALID_ARGUMENT, row + "top_p and min_p must not be NaN");
+        const char* what = nullptr;
+        if (temperature && !(temperature[b] >= 0.0f && std::isfinite(temperature[b]))) what = "temperature must be finite and not negative";
+        else if (!(uniform[b] >= 0.0f && uniform[b] < 1.0f)) what = "uniform must be in [0, 1)";
+        else if ((top_p && std::isnan(top_p[b])) || (min_p && std::isnan(min_p[b]))) what = "top_p and min_p must not be NaN";
+        if (what) return fail(B200_INVALID_ARGUMENT, "decoder_sample: row " + std::to_string(b) + ": " + what);
     }
     cudaStream_t s = d->ctx->stream;
     if (d->sample_copy_pending) CU_TRY(cudaEventSynchronize(d->sample_copied));      // read when the copy executes, as the ids are

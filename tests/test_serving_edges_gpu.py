@@ -409,7 +409,7 @@ def test_decoder_draws_for_the_rows_that_took_part(be):
                 if active[r]:
                     want = sample_ref(logits[r], float(np.float32(temperature[r])), 0, float(np.float32(top_p[r])), 0.0, float(np.float32(uniform[r])))[0]
                 assert got[r] == want
-        with pytest.raises(BackendError):
+        with pytest.raises(BackendError, match="row 1: uniform"):
             dec.sample([0.1, nan, 0.1])                       # the row that takes part
         step_rows(dec, None, [1, 1, 1])
         with pytest.raises(BackendError):
