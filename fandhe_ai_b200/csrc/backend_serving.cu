@@ -204,8 +204,8 @@ int32_t b200_rope_paged_kv_append(b200_ctx* ctx, const b200_buf* qkv, size_t qkv
     const uint64_t table = a->n_positions * (a->rotary_dim / 2) * 4;
     if (int32_t st = check_aligned(ctx, op, qkv, qkv_off, span_bytes(a->rows, r.sh.row_stride, width, item), "qkv", 16)) return st;
     if (int32_t st = check_aligned(ctx, op, q_out, q_out_off, a->rows * heads * item, "q_out", 16)) return st;
-    if (int32_t st = check_aligned(ctx, op, cos_table, 0, table, "cos_table", 16)) return st;
-    if (int32_t st = check_aligned(ctx, op, sin_table, 0, table, "sin_table", 16)) return st;
+    if (int32_t st = check_aligned(ctx, op, cos_table, 0, table, "cos_table", 16, table == 0)) return st;
+    if (int32_t st = check_aligned(ctx, op, sin_table, 0, table, "sin_table", 16, table == 0)) return st;
     if (int32_t st = check_aligned(ctx, op, positions, 0, a->rows * 4, "positions", 4, true)) return st;
     if (int32_t st = check_index_buffers(ctx, op, r, a->batch, block_tables, q_starts, seq_lens)) return st;
     if (int32_t st = check_aligned(ctx, op, k_pool, 0, r.pool_bytes, "k_pool", 16)) return st;

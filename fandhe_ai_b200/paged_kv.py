@@ -219,13 +219,14 @@ def validate_rope_append(args: RopeAppendArgs) -> None:
     check(lib().b200_validate_rope_append(args._c))
 
 
-def rope_paged_kv_append(be: Backend, qkv: DeviceBuffer, cos_table: DeviceBuffer, sin_table: DeviceBuffer,
+def rope_paged_kv_append(be: Backend, qkv: DeviceBuffer, cos_table: DeviceBuffer | None, sin_table: DeviceBuffer | None,
                          block_tables: DeviceBuffer, q_starts: DeviceBuffer, seq_lens: DeviceBuffer, k_pool: DeviceBuffer,
                          v_pool: DeviceBuffer, args: RopeAppendArgs, q_out: DeviceBuffer,
                          positions: DeviceBuffer | None = None, qkv_off: int = 0, q_out_off: int = 0) -> DeviceBuffer:
     """Appends the keys and values of a ragged batch (rows of [q | k | v]) to the paged cache, q and k rotated to their
-    positions; returns q_out, the rotated queries."""
-    check(lib().b200_rope_paged_kv_append(be._ctx, qkv.handle, qkv_off, cos_table.handle, sin_table.handle,
+    positions; returns q_out, the rotated queries.  No tables are needed without rotation."""
+    check(lib().b200_rope_paged_kv_append(be._ctx, qkv.handle, qkv_off, cos_table.handle if cos_table is not None else None,
+                                          sin_table.handle if sin_table is not None else None,
                                           positions.handle if positions is not None else None, block_tables.handle,
                                           q_starts.handle, seq_lens.handle, k_pool.handle, v_pool.handle, args._c,
                                           q_out.handle, q_out_off))

@@ -372,7 +372,8 @@ typedef struct b200_rope_append_args {
  * holds the q heads, then the k heads, then the v heads (the order of B200_W_QKV).  With the pair (a, b) at the angle of the
  * row's position: (a, b) -> (a cos - b sin, b cos + a sin), computed in f32 and rounded once to the target's type.  Keys and
  * values go to the pool row of the token's place in the cache; q_out gets the rotated queries as dense rows
- * [rows, num_heads * head_dim].  positions: u32 [rows] row of the cos / sin tables for each token, NULL: its place in the
+ * [rows, num_heads * head_dim].  cos_table and sin_table: f32 [n_positions, rotary_dim / 2], NULL where that is empty (no
+ * rotation).  positions: u32 [rows] row of the cos / sin tables for each token, NULL: its place in the
  * cache.  q_out must not overlap qkv.  Two tokens with the same cache place (a block shared by two sequences) leave either. */
 int32_t b200_rope_paged_kv_append(b200_ctx* ctx, const b200_buf* qkv, size_t qkv_off, const b200_buf* cos_table,
                                   const b200_buf* sin_table, const b200_buf* positions, const b200_buf* block_tables,

@@ -417,3 +417,21 @@ def test_decoder_draws_for_the_rows_that_took_part(be):
         assert (dec.sample([0.1, 0.1, 0.1]) >= 0).all()
     finally:
         dec.close()
+
+
+# ------------------------------------------------------------------------------------------ arguments
+
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_append_without_rotation_takes_no_tables(be, adjacent):
+    bt = Batch([3, 2], [20, 2], heads=4, kv_heads=1, dh=64, seed=5)
+    qkv = np.random.default_rng(6).standard_normal((5, 6 * 64)).astype(np.float32)
+    tables, st, sl = be.upload(bt.tables), be.upload(bt.q_starts), be.upload(bt.seq_lens)
+    kp, vp = be.upload(bt.pool_array(bt.k)), be.upload(bt.pool_array(bt.v))
+    layout = P.PagedKvLayout(bt.blocks, bt.block, 64, BF16)
+    for rotary, n_pos in ((0, 0), (0, 77)):
+        q = be.alloc_zeroed((5, 256))
+        P.rope_paged_kv_append(be, be.upload(qkv), None, None, tables, st, sl, kp, vp, P.RopeAppendArgs(layout, 2, 5, 4, 1, bt.width, rotary, n_pos, adjacent), q)
+        assert np.array_equal(q.numpy(), qkv[:, :256])
+    with pytest.raises(BackendError) as e:
+        P.rope_paged_kv_append(be, be.upload(qkv), None, None, tables, st, sl, kp, vp, P.RopeAppendArgs(layout, 2, 5, 4, 1, bt.width, 64, 32, adjacent), q)
+    assert e.value.kind == "InvalidArgument"
