@@ -29,6 +29,13 @@ int32_t check_aligned(const b200_ctx* ctx, const char* op, const b200_buf* buf, 
     return B200_OK;
 }
 
+// Do two ranges of the caller's memory share a byte?  (Handles of imported memory may name the same one.)
+bool overlap(const b200_buf* a, size_t a_off, uint64_t a_bytes, const b200_buf* b, size_t b_off, uint64_t b_bytes) {
+    if (!a || !b || a_bytes == 0 || b_bytes == 0) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a->ptr) + a_off, y = reinterpret_cast<uintptr_t>(b->ptr) + b_off;
+    return x < y + b_bytes && y < x + a_bytes;
+}
+
 // The part of the arguments that append and attention share
 struct Ragged {
     RaggedShape sh;
@@ -211,6 +218,13 @@ int32_t b200_rope_paged_kv_append(b200_ctx* ctx, const b200_buf* qkv, size_t qkv
     if (int32_t st = check_aligned(ctx, op, k_pool, 0, r.pool_bytes, "k_pool", 16)) return st;
     if (int32_t st = check_aligned(ctx, op, v_pool, 0, r.pool_bytes, "v_pool", 16)) return st;
     if (a->rows == 0 || a->batch == 0) return B200_OK;
+    const uint64_t in_bytes = span_bytes(a->rows, r.sh.row_stride, width, item), out_bytes = a->rows * heads * item;
+    if (overlap(qkv, qkv_off, in_bytes, q_out, q_out_off, out_bytes)) return bad(op, "q_out overlaps qkv");
+    for (const b200_buf* pool : {k_pool, v_pool}) {
+        if (overlap(pool, 0, r.pool_bytes, qkv, qkv_off, in_bytes) || overlap(pool, 0, r.pool_bytes, q_out, q_out_off, out_bytes))
+            return bad(op, "a pool overlaps qkv or q_out");
+    }
+    if (overlap(k_pool, 0, r.pool_bytes, v_pool, 0, r.pool_bytes)) return bad(op, "k_pool overlaps v_pool");
     if (int32_t st = set_device(ctx)) return st;
     const RopeShape rope = {int(a->rotary_dim), a->adjacent_pairs != 0, int64_t(a->n_positions)};
     const cudaError_t e = rope_paged_kv_append(
@@ -248,6 +262,15 @@ int32_t b200_paged_chunk_attention(b200_ctx* ctx, const b200_buf* q, size_t q_of
     const size_t need = paged_chunk_workspace_bytes(r.sh, a->io_dtype == B200_BF16, a->layout.dtype == B200_BF16, ctx->sm_count);
     if (int32_t st = check_aligned(ctx, op, workspace, 0, need, "workspace", 16, need == 0)) return st;
     if (a->rows == 0 || a->batch == 0 || a->max_q_len == 0) return B200_OK;
+    // Results in the queries' own places are fine: a row and head is read by the blocks that write it, or before the join does.
+    const uint64_t in_bytes = span_bytes(a->rows, r.sh.row_stride, width, item), out_bytes = a->rows * width * item;
+    const bool in_place = static_cast<uint8_t*>(q->ptr) + q_off == static_cast<uint8_t*>(out->ptr) + out_off && uint64_t(r.sh.row_stride) == width;
+    if (!in_place && overlap(q, q_off, in_bytes, out, out_off, out_bytes)) return bad(op, "out overlaps q (it may only be q itself, with dense rows)");
+    for (const b200_buf* pool : {k_pool, v_pool})
+        if (overlap(pool, 0, r.pool_bytes, out, out_off, out_bytes) || overlap(pool, 0, r.pool_bytes, workspace, 0, need))
+            return bad(op, "a pool overlaps out or the workspace");
+    if (overlap(workspace, 0, need, q, q_off, in_bytes) || overlap(workspace, 0, need, out, out_off, out_bytes))
+        return bad(op, "the workspace overlaps q or out");
     if (int32_t st = set_device(ctx)) return st;
     const cudaError_t e = paged_chunk_attention(
         r.sh, buf_ptr<const uint8_t>(q, q_off), a->io_dtype == B200_BF16, k_pool->ptr, v_pool->ptr, a->layout.dtype == B200_BF16,

@@ -374,7 +374,7 @@ typedef struct b200_rope_append_args {
  * values go to the pool row of the token's place in the cache; q_out gets the rotated queries as dense rows
  * [rows, num_heads * head_dim].  cos_table and sin_table: f32 [n_positions, rotary_dim / 2], NULL where that is empty (no
  * rotation).  positions: u32 [rows] row of the cos / sin tables for each token, NULL: its place in the
- * cache.  q_out must not overlap qkv.  Two tokens with the same cache place (a block shared by two sequences) leave either. */
+ * cache.  Overlaps of qkv, q_out and the pools are refused.  Two tokens with the same cache place (a block shared by two sequences) leave either. */
 int32_t b200_rope_paged_kv_append(b200_ctx* ctx, const b200_buf* qkv, size_t qkv_off, const b200_buf* cos_table,
                                   const b200_buf* sin_table, const b200_buf* positions, const b200_buf* block_tables,
                                   const b200_buf* q_starts, const b200_buf* seq_lens, b200_buf* k_pool, b200_buf* v_pool,
@@ -406,7 +406,8 @@ int32_t b200_paged_chunk_workspace(b200_ctx* ctx, const b200_paged_chunk_args* a
 
 /* Attention of every new token over its sequence's cached tokens up to and including itself (their keys and values are in the
  * cache already): out[r, h, :] = softmax_j(scale * q_r . k_j) . v_j over j <= seq_len - new + i for the i-th new token.
- * out is dense [rows, num_heads * head_dim].  What the cache holds beyond a token's reach does not matter, NaN and
+ * out is dense [rows, num_heads * head_dim]; it may be q itself where q's rows are dense too, and any other overlap of q, out, the
+ * workspace and a pool that is written over is refused.  What the cache holds beyond a token's reach does not matter, NaN and
  * infinities included.  With io_dtype F32 the products are exact to f32 (q and the softmax weights enter the bf16 tensor
  * cores as sums of bf16 terms); with BF16 the softmax weights are rounded to bf16 for the second product.  Accumulators,
  * maxima and sums are f32.  The contents of the workspace need not be kept between calls; calls that may overlap (other

@@ -8,7 +8,7 @@ from fandhe_ai_b200 import paged_kv as P
 from fandhe_ai_b200.decoder import SampleArgs, sample_tokens
 
 from serving_ref import Batch, attention_ref, bf16, sample_ref
-from test_serving_gpu import check_attention, check_draw, draw, make_small_decoder, run_attention
+from test_serving_gpu import check_attention, check_draw, down, draw, layout_of, make_small_decoder, run_attention, up
 
 pytestmark = pytest.mark.gpu
 
@@ -435,3 +435,50 @@ def test_append_without_rotation_takes_no_tables(be, adjacent):
     with pytest.raises(BackendError) as e:
         P.rope_paged_kv_append(be, be.upload(qkv), None, None, tables, st, sl, kp, vp, P.RopeAppendArgs(layout, 2, 5, 4, 1, bt.width, 64, 32, adjacent), q)
     assert e.value.kind == "InvalidArgument"
+
+
+def test_overlapping_memory_is_refused(be):
+    bt = Batch([4, 4], [100, 60], heads=4, kv_heads=2, seed=16)
+    tables, st, sl = be.upload(bt.tables), be.upload(bt.q_starts), be.upload(bt.seq_lens)
+    kp, vp = be.upload(bt.pool_array(bt.k)), be.upload(bt.pool_array(bt.v))
+    layout = P.PagedKvLayout(bt.blocks, bt.block, 256, BF16)
+    args = P.PagedChunkArgs(layout, 2, 8, 4, 100, 4, 2, bt.width, 0.1)
+    need = P.paged_chunk_workspace(be, args)
+    big = be.alloc_zeroed((1 << 20,))
+    row = 512 * 4
+
+    def refused(call, *a, **kw):
+        with pytest.raises(BackendError) as e:
+            call(be, *a, **kw)
+        assert e.value.kind == "InvalidArgument" and "overlap" in e.value.message
+
+    ws, q, out = be.alloc_zeroed((max(16, need),), np.uint8), be.alloc_zeroed((8, 512)), be.alloc_zeroed((8, 512))
+    refused(P.paged_chunk_attention, big, kp, vp, tables, st, sl, args, ws, big, q_off=0, out_off=row)
+    wide = P.PagedChunkArgs(layout, 2, 8, 4, 100, 4, 2, bt.width, 0.1, q_stride=516)
+    refused(P.paged_chunk_attention, big, kp, vp, tables, st, sl, wide, ws, big)                # the same start, rows apart
+    refused(P.paged_chunk_attention, q, kp, big, tables, st, sl, args, ws, big, out_off=0)
+    if need:
+        refused(P.paged_chunk_attention, big, kp, vp, tables, st, sl, args, big, out)
+        refused(P.paged_chunk_attention, q, kp, vp, tables, st, sl, args, big, big, out_off=16)
+    cos, sin = (be.upload(x) for x in P.rope_table(1e4, 128, 200))
+    ra = P.RopeAppendArgs(layout, 2, 8, 4, 2, bt.width, 128, 200)
+    refused(P.rope_paged_kv_append, big, cos, sin, tables, st, sl, kp, vp, ra, big, q_out_off=7 * 1024 * 4)
+    refused(P.rope_paged_kv_append, big, cos, sin, tables, st, sl, big, vp, ra, q)
+    refused(P.rope_paged_kv_append, be.alloc_zeroed((8, 1024)), cos, sin, tables, st, sl, kp, kp, ra, q)
+    refused(P.rope_paged_kv_append, be.alloc_zeroed((8, 1024)), cos, sin, tables, st, sl, kp, big, ra, big)
+    assert not be.poisoned
+
+
+@pytest.mark.parametrize("io_bf16", [False, True])
+@pytest.mark.parametrize("case", FORMS)
+def test_attention_in_place(be, case, io_bf16):
+    bt = Batch(seed=60, pad_rows=2, **case)
+    q = bf16(bt.q) if io_bf16 else bt.q
+    want = run_attention(be, bt, q, io_bf16, 0.1)
+    both = up(be, q, io_bf16)
+    args = P.PagedChunkArgs(layout_of(bt), bt.batch, bt.rows, max(bt.new), max(bt.total), bt.heads, bt.kv_heads, bt.width, 0.1, BF16 if io_bf16 else F32)
+    ws = be.alloc_zeroed((max(16, P.paged_chunk_workspace(be, args)),), np.uint8)
+    tables, st, sl = be.upload(bt.tables), be.upload(bt.q_starts), be.upload(bt.seq_lens)
+    P.paged_chunk_attention(be, both, be.upload(bt.pool_array(bt.k)), be.upload(bt.pool_array(bt.v)), tables, st, sl, args, ws, both)
+    got, n = down(both, q.shape, io_bf16), bt.rows - 2
+    assert np.array_equal(got[:n], want[:n]) and np.array_equal(got[n:], q[n:])
