@@ -482,3 +482,97 @@ def test_attention_in_place(be, case, io_bf16):
     P.paged_chunk_attention(be, both, be.upload(bt.pool_array(bt.k)), be.upload(bt.pool_array(bt.v)), tables, st, sl, args, ws, both)
     got, n = down(both, q.shape, io_bf16), bt.rows - 2
     assert np.array_equal(got[:n], want[:n]) and np.array_equal(got[n:], q[n:])
+
+
+# ------------------------------------------------------------------------------------------ what only a small part of a number carries
+
+# few rows, at most 32 rows (the three terms share the accumulator rows), more rows, keys shared out; heads of 64 and 128
+TERMS = [dict(tokens=t, dh=dh, kv_heads=kv, group=g, total=n) for dh in (64, 128)
+         for t, kv, g, n in ((2, 2, 4, 300), (1, 1, 8, 3000), (7, 2, 4, 300), (30, 2, 1, 290), (33, 2, 4, 400), (100, 1, 1, 300), (25, 2, 4, 2500))]
+
+
+def weighted_pairs(case, x, at):
+    """Sequences in which the keys at[b] (score 0, V 0) and at[b] + 1 (score -x[b], V 1) are the only ones with a weight."""
+    n = len(x)
+    bt = Batch([case["tokens"]] * n, [case["total"]] * n, heads=case["kv_heads"] * case["group"], kv_heads=case["kv_heads"], dh=case["dh"], seed=70)
+    bt.k[:], bt.v[:], bt.q[:] = 0.0, 0.0, 0.0
+    bt.q[:, ::bt.dh] = 1.0
+    bt.k[..., ::bt.dh] = -1.0e4
+    for b in range(n):
+        blk, off = bt.places(b)
+        bt.k[blk[at[b]], off[at[b]]] = 0.0
+        bt.k[blk[at[b] + 1], off[at[b] + 1], ::bt.dh] = -x[b]
+        bt.v[blk[at[b] + 1], off[at[b] + 1]] = 1.0
+    return bt
+
+
+@pytest.mark.parametrize("case", TERMS)
+def test_attention_f32_weights_keep_all_their_bits(be, case):
+    """out = w / (1 + w), w = e^-x: a weight cut to 16 bits is off by up to 2^-15 of it, which the bound does not allow.
+
+    The bound, relative to out.  The argument of the exponential: c and its product round (2 2^-24 of |x| log2 e), times ln 2, twice where a
+    partial maximum is scaled down: |x| 2^-22; the exponentials 2^-22 each, two: 2^-21; doubled, since out has w above and below.
+    Then the sum, its reciprocal and the product (3 2^-24), and the accumulator, cut at each of its three terms (3 2^-23)."""
+    first = case["total"] - case["tokens"]
+    at = [p for p in (0, 3, 38, 62, 70, 94, 100, 126, 130, 165, 200, 228, 260) if p + 1 < first]
+    rng = np.random.default_rng(71)
+    x = bf16(rng.uniform(0.1, 3.5, 4 * len(at)).astype(np.float32))
+    bt = weighted_pairs(case, x, at * 4)
+    got = run_attention(be, bt, bt.q, False, 1.0)
+    w = np.exp(-x.astype(np.float64))
+    want = np.repeat(w / (1 + w), case["tokens"])[:, None]
+    lim = want * (2 * (np.repeat(x, case["tokens"])[:, None] * 2.0 ** -22 + 2.0 ** -21) + 3 * 2.0 ** -24 + 3 * 2.0 ** -23)
+    err = np.abs(got - want)
+    # the test itself: weights without their third term would not pass
+    w16 = (w.astype(np.float32).view(np.uint32) & 0xFFFF0000).view(np.float32).astype(np.float64)
+    rest = (w.astype(np.float32) - w16).astype(np.float32)
+    cut = w16 + (rest.view(np.uint32) & 0xFFFF0000).view(np.float32)
+    assert (np.abs(cut / (1 + w) - w / (1 + w)) > 2 * lim[::case["tokens"], 0]).any()
+    assert (err <= lim).all(), f"off by {(err / want).max():.3g}, allowed {(lim / want)[np.unravel_index(np.argmax(err / want), err.shape)[0], 0]:.3g}"
+
+
+@pytest.mark.parametrize("case", TERMS)
+def test_attention_f32_queries_keep_all_their_bits(be, case):
+    """A score of 128 2^12 (q0 - q1) = +-1.5 that stands in the last bits of q0 alone: q0 = 1 + 2^-10 + d, q1 = 1 + 2^-10, d = +-0.75 2^-18.
+
+    The products cancel at 2^12 in an accumulator that keeps 2^-23 of its largest addend; two cuts (the first element's product and
+    the second's) are 2 2^-11, times the scale 0.125 in the score, e^0.125 - 1 in a weight, above and below: 0.29 of out.
+    Without the third term the score is 0 and out is off by 1 - e^-1.5 = 0.78 of it, or e^1.5 - 1."""
+    n = 3
+    bt = Batch([case["tokens"]] * n, [case["total"]] * n, heads=case["kv_heads"] * case["group"], kv_heads=case["kv_heads"], dh=case["dh"], seed=72)
+    bt.k[:], bt.v[:], bt.q[:] = 0.0, 0.0, 0.0
+    d = np.where(np.arange(bt.rows) % 2 == 0, 1.0, -1.0) * 0.75 * 2.0 ** -18
+    bt.q[:, 0::bt.dh] = (1 + 2.0 ** -10 + d)[:, None]
+    bt.q[:, 1::bt.dh] = 1 + 2.0 ** -10
+    for b, at in enumerate((0, 60, case["total"] - case["tokens"] - 1)):
+        blk, off = bt.places(b)
+        bt.k[blk[at], off[at], 0::bt.dh], bt.k[blk[at], off[at], 1::bt.dh] = 2.0 ** 12, -2.0 ** 12
+        bt.v[blk[at], off[at]] = 1.0
+    got = run_attention(be, bt, bt.q, False, 128.0)
+    for row in range(bt.rows):
+        see = case["total"] - case["tokens"] + 1 + row % case["tokens"]
+        e = np.exp(128.0 * 2.0 ** 12 * d[row])
+        want = e / (e + see - 1)
+        assert (np.abs(got[row] - want) <= 0.29 * want).all()
+
+
+@pytest.mark.parametrize("io_bf16", [False, True])
+@pytest.mark.parametrize("case", FORMS)
+def test_attention_a_token_sees_itself_and_not_the_next(be, case, io_bf16):
+    """The values of the new tokens grow by half from one to the next, so that a row's own key is a third of what it sums up: one key
+    too few or too many does not fit the bound of any form."""
+    bt = Batch(seed=73, **case)
+    for b in range(bt.batch):
+        blk, off = bt.places(b)
+        for i in range(bt.new[b]):
+            at = bt.total[b] - bt.new[b] + i
+            bt.v[blk[at], off[at]] = bf16(np.float32(300.0 * 1.5 ** i) * np.where(np.arange(bt.kv_heads * bt.dh) % 3 == 0, -1, 1).astype(np.float32))
+    check_attention(be, bt, io_bf16, scale=0.02)
+    # the test itself: the same rows with one key less are outside the bound
+    q = bf16(bt.q) if io_bf16 else bt.q
+    ref, bound = attention_ref(bt, q, 0.02, split_terms=not io_bf16)
+    blk, off = bt.places(0)
+    at = bt.total[0] - bt.new[0]
+    bt.v[blk[at], off[at]] = 0.0
+    less, _ = attention_ref(bt, q, 0.02, split_terms=not io_bf16)
+    assert (np.abs(less[0] - ref[0]) > 2 * bound[0] + 2.0 ** -7 * np.abs(ref[0])).all()
