@@ -558,13 +558,14 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     constexpr int kTerms = decltype(terms)::value, H = decltype(half)::value;
                     if (elect_one()) {
 #pragma unroll
-                        for (int term = 0; term < kTerms; ++term)
+                        for (int left = kTerms - 1; left >= 0; --left)      // the small terms first, as above
 #pragma unroll
                             for (int kk = 0; kk < kTcKeys / 16; ++kk) {
+                                const int term = left;
                                 constexpr int kFirst = F32 ? 4 : 6;            // products of 16 keys in the first part
                                 if ((kk < kFirst) != (H == 0)) continue;
                                 const uint32_t cols = kTerms == 3 ? weight_columns<D>(H, term) + (kk - H * kFirst) * 8 : kk * 8;
-                                umma_bf16_ts(d_o, d_s + cols, v_desc + ((kk * 2048) >> 4), kIdescO, term + kk > 0 ? 1u : keep);
+                                umma_bf16_ts(d_o, d_s + cols, v_desc + ((kk * 2048) >> 4), kIdescO, term < kTerms - 1 || kk > 0 ? 1u : keep);
                             }
                         if (H == 0 && kTerms == 3 && D == 128) tc5_commit(smem_u32(&sh.p_free[s]));
                         if (H == 1) {
