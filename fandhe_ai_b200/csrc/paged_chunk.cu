@@ -356,6 +356,8 @@ struct ChunkPlan {
     int chunk_tiles, max_chunks;
 };
 
+constexpr int kFewRows = 10;      // TcCfg<., true>::kTinyRows
+
 ChunkPlan plan_chunk(const RaggedShape& sh, int io_bf16, int kv_bf16, int sm_count) {
     ChunkPlan plan = {false, 0, 0, 1};
     const int item = io_bf16 ? 2 : 4;
@@ -368,14 +370,17 @@ ChunkPlan plan_chunk(const RaggedShape& sh, int io_bf16, int kv_bf16, int sm_cou
     const int64_t units = (by_len < by_rows ? by_len : by_rows) * sh.num_kv_heads;
     const int tiles = (sh.max_seq_len + kTcKeys - 1) / kTcKeys;
     // Key ranges per row: the number that makes the launch shortest when an item costs its key tiles plus about three tiles of
-    // start and finish, and the items are dealt out to the SMs in equal rounds.
-    int best = 1;
+    // start and finish, and the items are dealt out to the SMs in equal rounds.  The variant for few f32 rows has ranges of at most
+    // 6144 keys: its accumulators are cut at every addition (see the kernel), and nothing is put aside there.
+    const int longest = !io_bf16 && int64_t(sh.max_q_len) * group <= kFewRows ? 48 : tiles;
+    int best = 1, best_over = INT32_MAX;      // over: tiles beyond the longest range
     int64_t best_cost = INT64_MAX;
     for (int n = 1; n <= 64 && (n == 1 || tiles / n >= 2); ++n) {
-        const int per = (tiles + n - 1) / n, count = (tiles + per - 1) / per;
+        const int per = (tiles + n - 1) / n, count = (tiles + per - 1) / per, over = per > longest ? per - longest : 0;
         if (count > 1 && sh.rows * sh.num_q_heads * count * (sh.head_dim * 4 + 8) > (int64_t(512) << 20)) break;
         const int64_t cost = ((units * count + sm_count - 1) / sm_count) * (per + 3);
-        if (cost < best_cost) {
+        if (over < best_over || (over == best_over && cost < best_cost)) {
+            best_over = over;
             best_cost = cost;
             best = n;
         }
@@ -388,6 +393,8 @@ ChunkPlan plan_chunk(const RaggedShape& sh, int io_bf16, int kv_bf16, int sm_cou
     plan.tc5 = plan.items < 0x7FFFFFFF && of_32 < 0x7FFFFFFF && int64_t(sh.max_q_len) * group < 0x7FFFFFFF;
     return plan;
 }
+
+static_assert(TcCfg<64, true>::kTinyRows == kFewRows && TcCfg<128, true>::kTinyRows == kFewRows, "");
 
 template <int D, bool F32, bool TINY, typename T>
 cudaError_t launch_tc5_kind(const ChunkPlan& plan, const RaggedShape& sh, const void* q, const void* k_pool, const void* v_pool,

@@ -67,6 +67,7 @@ struct TcCfg {
     static constexpr int kSmem = kQBytes + kStages * kTileBytes + kTcBookBytes;
     static constexpr int kRows = F32 ? 128 : 256;                            // rows of an item
     static constexpr int kTinyRows = F32 ? 10 : 32;
+    static constexpr int kHold = 4, kHoldStack = 12;                         // f32: tiles of a slot after which O is put aside
 };
 
 struct TcShape {
@@ -524,7 +525,7 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 tc5_commit(smem_u32(&sh.empty[stage]));
                 if (split) tc5_commit(smem_u32(&sh.empty[stage]));
             };
-            for (int t = split ? s : 0; ok && t < n; t += step) {
+            for (int t = split ? s : 0, nth = 0; ok && t < n; t += step, ++nth) {
                 {
                     const uint32_t at = order.k(t), stage = at % kNst;
                     ok = wait(full_bar(at), full_parity(at));
@@ -552,7 +553,9 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 const uint32_t at = order.v(t), stage = at % kNst;
                 ok = wait(full_bar(at), full_parity(at));
                 const uint64_t v_desc = umma_desc_mn128(ring_addr + stage * Cfg::kTileBytes, kHalfBytes);
-                const uint32_t keep = t >= step;            // not the first product of this item
+                // not the first product of this item, nor the first after O was put aside
+                if (F32 && !TINY && nth == (stack ? Cfg::kHoldStack : Cfg::kHold)) nth = 0;
+                const uint32_t keep = nth > 0;
                 const bool last = t + step >= n;
                 auto multiply = [&](auto half, auto terms) {
                     constexpr int kTerms = decltype(terms)::value, H = decltype(half)::value;
@@ -772,6 +775,38 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
 
             float m = -INFINITY, l = 0.0f;
+            // f32 activations: the MMAs cut their sums towards zero, up to the last bit at each of a tile's additions (24 for three terms of 128
+            // keys), so an accumulator loses about 1.4e-8 of itself each time.  Every few tiles its row is therefore put aside, in local
+            // memory, and added up by f32 additions that round (512 tokens over 8000: off by 1.4e-5 without, 1.9e-6 with; 356 us
+            // without, 392 with).
+            // (The warps of few rows add two products of their own keys a tile; their key ranges are short enough, see plan_chunk.)
+            constexpr bool kHolds = F32 && !TINY;
+            const int hold = stack ? Cfg::kHoldStack : Cfg::kHold;
+            [[maybe_unused]] float held[kHolds ? D : 1], held_m = 0.0f;
+            [[maybe_unused]] int since = 0;
+            [[maybe_unused]] bool some = false;
+            // O and what was put aside (if anything was), 16 columns at a time, the next ones already on their way
+            [[maybe_unused]] auto add_held = [&](auto put) {
+                const float f = held_m == m ? 1.0f : ex2((held_m - m) * c);
+                float next[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) next[k] = some ? held[k] : 0.0f;
+#pragma unroll 1
+                for (int g = 0; g < D; g += 16) {
+                    float sum[16];
+                    uint32_t o[16];
+                    tmem_ld_32x16(t_o + g, o);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        sum[k] = next[k];
+                        if (some && g + 16 < D) next[k] = held[g + 16 + k];
+                    }
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) sum[k] = some ? fmaf(sum[k], f, __uint_as_float(o[k])) : __uint_as_float(o[k]);
+                    put(g, sum);
+                }
+            };
             const int masked_from = it.min_limit / kTcKeys - it.t0, step = split ? 2 : 1, nt = it.nt, k0 = it.t0 * kTcKeys;
             int done = 0;
             for (int t = split ? wg : 0; t < nt; t += step, ++done) {
@@ -788,6 +823,17 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     continue;
                 }
                 tc5_fence_after();
+                if constexpr (kHolds) {      // (the products before this one's scores are complete)
+                    if (since++ == hold) {
+                        add_held([&](int col, const float (&sum)[16]) {
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) held[col + k] = sum[k];
+                        });
+                        some = true;
+                        since = 1;
+                        held_m = m;
+                    }
+                }
                 const bool masked = t >= masked_from;                          // the same for all lanes, as the collective loads and stores need
                 const int visible = limit - k0 - t * kTcKeys;
                 // Running maximum; true when O was rescaled.  m may stay behind by 2^8 in the weight.
@@ -1053,6 +1099,17 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 tc5_fence_after();
             }
             if (!ok) break;
+            if constexpr (kHolds) {
+                if (some) {      // what was put aside comes back
+                    add_held([&](int col, const float (&sum)[16]) {
+                        uint32_t o[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(sum[k]);
+                        tmem_st_32x16(t_o + col, o);
+                    });
+                    tmem_st_wait();
+                }
+            }
 
             // ---- results.  Rows go through shared memory (the query tiles are done with), so that a warp writes whole rows:
             // row r of a staging area of W-element rows keeps its 16-byte piece j at piece j ^ (r & 7).

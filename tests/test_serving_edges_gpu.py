@@ -163,16 +163,21 @@ def test_stream_order_inside_a_captured_graph(be):
     sample_tokens(be, hx, SampleArgs(4, 5000), hu, hid, temperature=hu)
     assert hid.numpy().tolist() == [77] * 4
     del graph
-def test_measured_calls_are_ordered_with_the_callers_stream(be):
-    """perf/operators.py hands out tensors of torch: its calls wait for what the current stream has still to write, and work that
-    the caller puts behind them sees finished results - without a wait of the host in between."""
-    torch = pytest.importorskip("torch")
+def measured_cases():
     import importlib.util
     from pathlib import Path
 
     spec = importlib.util.spec_from_file_location("measured_cases", Path(__file__).resolve().parents[1] / "perf" / "operators.py")
     m = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(m)
+    return m
+
+
+def test_measured_calls_are_ordered_with_the_callers_stream(be):
+    """perf/operators.py hands out tensors of torch: its calls wait for what the current stream has still to write, and work that
+    the caller puts behind them sees finished results - without a wait of the host in between."""
+    torch = pytest.importorskip("torch")
+    m = measured_cases()
     m.own = True
     case = dict(op="attention", dtype="bf16", seqs=2, chunked=2, chunk_lo=900, chunk_hi=1000, step=1, prefix_lo=0, prefix_hi=0, lens=1,
                 heads=8, kv_heads=8, head_dim=128, block=16)
@@ -576,3 +581,17 @@ def test_attention_a_token_sees_itself_and_not_the_next(be, case, io_bf16):
     bt.v[blk[at], off[at]] = 0.0
     less, _ = attention_ref(bt, q, 0.02, split_terms=not io_bf16)
     assert (np.abs(less[0] - ref[0]) > 2 * bound[0] + 2.0 ** -7 * np.abs(ref[0])).all()
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("seqs,chunk,cached", [(2, 512, 600), (2, 512, 8000), (4, 300, 4000), (48, 1, 16000)])
+def test_attention_f32_error_does_not_grow_with_the_cache(dh, seqs, chunk, cached):
+    """The tensor cores cut a sum at each addition: by half a last place on average, 2^-24 of it at most, always towards zero, so the
+    parts add up.  An accumulator takes at most 96 additions before f32 additions go on with it, and a score 24 of its own size
+    (rms 1.5, which moves the weights as much): (96 + 1.5 24) 2^-24 of the result.  Half that many again for all that rounds."""
+    m = measured_cases()
+    m.own = True
+    case = dict(op="attention", dtype="f32", seqs=seqs, chunked=seqs, chunk_lo=chunk, chunk_hi=chunk, step=1, prefix_lo=cached, prefix_hi=cached,
+                lens=2, heads=32, kv_heads=8, head_dim=dh, block=16)
+    out, want = m.run(m.prepare(case, 3))["out"].double(), m.exact(case, 3)["out"]
+    assert float((out - want).norm() / want.norm()) <= 1.5 * (96 + 1.5 * 24) * 2.0 ** -24
