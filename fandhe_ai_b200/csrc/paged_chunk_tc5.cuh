@@ -11,7 +11,8 @@
 // While one slot is in its softmax, the tensor cores work for the other one.
 //
 //   S = Q K^T   tcgen05.mma, operands from shared memory (128-byte swizzle, K-major), 128 columns of tensor memory a slot
-//   P = 2^(S c - m c), c = scale log2 e; bf16, written over S
+//   P = 2^(S c - m c), c = scale log2 e; bf16, written over S (the MMA takes both operands in one type, and V is bf16; the sum l is of the
+//       f32 weights, so a result is off by the mean of their roundings, 2^-8 each at most, beside the rounding of its own)
 //   O += P V    tcgen05.mma, P from tensor memory, V from shared memory as it stands in the cache (MN-major), f32 accumulator
 // The running maximum m of a row is raised only when a new score exceeds it by more than 2^8 in the weight: until then the
 // weights are merely larger than one, and O need not be rescaled.
@@ -39,19 +40,20 @@
 // of rows that some query must not see are replaced by zero, and if there were any the epilogue adds them back to the rows that do see them
 // (as it does where a visible infinity met a weight of zero in some term or quarter).
 //
-// Measured on a B200 (us; 32 / 8 heads of 128 unless said otherwise): 2039 bf16 tokens over 30011 cached ones 1180 to 1225 (the
-// power cap decides), which is 846 to 878 TFLOP/s; four prompts of 2048 188 (731 TFLOP/s); one f32 token of each of 128 sequences
-// over 256 to 2048 184 (3.2 TB/s); four chunks of about 400 f32 tokens among 60 single ones 236; sixteen f32 prompts of 300 to
-// 1024, 12 heads of 64, 158; four drafted bf16 tokens of eight sequences 21.  Bound by the chain of a slot (about 3800 clocks a
-// tile where the products alone take 1024, two slots side by side) and, for short items, by their start and finish; not by HBM
-// and not by the tensor cores' rate.  What an item does once is kept short for that reason (prompts, step by step): code that runs once is not
+// Measured on a B200 (us; 32 / 8 heads of 128 unless said otherwise): 2039 bf16 tokens over 30011 cached ones 1185 to 1225 (the
+// power cap decides), which is 846 to 875 TFLOP/s; four prompts of 2048 187 to 198 (694 to 735 TFLOP/s); one f32 token of each of 128
+// sequences over 256 to 2048 184 (3.2 TB/s); four chunks of about 400 f32 tokens among 60 single ones 266; sixteen f32 prompts of 300 to
+// 1024, 12 heads of 64, 162; four drafted bf16 tokens of eight sequences 21.  Bound by the chain of a slot and, for short
+// items, by their start and finish; not by HBM and not by the tensor cores' rate: the long case takes 2.8 us a key tile and SM,
+// both slots together, which is 4700 clocks at its 1690 MHz, where the products of both take 2048 and their exponentials 2048.
+// What an item does once is kept short for that reason (prompts, step by step): code that runs once is not
 // unrolled, since the instruction cache shows (239 -> 213); bf16 queries go to shared memory by asynchronous copies (213 -> 196);
-// finished bf16 rows leave in one pass, staged as bf16 (196 -> 188).
+// finished bf16 rows leave in one pass, staged as bf16 (196 -> 188 in that run).
 
 constexpr int kTcSoftmaxWarps = 8;
-constexpr int kTcThreads = 32 * (kTcSoftmaxWarps + 4);
 // Registers a thread: 168 at launch (384 threads); the softmax threads hold a row of 128 scores and take 216, the other four warps
 // give theirs up: 256 x 216 + 128 x 72 = 384 x 168.
+constexpr int kTcThreads = 32 * (kTcSoftmaxWarps + 4);
 constexpr int kTcKeys = 128;               // keys of a tile
 constexpr int kTcBookBytes = 3 << 10;      // of shared memory, for everything but tiles
 constexpr int kTcItemSlots = 4;            // items known ahead
@@ -67,7 +69,7 @@ struct TcCfg {
     static constexpr int kSmem = kQBytes + kStages * kTileBytes + kTcBookBytes;
     static constexpr int kRows = F32 ? 128 : 256;                            // rows of an item
     static constexpr int kTinyRows = F32 ? 10 : 32;
-    static constexpr int kHold = 4, kHoldStack = 12;                         // f32: tiles of a slot after which O is put aside
+    static constexpr int kHold = 2, kHoldStack = 6;                          // f32: tiles of a slot after which O is put aside
 };
 
 struct TcShape {
@@ -776,9 +778,10 @@ paged_chunk_tc5_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
             float m = -INFINITY, l = 0.0f;
             // f32 activations: the MMAs cut their sums towards zero, up to the last bit at each of a tile's additions (24 for three terms of 128
-            // keys), so an accumulator loses about 1.4e-8 of itself each time.  Every few tiles its row is therefore put aside, in local
-            // memory, and added up by f32 additions that round (512 tokens over 8000: off by 1.4e-5 without, 1.9e-6 with; 356 us
-            // without, 392 with).
+            // keys), so an accumulator loses about 1.4e-8 of itself each time.  After 48 additions - two tiles, or six of a stacked item -
+            // its row is therefore put aside, in local memory, and added up by f32 additions that round.  512 tokens over 8000, in
+            // 1e-6 off and us: 13.9 and 356 without; 1.9 and 392 every four tiles, 1.5 and 406 every three, 1.1 and 434 every two, 0.7
+            // and 567 every tile; plain f32 operations 0.9.
             // (The warps of few rows add two products of their own keys a tile; their key ranges are short enough, see plan_chunk.)
             constexpr bool kHolds = F32 && !TINY;
             const int hold = stack ? Cfg::kHoldStack : Cfg::kHold;
