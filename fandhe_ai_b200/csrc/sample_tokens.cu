@@ -19,8 +19,8 @@
 // usually a few hundred) move to a list in index order, and what follows works on that.  A bin that holds more than kCandidates tokens (flat or heavily tied rows) is
 // resolved by bisection over the ordered pair (logit, index) instead.
 //
-// Measured on a B200: one row of 128256 f32 logits 25 us, 128 such rows with every filter 106 us, 512 rows of 32000 bf16 logits 60 us.
-// Bound by latency, not by HBM (whose share is 10 us of the 106): a row takes about 37 thousand clocks, of which 5 load it, 9 go
+// Measured on a B200: one row of 128256 f32 logits 25 us, 128 such rows with every filter 107 us, 512 rows of 32000 bf16 logits 60 us,
+// of 32768 62 us.  Bound by latency, not by HBM (whose share is 10 us of the 107): a row takes about 37 thousand clocks, of which 5 load it, 9 go
 // into the bins and the f64 sum, 9 into cluster barriers and 4 each into leaving tokens behind and ranking the border's bin.
 #include <cfloat>
 #include <type_traits>
