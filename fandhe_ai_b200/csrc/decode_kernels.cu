@@ -273,17 +273,18 @@ int grid_for(int64_t n, int threads) {
 }
 size_t row_smem(int n) { return 32 * sizeof(double) + static_cast<size_t>(n) * sizeof(float); }
 
-template <typename K>
-cudaError_t ensure_smem(K kernel, size_t bytes) {
+template <auto Kernel>
+cudaError_t ensure_smem(size_t bytes) {
     if (bytes <= 48 * 1024) return cudaSuccess;
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    static int configured[64] = {};
+    return ensure_dynamic_smem(Kernel, static_cast<int>(bytes), configured);
 }
 
 }  // namespace
 
 cudaError_t embed_norm_quant(const int* ids, const float* table, int vocab, int M, int d, const float* norm_w, float eps,
                              float* h, int8_t* xq, float* sx, uint32_t* err, cudaStream_t s) {
-    cudaError_t e = ensure_smem(embed_norm_quant_kernel, row_smem(d));
+    cudaError_t e = ensure_smem<embed_norm_quant_kernel>(row_smem(d));
     if (e != cudaSuccess) return e;
     embed_norm_quant_kernel<<<M, kRowThreads, row_smem(d), s>>>(ids, table, vocab, d, norm_w, eps, h, xq, sx, err);
     return cudaGetLastError();
@@ -291,7 +292,7 @@ cudaError_t embed_norm_quant(const int* ids, const float* table, int vocab, int 
 cudaError_t resid_norm_quant(const int* raw, int splits, int M, int d, const float* sx_in, const float* sw,
                              const float* pre, const float* norm_w, float eps, float* h, int8_t* xq, float* sx_out,
                              cudaStream_t s) {
-    cudaError_t e = ensure_smem(resid_norm_quant_kernel, row_smem(d));
+    cudaError_t e = ensure_smem<resid_norm_quant_kernel>(row_smem(d));
     if (e != cudaSuccess) return e;
     resid_norm_quant_kernel<<<M, kRowThreads, row_smem(d), s>>>(raw, splits, M, d, sx_in, sw, pre, norm_w, eps, h, xq,
                                                                sx_out);
@@ -304,7 +305,7 @@ cudaError_t dequant_planes(const int* raw, int splits, int M, int N, const float
 }
 cudaError_t gate_quant(const int* raw, int splits, int M, int F, const float* sx_in, const float* sw, int8_t* xq,
                        float* sx_out, cudaStream_t s) {
-    cudaError_t e = ensure_smem(gate_quant_kernel, row_smem(F));
+    cudaError_t e = ensure_smem<gate_quant_kernel>(row_smem(F));
     if (e != cudaSuccess) return e;
     gate_quant_kernel<<<M, kRowThreads, row_smem(F), s>>>(raw, splits, M, F, sx_in, sw, xq, sx_out);
     return cudaGetLastError();
