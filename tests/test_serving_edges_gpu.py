@@ -317,7 +317,8 @@ def check_non_finite(be, bt, io_bf16, scale, places):
             if key <= first + i:
                 for h in range(g):
                     at = h * bt.dh + e
-                    want[i, at] = value + (want[i, at] if not np.isfinite(want[i, at]) else 0.0)
+                    with np.errstate(invalid="ignore"):      # inf - inf
+                        want[i, at] = value + (want[i, at] if not np.isfinite(want[i, at]) else 0.0)
     touched = ~np.isfinite(want)
     assert touched.any() and (np.abs(got - ref) <= bound + step * 1.001 * (np.abs(ref) + bound))[~touched].all()
     assert np.array_equal(got[touched], want[touched].astype(np.float32), equal_nan=True)
@@ -595,3 +596,72 @@ def test_attention_f32_error_does_not_grow_with_the_cache(dh, seqs, chunk, cache
                 lens=2, heads=32, kv_heads=8, head_dim=dh, block=16)
     out, want = m.run(m.prepare(case, 3))["out"].double(), m.exact(case, 3)["out"]
     assert float((out - want).norm() / want.norm()) <= 1.5 * (48 + 1.5 * 24) * 2.0 ** -24
+
+
+# ------------------------------------------------------------------------------------------ large and crowded
+
+@pytest.mark.parametrize("dh,kv_heads,pool_bf16", [(128, 8, True), (64, 16, True), (80, 8, True), (128, 4, False)])
+def test_pools_whose_offsets_pass_32_bits(be, dh, kv_heads, pool_bf16):
+    """The same batch in the first blocks of a pool and in its last ones, more than 2^31 elements further on."""
+    torch = pytest.importorskip("torch")
+    block, ekv = 16, dh * kv_heads
+    blocks = (1 << 31) // (block * ekv) + 200
+    dtype = torch.bfloat16 if pool_bf16 else torch.float32
+    bt = Batch([70, 1, 9], [500, 333, 9], heads=kv_heads * 2, kv_heads=kv_heads, dh=dh, pool_bf16=pool_bf16, seed=80)
+    kp, vp = (torch.empty(blocks, block, ekv, dtype=dtype, device="cuda") for _ in range(2))
+    assert kp.numel() > 1 << 31
+    qkv = torch.randn(bt.rows, (bt.heads + 2 * kv_heads) * dh, device="cuda")
+    cos, sin = (torch.from_numpy(x).cuda() for x in P.rope_table(1e4, dh, 600))
+    layout = P.PagedKvLayout(blocks, block, ekv, BF16 if pool_bf16 else F32)
+    aa = P.RopeAppendArgs(layout, bt.batch, bt.rows, bt.heads, kv_heads, bt.width, dh, 600)
+    ca = P.PagedChunkArgs(layout, bt.batch, bt.rows, max(bt.new), max(bt.total), bt.heads, kv_heads, bt.width, 0.1)
+    ws = torch.zeros(max(16, P.paged_chunk_workspace(be, ca)), dtype=torch.uint8, device="cuda")
+    starts, lens = (torch.from_numpy(x.astype(np.int32)).cuda() for x in (bt.q_starts, bt.seq_lens))
+    results = []
+    for shift in (0, blocks - bt.blocks):
+        t = torch.from_numpy(np.where(bt.tables == P.SENTINEL, -1, bt.tables.astype(np.int64) + shift).astype(np.int32)).cuda()
+        kp[shift:shift + bt.blocks] = torch.from_numpy(bt.k).cuda().to(dtype)
+        vp[shift:shift + bt.blocks] = torch.from_numpy(bt.v).cuda().to(dtype)
+        q, out = (torch.zeros(bt.rows, bt.heads * dh, device="cuda") for _ in range(2))
+        h = [be.import_tensor(x) for x in (qkv, cos, sin, t, starts, lens, kp, vp, q, out, ws)]
+        stream = torch.cuda.current_stream().cuda_stream
+        be.wait_stream(stream)
+        P.rope_paged_kv_append(be, *h[:8], aa, h[8])
+        P.paged_chunk_attention(be, h[8], h[6], h[7], h[3], h[4], h[5], ca, h[10], h[9])
+        be.stream_wait(stream)
+        results.append([x.clone() for x in (q, out, kp[shift:shift + bt.blocks], vp[shift:shift + bt.blocks])])
+        be.synchronize_device()
+        for x in h:
+            x.release()
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and bool(results[0][1].abs().sum(1).gt(0).all())
+    del kp, vp, results
+    torch.cuda.empty_cache()
+
+
+def test_contexts_side_by_side(be):
+    """Two contexts with streams and workspaces of their own: launches of all forms overlap on the GPU and answer as they do alone."""
+    other = Backend(0)
+    try:
+        jobs = []
+        for ctx, seed in ((be, 90), (other, 91)):
+            for kw, io_bf16 in ((dict(new=[1] * 60, total=[700] * 60), False), (dict(new=[300, 1, 5], total=[900, 2000, 60]), True),
+                                (dict(new=[90, 20], total=[400, 1500], dh=64, heads=4, kv_heads=4), False)):
+                bt = Batch(seed=seed, **kw)
+                q = bf16(bt.q) if io_bf16 else bt.q
+                want = run_attention(ctx, bt, q, io_bf16, 0.1)
+                args = P.PagedChunkArgs(layout_of(bt), bt.batch, bt.rows, max(bt.new), max(bt.total), bt.heads, bt.kv_heads, bt.width, 0.1,
+                                        BF16 if io_bf16 else F32)
+                ws = ctx.alloc_zeroed((max(16, P.paged_chunk_workspace(ctx, args)),), np.uint8)
+                operands = (up(ctx, q, io_bf16), up(ctx, bt.k, True), up(ctx, bt.v, True), ctx.upload(bt.tables), ctx.upload(bt.q_starts),
+                            ctx.upload(bt.seq_lens), args, ws)
+                jobs.append((ctx, want, io_bf16, operands, up(ctx, np.zeros_like(q), io_bf16)))
+        be.synchronize_device()
+        other.synchronize_device()
+        for _ in range(20):
+            for i in (0, 3, 1, 4, 2, 5):
+                ctx, _, _, operands, out = jobs[i]
+                P.paged_chunk_attention(ctx, *operands, out)
+        for ctx, want, io_bf16, _, out in jobs:
+            assert np.array_equal(down(out, want.shape, io_bf16), want)
+    finally:
+        other.close()
